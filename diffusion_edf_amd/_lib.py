@@ -14,13 +14,15 @@ _LIB_PATH = os.environ.get("DEDF_LIB") or os.path.join(os.path.dirname(os.path.a
 MAX_SCALES = 8
 
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_RUNTIME = 0, 1, 2, 3
-ABI_VERSION = 6          # DEDF_ABI_VERSION of include/dedf.h this binding mirrors
+ABI_VERSION = 7          # DEDF_ABI_VERSION of include/dedf.h this binding mirrors
 
 SYMBOLS = [
     "dedf_version", "dedf_abi_version", "dedf_struct_size", "dedf_param_count", "dedf_param_name", "dedf_param_numel", "dedf_create", "dedf_destroy",
     "dedf_last_error", "dedf_set_key_clouds", "dedf_set_key_weights", "dedf_set_query", "dedf_score", "dedf_energy", "dedf_sample", "dedf_get_stats",
     "dedf_debug_enable", "dedf_debug_copy", "dedf_debug_packed", "dedf_profile_enable", "dedf_profile_read",
     "dedf_fps", "dedf_radius", "dedf_radius_scratch_bytes", "dedf_layer_forward", "dedf_linear_rs", "dedf_field", "dedf_keypoint_weight", "dedf_layer_defer_check", "dedf_layer_check", "dedf_layer_share_workspace", "dedf_set_radial_table", "dedf_linear_rs_lmax",
+    "dedf_edge_segments", "dedf_edge_attention", "dedf_edge_attention_backward", "dedf_edge_attention_scratch_bytes",
+    "dedf_norm_gate_residual", "dedf_norm_gate_residual_backward", "dedf_norm_scratch_bytes", "dedf_channel_dropout",
 ]
 
 
@@ -48,6 +50,20 @@ class DedfStats(C.Structure):
 
 class DedfProfile(C.Structure):
     _fields_ = [("n_evals", C.c_int64), ("n_edges", C.c_int64), ("n_dst", C.c_int64), ("ms", C.c_double * 6)]
+
+
+class DedfEdgeAttn(C.Structure):
+    _fields_ = [("n_edges", C.c_int64), ("n_dst", C.c_int), ("heads", C.c_int), ("k", C.c_int), ("d", C.c_int), ("type", C.c_int), ("n_buckets", C.c_int),
+                ("alpha", C.c_void_p), ("alpha_stride", C.c_int64), ("value", C.c_void_p), ("value_stride", C.c_int64), ("alpha_dot", C.c_void_p),
+                ("dst", C.c_void_p), ("rowptr", C.c_void_p), ("edge_logits", C.c_void_p), ("edge_length", C.c_void_p),
+                ("bias_boundaries", C.c_void_p), ("bias_table", C.c_void_p), ("dropout", C.c_double), ("rng", C.c_void_p)]
+
+
+class DedfNorm(C.Structure):
+    _fields_ = [("type", C.c_int), ("n_rows", C.c_int), ("n_blocks", C.c_int), ("groups", C.c_int), ("mul", C.c_int * 4), ("degree", C.c_int * 4),
+                ("x", C.c_void_p), ("y", C.c_void_p), ("gate", C.c_void_p), ("gate_f", C.c_int), ("scale", C.c_float), ("eps", C.c_float),
+                ("post_weight", C.c_void_p), ("post_bias", C.c_void_p), ("next_weight", C.c_void_p), ("next_bias", C.c_void_p),
+                ("dropout", C.c_double), ("rng", C.c_void_p)]
 
 
 PROF_CLASSES = ["pose_time", "neighbors", "edge", "aggregate", "node", "reduce"]
@@ -78,7 +94,7 @@ def load() -> C.CDLL:
     lib.dedf_struct_size.argtypes = [C.c_int]; lib.dedf_struct_size.restype = C.c_size_t
     if lib.dedf_abi_version() != ABI_VERSION:
         raise RuntimeError(f"{_LIB_PATH} has ABI version {lib.dedf_abi_version()}, this binding mirrors {ABI_VERSION}; rebuild the library")
-    for which, cls in enumerate((DedfConfig, DedfSchedule, DedfStats, DedfProfile)):
+    for which, cls in enumerate((DedfConfig, DedfSchedule, DedfStats, DedfProfile, DedfEdgeAttn, DedfNorm)):
         if lib.dedf_struct_size(which) != C.sizeof(cls):
             raise RuntimeError(f"{cls.__name__}: the library's struct has {lib.dedf_struct_size(which)} bytes, the ctypes mirror {C.sizeof(cls)}")
     lib.dedf_param_count.argtypes = [P(DedfConfig)]; lib.dedf_param_count.restype = C.c_int
@@ -121,6 +137,18 @@ def load() -> C.CDLL:
     lib.dedf_debug_packed.argtypes = [C.c_void_p, C.c_char_p, P(P(C.c_float)), P(C.c_size_t)]; lib.dedf_debug_packed.restype = C.c_int
     lib.dedf_profile_enable.argtypes = [C.c_void_p, C.c_int]; lib.dedf_profile_enable.restype = C.c_int
     lib.dedf_profile_read.argtypes = [C.c_void_p, P(DedfProfile)]; lib.dedf_profile_read.restype = C.c_int
+    V = C.c_void_p
+    lib.dedf_edge_segments.argtypes = [V, C.c_int64, C.c_int, V, V, V, V]; lib.dedf_edge_segments.restype = C.c_int
+    lib.dedf_edge_attention_scratch_bytes.argtypes = [P(DedfEdgeAttn), C.c_int]; lib.dedf_edge_attention_scratch_bytes.restype = C.c_size_t
+    lib.dedf_edge_attention.argtypes = [P(DedfEdgeAttn), V, V, V, V, V, C.c_size_t, V]; lib.dedf_edge_attention.restype = C.c_int
+    lib.dedf_edge_attention_backward.argtypes = [P(DedfEdgeAttn), V, V, V, V, V, V, V, V, V, C.c_size_t, V]
+    lib.dedf_edge_attention_backward.restype = C.c_int
+    lib.dedf_norm_gate_residual.argtypes = [P(DedfNorm), V, V, V, V]; lib.dedf_norm_gate_residual.restype = C.c_int
+    lib.dedf_norm_scratch_bytes.argtypes = [P(DedfNorm)]; lib.dedf_norm_scratch_bytes.restype = C.c_size_t
+    lib.dedf_norm_gate_residual_backward.argtypes = [P(DedfNorm), V, V, V, V, V, V, V, V, V, V, C.c_size_t, V]
+    lib.dedf_norm_gate_residual_backward.restype = C.c_int
+    lib.dedf_channel_dropout.argtypes = [C.c_int, C.c_int, C.c_int, P(C.c_int), P(C.c_int), V, C.c_double, V, V, V, V]
+    lib.dedf_channel_dropout.restype = C.c_int
     _lib = lib
     return lib
 

@@ -916,6 +916,8 @@ size_t dedf_struct_size(int which) {
         case 1: return sizeof(dedf_schedule);
         case 2: return sizeof(dedf_stats);
         case 3: return sizeof(dedf_profile);
+        case 4: return sizeof(dedf_edge_attn);
+        case 5: return sizeof(dedf_norm);
         default: return 0;
     }
 }

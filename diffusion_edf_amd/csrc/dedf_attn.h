@@ -1,0 +1,584 @@
+// Attention over a sorted edge list in its training form: the last part of GraphAttentionMLP2 (reference graph_attention.py:237-273) with gradients.
+//
+//   s[e,h] = sum_k act(a[e,h,k]) w[h,k]           act(x) = c x (0.2 + 0.8 sigma(x)), SmoothLeakyReLU(0.2) under normalize2mom
+//   t[e,h] = s + l[e] + T[bucket(len[e]), h]      bucket(x) = number of boundaries <= x
+//   p      = softmax of t over the edges of a destination; an edge and head with t = -inf takes no part
+//   P      = p m / (1 - q)                        m from Philox4x32-10, key = seed, counter = (edge, head / 4, offset), word head % 4
+//   out[n,h,:] = sum_e P v[e,h,:]
+// backward, from a row and head's maximum M and sum Z = sum exp(t - M) alone (the probabilities are recomputed, the mask is drawn again):
+//   p = exp(t - M) / Z   dP = m/(1-q) (dout . v)   delta = dout . out   dt = p (dP - delta)
+//   dv = P dout   dl = sum_h dt   dT[b,h] = sum dt   dw = sum_e dt act(a)   da = dt w act'(a)
+//
+// Both directions stream the per-edge rows once, so memory bandwidth bounds them.  A wave owns a contiguous RANGE of edges whatever the rows are:
+// the load is even for any degree distribution, from one edge per row to one row with every edge.  It walks its range in batches of 16 edges; a lane
+// holds 4 consecutive channels (a "quad") of every row, 16 rows in flight.  Rows that lie inside a range are finished by its wave; a row that
+// crosses ranges leaves one record per range (running maximum, sum, weighted sum), which k_attn_merge joins in order: no atomics, and the result
+// depends on the sizes alone.  Logits and maxima are held in 64 bits (with masks of a type's lowest value in edge_logits, t loses s in 32), and M and Z
+// apart: beside such a mask log Z would be lost in 64.
+#pragma once
+#include "dedf_philox.h"
+
+namespace dedf {
+namespace attn {
+
+constexpr int kBatch = 16;                 // edges per step of a wave
+constexpr int kWaves = 4;                  // waves per workgroup
+constexpr float kActNorm = 1.531320475574866f;
+constexpr double kLog2e = 1.4426950408889634;
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef double d2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+template <class T> struct Quad;
+template <> struct Quad<float> { typedef f4 type; };
+template <> struct Quad<_Float16> { typedef h4 type; };
+template <> struct Quad<__bf16> { typedef b4 type; };
+
+struct Args {
+    int64_t n_edges;
+    int n_dst, heads, k, d;
+    const void* a; const void* v; const float* w;
+    int64_t a_stride, v_stride;            // elements between the rows of two edges
+    int a_vec, v_vec;                      // rows start on whole quads (base, stride and width): one load per quad
+    const int* dst; const int* rowptr;
+    const float* logits; const float* length; const float* bounds; const float* table;
+    int n_buckets;
+    uint32_t threshold; float keep_scale;  // dropout: kept iff word >= threshold; threshold 0 = none
+    const int64_t* rng;
+    int range, n_waves;                    // edges per wave, waves
+};
+
+// quad of a row, as stored: one load where rows start on whole quads, else its `left` elements
+template <class T> __device__ inline typename Quad<T>::type whole_quad(const T* p) { return *(const typename Quad<T>::type*)p; }
+template <class T> __device__ inline typename Quad<T>::type part_quad(const T* p, int left) {
+    typename Quad<T>::type r = {(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) if (i < left) r[i] = p[i];
+    return r;
+}
+template <class T> __device__ inline void store_quad(T* p, f4 x, int vec, int left) {
+    if (vec) { *(typename Quad<T>::type*)p = typename Quad<T>::type{(T)x[0], (T)x[1], (T)x[2], (T)x[3]}; return; }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) if (i < left) p[i] = (T)x[i];
+}
+
+// LDS of one wave is written and read by its own lanes only: LDS operations of a wave complete in order, the compiler must keep that order
+__device__ inline void wave_sync() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
+
+// exp(x), x <= 0 (or -inf / NaN), to 1e-7 relative: the exponent is split into whole and fraction in 64 bits, so a long way below the maximum
+// loses nothing
+__device__ inline float exp_d(double x) {
+    if (x < -150.0) return 0.0f;
+    const double y = x * kLog2e, n = __builtin_rint(y);
+    return __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f((float)(y - n)), (int)n);
+}
+__device__ inline float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
+__device__ inline float act(float x) { return kActNorm * x * (0.2f + 0.8f * sigmoid(x)); }
+
+// number of boundaries <= x in a sorted list
+__device__ inline int bucket_of(const float* bounds, int n, float x) {
+    int lo = 0, hi = n;
+    while (lo < hi) { const int mid = (lo + hi) >> 1; if (bounds[mid] <= x) lo = mid + 1; else hi = mid; }
+    return lo;
+}
+
+// what both directions share: the wave's place, its LDS, the batch's per-edge values, the logits
+//   SUB: a quad is cut into 4 / SUB parts that each lie inside one head (SUB 4: head widths divisible by 4; 2: even; 1: any)
+//   WIDE: up to 4 quads per lane (value rows of up to 1 024 channels), feature rows of up to 256
+template <class T, int SUB, bool WIDE> struct Wave {
+    static constexpr int NV = WIDE ? 4 : 1, NA = 4, GA = WIDE ? 4 : 16;      // GA edges x feature quads fill NA loads of a wave
+    static constexpr int PARTS = 4 / SUB;
+    static constexpr int kPart = SUB == 1 ? 2048 : 1024;                     // floats of the partial-sum buffer
+    const Args& P;
+    int lane, wave, H, K, D, HK, HD, qa, qv, sub_a, n_sub_a;
+    uint32_t inv_h, inv_qa;
+    int64_t e0, e1;
+    float* part; double* t; float* keep; const float* w; const float* bounds; const float* table;
+    uint64_t seed, offset;
+    int64_t base; int n;                                                     // the batch: edges base .. base + n - 1, n <= 16
+    int* e_dst; int* e_bucket; float* e_logit;                               // its edges' destination, length bucket, edge logit
+
+    static __host__ __device__ size_t wave_bytes(int H) { return (size_t)kPart * 4 + (size_t)kBatch * (H + 1) * 12; }
+    static __host__ __device__ size_t shared_bytes(int HK, int H, int B) { return (((size_t)((HK + 3) & ~3) + (B ? B + (size_t)B * H : 0)) * 4 + 15) & ~(size_t)15; }
+
+    __device__ Wave(const Args& p, char* lds, size_t own_bytes) : P(p) {
+        lane = threadIdx.x & 63; wave = threadIdx.x >> 6;
+        H = p.heads; K = p.k; D = p.d; HK = H * K; HD = H * D;
+        qa = (HK + 3) >> 2; qv = (HD + 3) >> 2;
+        sub_a = (K & 3) ? 1 : 4; n_sub_a = K / sub_a;
+        inv_h = (65536 + H - 1) / H; inv_qa = (65536 + qa - 1) / qa;
+        float* s = (float*)lds;
+        const int hk4 = (HK + 3) & ~3, B = p.n_buckets;
+        for (int i = threadIdx.x; i < hk4; i += blockDim.x) s[i] = i < HK ? p.w[i] : 0.0f;
+        w = s; s += hk4;
+        for (int i = threadIdx.x; i < B - 1; i += blockDim.x) s[i] = p.bounds[i];
+        bounds = s; s += B;
+        for (int i = threadIdx.x; i < B * H; i += blockDim.x) s[i] = p.table[i];
+        table = s;
+        char* mine = lds + shared_bytes(HK, H, B) + wave * own_bytes;
+        t = (double*)mine; part = (float*)(mine + (size_t)kBatch * H * 8); keep = part + kPart;
+        e_logit = keep + kBatch * H; e_dst = (int*)(e_logit + kBatch); e_bucket = e_dst + kBatch;
+        seed = offset = 0;
+        if (p.threshold) { seed = (uint64_t)p.rng[0]; offset = (uint64_t)p.rng[1]; }
+        const int64_t id = (int64_t)blockIdx.x * kWaves + wave;
+        e0 = min(id * p.range, p.n_edges); e1 = min(e0 + p.range, p.n_edges);
+        __syncthreads();
+    }
+    __device__ void load_edges(int64_t b) {
+        base = b; n = (int)min((int64_t)kBatch, e1 - b);
+        if (lane < kBatch) {          // (places behind the last edge repeat it)
+            const int64_t e = b + min(lane, n - 1);
+            e_dst[lane] = P.dst[e];
+            e_logit[lane] = P.logits ? P.logits[e] : 0.0f;
+            e_bucket[lane] = P.n_buckets ? bucket_of(bounds, P.n_buckets - 1, P.length[e]) : 0;
+        }
+    }
+    // feature quad i of the edges e_first .. e_first + GA - 1: its edge (relative to e_first) and quad; false if there is none
+    __device__ bool a_place(int i, int e_first, int& e, int& q) const {
+        const int idx = i * 64 + lane;
+        e = (int)((idx * inv_qa) >> 16); q = idx - e * qa;
+        return e < GA && e_first + e < n;
+    }
+    // Loads go out together and unconditionally (places that do not exist repeat the batch's last edge or the row's last quad): a branch around each
+    // would make the wave wait for one row at a time.
+    typedef typename Quad<T>::type Raw;
+    __device__ void load_a(Raw (&a)[NA], int e_first) const {
+        const T* row = (const T*)P.a;
+        if (P.a_vec) {
+#pragma unroll
+            for (int i = 0; i < NA; ++i) {
+                int e, q;
+                a_place(i, e_first, e, q);
+                a[i] = whole_quad<T>(row + (base + min(e_first + e, n - 1)) * P.a_stride + 4 * q);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NA; ++i) {
+                int e, q;
+                a_place(i, e_first, e, q);
+                a[i] = part_quad<T>(row + (base + min(e_first + e, n - 1)) * P.a_stride + 4 * q, HK - 4 * q);
+            }
+        }
+    }
+    template <int G> __device__ void load_v(Raw (&v)[G][NV], int e_first) const {
+        const T* row = (const T*)P.v;
+        if (P.v_vec) {
+#pragma unroll
+            for (int e = 0; e < G; ++e)
+#pragma unroll
+                for (int j = 0; j < NV; ++j) v[e][j] = whole_quad<T>(row + (base + min(e_first + e, n - 1)) * P.v_stride + 4 * min(j * 64 + lane, qv - 1));
+        } else {
+#pragma unroll
+            for (int e = 0; e < G; ++e)
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    const int q = min(j * 64 + lane, qv - 1);
+                    v[e][j] = part_quad<T>(row + (base + min(e_first + e, n - 1)) * P.v_stride + 4 * q, HD - 4 * q);
+                }
+        }
+    }
+    // rows of a (n_dst, H D) tensor at the edges' destinations
+    template <int G> __device__ void load_at_dst(Raw (&v)[G][NV], const T* rows, int vec, int e_first) const {
+        if (vec) {
+#pragma unroll
+            for (int e = 0; e < G; ++e)
+#pragma unroll
+                for (int j = 0; j < NV; ++j) v[e][j] = whole_quad<T>(rows + (int64_t)__builtin_amdgcn_readfirstlane(e_dst[min(e_first + e, n - 1)]) * HD + 4 * min(j * 64 + lane, qv - 1));
+        } else {
+#pragma unroll
+            for (int e = 0; e < G; ++e)
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    const int q = min(j * 64 + lane, qv - 1);
+                    v[e][j] = part_quad<T>(rows + (int64_t)__builtin_amdgcn_readfirstlane(e_dst[min(e_first + e, n - 1)]) * HD + 4 * q, HD - 4 * q);
+                }
+        }
+    }
+    __device__ float dropped(int64_t edge, int h) const {
+        if (!P.threshold) return 1.0f;
+        const Words x = dropout_words((uint32_t)edge, (uint32_t)(h >> 2), offset, seed);
+        const uint32_t lo = h & 1 ? x.w[1] : x.w[0], hi = h & 1 ? x.w[3] : x.w[2];
+        return (h & 2 ? hi : lo) >= P.threshold ? P.keep_scale : 0.0f;
+    }
+    // t of the edges e_first .. e_first + GA - 1 (and their dropout factors) into LDS
+    __device__ void logits(const Raw (&a)[NA], int e_first) {
+        const int subs = sub_a == 4 ? qa : 4 * qa;
+        wave_sync();
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            int e, q;
+            if (!a_place(i, e_first, e, q)) continue;
+            const f4 wq = *(const f4*)(w + 4 * q);
+            f4 x;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = 4 * q + j < HK ? act((float)a[i][j]) * wq[j] : 0.0f;
+            if (sub_a == 4) part[e * subs + q] = (x[0] + x[1]) + (x[2] + x[3]);
+            else *(f4*)(part + e * subs + 4 * q) = x;
+        }
+        wave_sync();
+        for (int idx = lane; idx < GA * H; idx += 64) {
+            const int e = (int)((idx * inv_h) >> 16), h = idx - e * H, eb = e_first + e;
+            float s = 0.0f;
+            for (int i = 0; i < n_sub_a; ++i) s += part[e * subs + h * n_sub_a + i];
+            const float l = e_logit[eb];
+            double x = (double)s + (double)l;
+            if (P.n_buckets) { const float b = table[e_bucket[eb] * H + h]; x = b == -__builtin_inff() ? (double)b : x + (double)b; }
+            if (l == -__builtin_inff()) x = -__builtin_inf();          // a masked edge takes no part whatever its features hold
+            if (x == __builtin_inf()) x = __builtin_nan("");
+            t[eb * H + h] = x;
+            keep[eb * H + h] = eb < n ? dropped(base + eb, h) : 0.0f;
+        }
+    }
+};
+
+// ---- forward --------------------------------------------------------------------------------------------------------------------------------
+
+// running softmax of one row in a lane: its quads' weighted sums, and a maximum and sum for each head that the quads touch
+template <int NV, int PARTS> struct Row {
+    f4 acc[NV]; double m[NV][PARTS]; float sum[NV][PARTS];
+    __device__ void clear() {
+        for (int j = 0; j < NV; ++j) { acc[j] = f4{0, 0, 0, 0}; for (int p = 0; p < PARTS; ++p) { m[j][p] = -__builtin_inf(); sum[j][p] = 0.0f; } }
+    }
+    // another (weighted) term with logit x: weight of the old sum and of the term
+    __device__ static void weights(double& m, double x, float& w_old, float& w_new) {
+        if (x > m || x != x) { w_old = m == -__builtin_inf() ? 0.0f : exp_d(m - x); w_new = 1.0f; if (x != x) w_old = w_new = __builtin_nanf(""); m = x; }
+        else { w_old = 1.0f; w_new = exp_d(x - m); }
+    }
+};
+
+// Record of a row that crosses ranges, for each lane of the walk: [NV] quads, then per part a 64-bit maximum and a sum.  Slot 0 of a wave holds its
+// first row, slot 1 its last one.
+template <int NV, int PARTS> struct Record { f4 acc[NV]; double m[NV][PARTS]; float sum[NV][PARTS]; };
+
+template <class T, int SUB, bool WIDE> __device__ inline void
+finish_row(const Args& P, int row, const Row<WIDE ? 4 : 1, 4 / SUB>& r, int lane, int qv, int HD, T* out, float* out32, double* norm) {
+    constexpr int NV = WIDE ? 4 : 1, PARTS = 4 / SUB;
+    const int vec = (HD & 3) == 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int q = j * 64 + lane;
+        if (q >= qv) continue;
+        f4 o;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            const float inv = r.sum[j][p] == 0.0f ? 0.0f : 1.0f / r.sum[j][p];          // (no edge takes part: 0)
+#pragma unroll
+            for (int i = 0; i < SUB; ++i) o[p * SUB + i] = r.acc[j][p * SUB + i] * inv;
+            const int c = 4 * q + p * SUB;
+            if (norm && c < HD && c % P.d == 0) *(d2*)(norm + 2 * ((int64_t)row * P.heads + c / P.d)) = d2{r.m[j][p], (double)inv};
+        }
+        store_quad(out + (int64_t)row * HD + 4 * q, o, vec, HD - 4 * q);
+        if (out32) store_quad(out32 + (int64_t)row * HD + 4 * q, o, vec, HD - 4 * q);
+    }
+}
+
+template <class T, int SUB, bool WIDE> __global__ __launch_bounds__(256)
+void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, int64_t* rng_used) {
+    typedef Wave<T, SUB, WIDE> W;
+    constexpr int NV = W::NV, PARTS = W::PARTS, GA = W::GA;
+    extern __shared__ __align__(16) char lds[];
+    if (rng_used && P.threshold && blockIdx.x == 0 && threadIdx.x < 2) rng_used[threadIdx.x] = P.rng[threadIdx.x];
+    const int edge_blocks = (P.n_waves + kWaves - 1) / kWaves;
+    if ((int)blockIdx.x >= edge_blocks) {
+        // rows without edges: 64 rows a wave
+        const int H = P.heads, HD = H * P.d, lane = threadIdx.x & 63;
+        const int64_t first = (((int64_t)blockIdx.x - edge_blocks) * kWaves + (threadIdx.x >> 6)) * 64, row = first + lane;
+        uint64_t empty = __ballot(row < P.n_dst && P.rowptr[min(row, (int64_t)P.n_dst - 1)] == P.rowptr[min(row, (int64_t)P.n_dst - 1) + 1]);
+        while (empty) {
+            const int64_t r = first + __builtin_ctzll(empty);
+            empty &= empty - 1;
+            for (int i = lane; i < HD; i += 64) { out[r * HD + i] = (T)0.0f; if (out32) out32[r * HD + i] = 0.0f; }
+            if (norm && lane < H) *(d2*)(norm + 2 * (r * H + lane)) = d2{-__builtin_inf(), 0.0};
+        }
+        return;
+    }
+    W w(P, lds, W::wave_bytes(P.heads));
+    if (w.e0 >= w.e1) return;
+    const int lane = w.lane, H = w.H, HD = w.HD, qv = w.qv;
+    int head[NV][PARTS];
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) head[j][p] = min((4 * (j * 64 + lane) + p * SUB) / P.d, H - 1);
+    Row<NV, PARTS> r;
+    r.clear();
+    int cur = __builtin_amdgcn_readfirstlane(P.dst[w.e0]);
+    const bool open_front = w.e0 > 0 && P.dst[w.e0 - 1] == cur;
+    bool first_row = true;
+    Record<NV, PARTS>* rec = (Record<NV, PARTS>*)records + ((int64_t)blockIdx.x * kWaves + w.wave) * 2 * 64 + lane;
+    auto flush = [&](bool open_back) {
+        if ((first_row && open_front) || open_back) {
+            Record<NV, PARTS> x;
+            for (int j = 0; j < NV; ++j) { x.acc[j] = r.acc[j]; for (int p = 0; p < PARTS; ++p) { x.m[j][p] = r.m[j][p]; x.sum[j][p] = r.sum[j][p]; } }
+            rec[first_row ? 0 : 64] = x;
+        } else finish_row<T, SUB, WIDE>(P, cur, r, lane, qv, HD, out, out32, norm);
+    };
+    for (int64_t base = w.e0; base < w.e1; base += kBatch) {
+        w.load_edges(base);
+        for (int g = 0; g < kBatch && g < w.n; g += GA) {
+            typename W::Raw a[W::NA], v[GA][NV];
+            w.load_a(a, g);
+            w.template load_v<GA>(v, g);
+            w.logits(a, g);
+            wave_sync();
+#pragma unroll
+            for (int e = 0; e < GA; ++e) if (g + e < w.n) {
+                const int d = __builtin_amdgcn_readfirstlane(w.e_dst[g + e]);
+                if (d != cur) { flush(false); cur = d; first_row = false; r.clear(); }
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p) {
+                        const double x = w.t[(g + e) * H + head[j][p]];
+                        if (x == -__builtin_inf()) continue;
+                        const float kp = w.keep[(g + e) * H + head[j][p]];
+                        float w_old, w_new;
+                        Row<NV, PARTS>::weights(r.m[j][p], x, w_old, w_new);
+                        r.sum[j][p] = r.sum[j][p] * w_old + w_new;
+#pragma unroll
+                        for (int i = 0; i < SUB; ++i) {
+                            const float old = r.acc[j][p * SUB + i] * w_old;
+                            r.acc[j][p * SUB + i] = kp != 0.0f ? old + w_new * kp * (float)v[e][j][p * SUB + i] : old;
+                        }
+                    }
+            }
+            wave_sync();
+        }
+    }
+    flush(w.e1 < P.n_edges && P.dst[w.e1] == cur);
+}
+
+// Rows that cross ranges: workgroup b looks at the border between ranges b and b + 1, and joins a row whose first crossing that is.  Each wave joins
+// every fourth record, then the four are joined in order.
+template <class T, int SUB, bool WIDE> __global__ __launch_bounds__(256)
+void k_attn_merge(Args P, T* out, float* out32, double* norm, const void* records) {
+    constexpr int NV = WIDE ? 4 : 1, PARTS = 4 / SUB;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, H = P.heads, HD = H * P.d, qv = (HD + 3) >> 2;
+    const int64_t border = ((int64_t)blockIdx.x + 1) * P.range;
+    const int row = P.dst[border];
+    if (P.dst[border - 1] != row) return;
+    const int64_t begin = P.rowptr[row], w0 = blockIdx.x;
+    if (begin < w0 * P.range) return;                                   // an earlier border is its first
+    const int64_t w1 = ((int64_t)P.rowptr[row + 1] - 1) / P.range;
+    const Record<NV, PARTS>* rec = (const Record<NV, PARTS>*)records + lane;
+    Row<NV, PARTS> r;
+    r.clear();
+    auto join = [&](const f4 (&acc)[NV], const double (&m)[NV][PARTS], const float (&sum)[NV][PARTS]) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) {
+                if (m[j][p] == -__builtin_inf()) continue;
+                float w_old, w_new;
+                Row<NV, PARTS>::weights(r.m[j][p], m[j][p], w_old, w_new);
+                r.sum[j][p] = r.sum[j][p] * w_old + sum[j][p] * w_new;
+#pragma unroll
+                for (int i = 0; i < SUB; ++i) r.acc[j][p * SUB + i] = r.acc[j][p * SUB + i] * w_old + acc[j][p * SUB + i] * w_new;
+            }
+    };
+#pragma unroll 2
+    for (int64_t x = w0 + wave; x <= w1; x += kWaves) {
+        const Record<NV, PARTS> o = rec[(x * 2 + (x == w0 && begin > w0 * P.range ? 1 : 0)) * 64];
+        join(o.acc, o.m, o.sum);
+    }
+    __shared__ Record<NV, PARTS> share[kWaves - 1][64];
+    if (wave > 0) {
+        Record<NV, PARTS>& o = share[wave - 1][lane];
+        for (int j = 0; j < NV; ++j) { o.acc[j] = r.acc[j]; for (int p = 0; p < PARTS; ++p) { o.m[j][p] = r.m[j][p]; o.sum[j][p] = r.sum[j][p]; } }
+    }
+    __syncthreads();
+    if (wave > 0) return;
+    for (int o = 0; o < kWaves - 1; ++o) join(share[o][lane].acc, share[o][lane].m, share[o][lane].sum);
+    finish_row<T, SUB, WIDE>(P, row, r, lane, qv, HD, out, out32, norm);
+}
+
+// ---- backward -------------------------------------------------------------------------------------------------------------------------------
+
+// delta[n,h] = sum_c dout out32: a wave per row
+template <class T> __global__ __launch_bounds__(256)
+void k_attn_delta(int64_t n_rows, int H, int D, const T* grad, const float* out32, float* delta) {
+    const int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+    if (row >= n_rows) return;
+    const int lane = threadIdx.x & 63, HD = H * D;
+    const T* g = grad + row * HD; const float* o = out32 + row * HD;
+    for (int h = 0; h < H; ++h) {
+        float s = 0.0f;
+        for (int c = lane; c < D; c += 64) s += (float)g[h * D + c] * o[h * D + c];
+#pragma unroll
+        for (int x = 32; x >= 1; x >>= 1) s += __shfl_xor(s, x, 64);
+        if (lane == 0) delta[row * H + h] = s;
+    }
+}
+
+struct BackArgs {
+    const double* norm; const float* delta; const void* grad; int grad_vec;
+    void* da; void* dv; float* dl;          // any of them may be null
+    float* param_rows;                      // (workgroups, H K + B H) sums of dw and dT, or null
+};
+
+template <class T, int SUB, bool WIDE> __global__ __launch_bounds__(256)
+void k_attn_backward(Args P, BackArgs B) {
+    typedef Wave<T, SUB, WIDE> W;
+    constexpr int NV = W::NV, NA = W::NA, PARTS = W::PARTS, GA = W::GA, GV = WIDE ? 2 : 8;      // GV value rows at a time
+    extern __shared__ __align__(16) char lds[];
+    const int BH = P.n_buckets * P.heads;
+    const size_t own = W::wave_bytes(P.heads) + (size_t)kBatch * P.heads * 4 + (size_t)((BH + 1) & ~1) * 4;
+    W w(P, lds, (own + 15) & ~(size_t)15);
+    const int lane = w.lane, H = w.H, HD = w.HD, HK = w.HK, qv = w.qv, subs = qv * PARTS, per_head = P.d / SUB;
+    float* dt = (float*)(w.e_bucket + kBatch);          // [16][H]
+    float* bins = dt + kBatch * H;                      // [buckets][H]
+    for (int i = lane; i < BH; i += 64) bins[i] = 0.0f;
+    int head[NV][PARTS];
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) head[j][p] = min((4 * (j * 64 + lane) + p * SUB) / P.d, H - 1);
+    f4 dw[NA];
+    int head_a[NA];          // of the lane's feature quads, where a quad lies inside one head
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+        int e, q;
+        w.a_place(i, 0, e, q);
+        dw[i] = f4{0, 0, 0, 0};
+        head_a[i] = min(4 * q / P.k, H - 1);
+    }
+
+    for (int64_t base = w.e0; base < w.e1; base += kBatch) {
+        w.load_edges(base);
+        for (int g = 0; g < kBatch && g < w.n; g += GA) {
+            typename W::Raw a[NA];
+            w.load_a(a, g);
+            w.logits(a, g);
+            wave_sync();
+            for (int idx = lane; idx < GA * H; idx += 64) {          // t becomes p
+                const int e = (int)((idx * w.inv_h) >> 16), h = idx - e * H, eb = g + e;
+                if (eb >= w.n) continue;
+                const double x = w.t[eb * H + h];
+                const d2 at = *(const d2*)(B.norm + 2 * ((int64_t)w.e_dst[eb] * H + h));
+                w.t[eb * H + h] = x == -__builtin_inf() ? 0.0 : (double)(exp_d(x - at[0]) * (float)at[1]);
+            }
+            wave_sync();
+#pragma unroll 1
+            for (int s = g; s < g + GA && s < w.n; s += GV) {
+                typename W::Raw v[GV][NV], up[GV][NV];
+                w.template load_v<GV>(v, s);
+                w.template load_at_dst<GV>(up, (const T*)B.grad, B.grad_vec, s);
+                wave_sync();
+#pragma unroll
+                for (int e = 0; e < GV; ++e) if (s + e < w.n) {
+#pragma unroll
+                    for (int j = 0; j < NV; ++j) {
+                        const int q = j * 64 + lane;
+                        if (q >= qv) continue;
+                        f4 o;
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p) {
+                            const int at = (s + e) * H + head[j][p];
+                            const float f = (float)w.t[at] * w.keep[at];
+                            float dot = 0.0f;
+#pragma unroll
+                            for (int i = 0; i < SUB; ++i) {
+                                const int c = p * SUB + i;
+                                const float u = (float)up[e][j][c];
+                                o[c] = f == 0.0f ? 0.0f : f * u;
+                                dot += (float)v[e][j][c] * u;
+                            }
+                            w.part[e * subs + q * PARTS + p] = dot;
+                        }
+                        if (B.dv) store_quad((T*)B.dv + (base + s + e) * HD + 4 * q, o, (HD & 3) == 0, HD - 4 * q);
+                    }
+                }
+                wave_sync();
+                for (int idx = lane; idx < GV * H; idx += 64) {
+                    const int e = (int)((idx * w.inv_h) >> 16), h = idx - e * H, eb = s + e;
+                    if (eb >= w.n) continue;
+                    float dot = 0.0f;
+                    for (int i = 0; i < per_head; ++i) dot += w.part[e * subs + h * per_head + i];
+                    const float p = (float)w.t[eb * H + h], kp = w.keep[eb * H + h];
+                    const float dp = kp == 0.0f ? 0.0f : kp * dot;
+                    dt[eb * H + h] = p == 0.0f ? 0.0f : p * (dp - B.delta[(int64_t)w.e_dst[eb] * H + h]);
+                }
+            }
+            wave_sync();
+            if (B.dl && lane < GA && g + lane < w.n) {
+                float s = 0.0f;
+                for (int h = 0; h < H; ++h) s += dt[(g + lane) * H + h];
+                B.dl[base + g + lane] = s;
+            }
+#pragma unroll
+            for (int i = 0; i < NA; ++i) {
+                int e, q;
+                if (!w.a_place(i, g, e, q)) continue;
+                const f4 wq = *(const f4*)(w.w + 4 * q);
+                f4 o;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int h = w.sub_a == 4 ? head_a[i] : min((4 * q + j) / P.k, H - 1);
+                    const float f = dt[(g + e) * H + h], x = (float)a[i][j], sg = sigmoid(x);
+                    const float slope = kActNorm * (0.2f + 0.8f * sg * (1.0f + x * (1.0f - sg)));
+                    o[j] = f == 0.0f ? 0.0f : f * wq[j] * slope;
+                    dw[i][j] += f == 0.0f ? 0.0f : f * kActNorm * x * (0.2f + 0.8f * sg);
+                }
+                if (B.da) store_quad((T*)B.da + (base + g + e) * HK + 4 * q, o, (HK & 3) == 0, HK - 4 * q);
+            }
+            if (BH && B.param_rows && lane < H)          // in the edges' order: lane h alone adds to the sums of its head
+                for (int e = 0; e < GA && g + e < w.n; ++e) bins[w.e_bucket[g + e] * H + lane] += dt[(g + e) * H + lane];
+            wave_sync();
+        }
+    }
+    if (!B.param_rows) return;
+    // the workgroup's sums: each wave folds its feature quads by place, then the four waves are added in order
+    wave_sync();
+#pragma unroll
+    for (int i = 0; i < NA; ++i) *(f4*)(w.part + 4 * (i * 64 + lane)) = dw[i];
+    __syncthreads();
+    const size_t stride = (own + 15) & ~(size_t)15;
+    for (int c = threadIdx.x; c < HK; c += 256) {
+        float s = 0.0f;
+        for (int x = 0; x < kWaves; ++x) {
+            const float* part = (const float*)((const char*)w.part + ((ptrdiff_t)x - w.wave) * (ptrdiff_t)stride);
+            for (int i = c >> 2; i < GA * w.qa; i += w.qa) s += part[4 * i + (c & 3)];
+        }
+        B.param_rows[(size_t)blockIdx.x * (HK + BH) + c] = s;
+    }
+    for (int c = threadIdx.x; c < BH; c += 256) {
+        float s = 0.0f;
+        for (int x = 0; x < kWaves; ++x) s += *(const float*)((const char*)(bins + c) + ((ptrdiff_t)x - w.wave) * (ptrdiff_t)stride);
+        B.param_rows[(size_t)blockIdx.x * (HK + BH) + HK + c] = s;
+    }
+}
+
+// column sums of (rows, columns) in 64 bits, in order: 16 columns a workgroup
+static __global__ __launch_bounds__(256) void k_column_sums(const float* x, int rows, int columns, float* first, int n_first, float* second) {
+    __shared__ double share[16][16];
+    const int c = blockIdx.x * 16 + (threadIdx.x & 15), r0 = threadIdx.x >> 4;
+    double s = 0.0;
+    if (c < columns) for (int r = r0; r < rows; r += 16) s += (double)x[(size_t)r * columns + c];
+    share[r0][threadIdx.x & 15] = s;
+    __syncthreads();
+    if (r0 != 0 || c >= columns) return;
+    for (int r = 1; r < 16; ++r) s += share[r][threadIdx.x];
+    if (c < n_first) { if (first) first[c] = (float)s; }
+    else if (second) second[c - n_first] = (float)s;
+}
+
+// ---- the sorted edge list -------------------------------------------------------------------------------------------------------------------
+
+// 32-bit copy of the destinations, first edge of each row (rowptr[n_dst] = n_edges); *bad is set where the list is not sorted or leaves [0, n_dst)
+static __global__ __launch_bounds__(256) void k_edge_segments(const int64_t* edge_dst, int64_t n_edges, int n_dst, int* dst, int* rowptr, int* bad) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < n_edges) {
+        const int64_t d = edge_dst[i];
+        if (d < 0 || d >= n_dst || (i > 0 && edge_dst[i - 1] > d)) *bad = 1;
+        dst[i] = (int)min(max(d, (int64_t)0), (int64_t)n_dst - 1);
+    }
+    if (i <= n_dst) {
+        int64_t lo = 0, hi = n_edges;
+        while (lo < hi) { const int64_t mid = (lo + hi) >> 1; if (edge_dst[mid] < i) lo = mid + 1; else hi = mid; }
+        rowptr[i] = (int)lo;
+    }
+}
+
+}  // namespace attn
+}  // namespace dedf

@@ -1,0 +1,167 @@
+// C entries of the edge attention (include/dedf.h: dedf_edge_segments, dedf_edge_attention, dedf_edge_attention_backward)
+#include "../../include/dedf.h"
+#include "dedf_attn.h"
+#include <algorithm>
+#include <cmath>
+
+using namespace dedf::attn;
+
+// the launches for one element type: each type is a compilation of its own (DEDF_ELEMENT 0, 1, 2), the entries another (none)
+namespace dedf {
+namespace attn {
+
+struct Plan { Args a; bool wide; int sub; size_t record, lds_forward, lds_backward; int blocks; };
+
+struct Forward {
+    const Plan& p; void* out; float* out32; double* norm; int64_t* rng_used; void* records; hipStream_t st;
+    template <class T, int SUB, bool WIDE> int run() {
+        if (p.lds_forward > 65536 && hipFuncSetAttribute((const void*)k_attn_forward<T, SUB, WIDE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds_forward) != hipSuccess) return DEDF_ERR_RUNTIME;
+        const int empty_blocks = (p.a.n_dst + 64 * kWaves - 1) / (64 * kWaves);
+        hipLaunchKernelGGL((k_attn_forward<T, SUB, WIDE>), dim3(p.blocks + empty_blocks), dim3(256), p.lds_forward, st, p.a, (T*)out, out32, norm, records, rng_used);
+        if (p.a.n_waves > 1) hipLaunchKernelGGL((k_attn_merge<T, SUB, WIDE>), dim3(p.a.n_waves - 1), dim3(256), 0, st, p.a, (T*)out, out32, norm, (const void*)records);
+        return hipGetLastError() == hipSuccess ? DEDF_OK : DEDF_ERR_RUNTIME;
+    }
+};
+struct Backward {
+    const Plan& p; BackArgs b; const float* out32; float* delta; float* d_alpha_dot; float* d_table; hipStream_t st;
+    template <class T, int SUB, bool WIDE> int run() {
+        if (p.lds_backward > 65536 && hipFuncSetAttribute((const void*)k_attn_backward<T, SUB, WIDE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds_backward) != hipSuccess) return DEDF_ERR_RUNTIME;
+        const Args& a = p.a;
+        hipLaunchKernelGGL((k_attn_delta<T>), dim3((a.n_dst + kWaves - 1) / kWaves), dim3(256), 0, st, (int64_t)a.n_dst, a.heads, a.d, (const T*)b.grad, out32, delta);
+        hipLaunchKernelGGL((k_attn_backward<T, SUB, WIDE>), dim3(p.blocks), dim3(256), p.lds_backward, st, a, b);
+        if (b.param_rows) {
+            const int n_w = a.heads * a.k, columns = n_w + a.heads * a.n_buckets;
+            hipLaunchKernelGGL(k_column_sums, dim3((columns + 15) / 16), dim3(256), 0, st, (const float*)b.param_rows, p.blocks, columns, d_alpha_dot, n_w, d_table);
+        }
+        return hipGetLastError() == hipSuccess ? DEDF_OK : DEDF_ERR_RUNTIME;
+    }
+};
+
+template <class T, class F> int launch(int sub, bool wide, F f) {
+    return sub == 4 ? (wide ? f.template run<T, 4, true>() : f.template run<T, 4, false>()) : sub == 2 ? (wide ? f.template run<T, 2, true>() : f.template run<T, 2, false>())
+                    : (wide ? f.template run<T, 1, true>() : f.template run<T, 1, false>());
+}
+
+#define DEDF_LAUNCHES(T, PREFIX) PREFIX template int launch<T, Forward>(int, bool, Forward); PREFIX template int launch<T, Backward>(int, bool, Backward);
+#ifndef DEDF_ELEMENT
+DEDF_LAUNCHES(float, extern) DEDF_LAUNCHES(_Float16, extern) DEDF_LAUNCHES(__bf16, extern)
+#elif DEDF_ELEMENT == 0
+DEDF_LAUNCHES(float, )
+#elif DEDF_ELEMENT == 1
+DEDF_LAUNCHES(_Float16, )
+#else
+DEDF_LAUNCHES(__bf16, )
+#endif
+
+}  // namespace attn
+}  // namespace dedf
+
+#ifndef DEDF_ELEMENT
+namespace {
+
+constexpr int kMostWaves = 3072;          // 256 CUs x 12: what is resident at once
+constexpr size_t kMostLds = 160 * 1024;
+
+
+
+size_t element(int type) { return type == DEDF_F32 ? 4 : 2; }
+bool whole_quads(const void* p, int64_t stride, int width, int type) {
+    const size_t quad = 4 * element(type);
+    return (reinterpret_cast<uintptr_t>(p) % quad) == 0 && stride % 4 == 0 && width % 4 == 0;
+}
+
+int make_plan(const dedf_edge_attn* x, Plan& p) {
+    if (!x || x->n_edges < 0 || x->n_dst < 0 || x->heads < 1 || x->k < 1 || x->d < 1 || x->n_buckets < 0) return DEDF_ERR_INVALID;
+    if (x->type != DEDF_F32 && x->type != DEDF_F16 && x->type != DEDF_BF16) return DEDF_ERR_UNSUPPORTED;
+    if (x->n_edges >= (int64_t)1 << 31 || x->heads > 16 || x->k > 256 || x->d > 1024 || x->heads * x->k > 256 || x->heads * x->d > 1024) return DEDF_ERR_UNSUPPORTED;
+    if (x->n_buckets > 1024 || x->n_buckets * x->heads > 2048) return DEDF_ERR_UNSUPPORTED;
+    if (x->n_edges > 0 && (!x->alpha || !x->value || !x->alpha_dot || !x->dst)) return DEDF_ERR_INVALID;
+    if (x->n_dst > 0 && !x->rowptr) return DEDF_ERR_INVALID;
+    if (x->n_dst == 0 && x->n_edges > 0) return DEDF_ERR_INVALID;
+    if (x->n_buckets > 0 && (!x->bias_table || (x->n_edges > 0 && !x->edge_length) || (x->n_buckets > 1 && !x->bias_boundaries))) return DEDF_ERR_INVALID;
+    if (!(x->dropout >= 0.0 && x->dropout < 1.0) || (x->dropout > 0.0 && !x->rng)) return DEDF_ERR_INVALID;
+    if (x->alpha_stride < 0 || x->value_stride < 0) return DEDF_ERR_INVALID;
+    Args& a = p.a;
+    a = Args{};
+    a.n_edges = x->n_edges; a.n_dst = x->n_dst; a.heads = x->heads; a.k = x->k; a.d = x->d;
+    a.a = x->alpha; a.v = x->value; a.w = x->alpha_dot; a.a_stride = x->alpha_stride; a.v_stride = x->value_stride;
+    a.a_vec = whole_quads(a.a, a.a_stride, a.heads * a.k, x->type); a.v_vec = whole_quads(a.v, a.v_stride, a.heads * a.d, x->type);
+    a.dst = x->dst; a.rowptr = x->rowptr; a.logits = x->edge_logits; a.length = x->edge_length; a.bounds = x->bias_boundaries; a.table = x->bias_table;
+    a.n_buckets = x->n_buckets;
+    a.threshold = (uint32_t)std::floor(x->dropout * 4294967296.0);
+    a.keep_scale = (float)(1.0 / (1.0 - x->dropout)); a.rng = x->rng;
+    const int64_t even = (a.n_edges + kMostWaves - 1) / kMostWaves;
+    a.range = (int)std::max<int64_t>(kBatch, (even + kBatch - 1) / kBatch * kBatch);
+    a.n_waves = (int)((a.n_edges + a.range - 1) / a.range);
+    p.sub = x->d % 4 == 0 ? 4 : x->d % 2 == 0 ? 2 : 1;
+    p.wide = a.heads * a.k > 64 || a.heads * a.d > 256;
+    p.blocks = (a.n_waves + kWaves - 1) / kWaves;
+    const auto record = [](auto r) { return sizeof(r) * 64 * 2; };
+    p.record = p.wide ? (p.sub == 4 ? record(Record<4, 1>{}) : p.sub == 2 ? record(Record<4, 2>{}) : record(Record<4, 4>{}))
+                      : (p.sub == 4 ? record(Record<1, 1>{}) : p.sub == 2 ? record(Record<1, 2>{}) : record(Record<1, 4>{}));
+    const size_t own = p.sub == 1 ? Wave<float, 1, false>::wave_bytes(a.heads) : Wave<float, 4, false>::wave_bytes(a.heads);          // (whatever the type and width)
+    const int BH = a.n_buckets * a.heads;
+    const size_t shared = Wave<float, 4, false>::shared_bytes(a.heads * a.k, a.heads, a.n_buckets);
+    p.lds_forward = shared + kWaves * own;
+    p.lds_backward = shared + kWaves * ((own + (size_t)kBatch * a.heads * 4 + (size_t)((BH + 1) & ~1) * 4 + 15) & ~(size_t)15);
+    if (p.lds_forward > kMostLds || p.lds_backward > kMostLds) return DEDF_ERR_UNSUPPORTED;
+    return DEDF_OK;
+}
+size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
+size_t forward_bytes(const Plan& p) { return (size_t)p.blocks * kWaves * p.record; }
+template <class F> int by_shape(int type, int sub, bool wide, F f) {
+    return type == DEDF_F32 ? launch<float>(sub, wide, f) : type == DEDF_F16 ? launch<_Float16>(sub, wide, f) : launch<__bf16>(sub, wide, f);
+}
+size_t backward_bytes(const Plan& p) {
+    return up16((size_t)p.a.n_dst * p.a.heads * 4) + (size_t)p.blocks * (p.a.heads * (p.a.k + p.a.n_buckets)) * 4;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dedf_edge_segments(const int64_t* edge_dst, int64_t n_edges, int n_dst, int32_t* dst, int32_t* rowptr, int32_t* bad, void* stream) {
+    if (n_edges < 0 || n_dst < 0 || !rowptr || !bad || (n_edges > 0 && (!edge_dst || !dst || n_dst == 0))) return DEDF_ERR_INVALID;
+    if (n_edges >= (int64_t)1 << 31) return DEDF_ERR_UNSUPPORTED;
+    const int64_t n = std::max<int64_t>(n_edges, (int64_t)n_dst + 1);
+    hipLaunchKernelGGL(k_edge_segments, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, static_cast<hipStream_t>(stream), edge_dst, n_edges, n_dst, dst, rowptr, bad);
+    return hipGetLastError() == hipSuccess ? DEDF_OK : DEDF_ERR_RUNTIME;
+}
+
+size_t dedf_edge_attention_scratch_bytes(const dedf_edge_attn* x, int backward) {
+    Plan p;
+    if (make_plan(x, p) != DEDF_OK) return 0;
+    return backward ? backward_bytes(p) : forward_bytes(p);
+}
+
+int dedf_edge_attention(const dedf_edge_attn* x, void* out, float* out_f, double* norm, int64_t* rng_used, void* scratch, size_t scratch_bytes, void* stream) {
+    Plan p;
+    const int rc = make_plan(x, p);
+    if (rc != DEDF_OK) return rc;
+    if (p.a.n_dst == 0) return DEDF_OK;
+    if (!out || scratch_bytes < forward_bytes(p) || (forward_bytes(p) > 0 && !scratch) || (reinterpret_cast<uintptr_t>(scratch) & 15)) return DEDF_ERR_INVALID;
+    Forward f{p, out, out_f, norm, rng_used, scratch, static_cast<hipStream_t>(stream)};
+    return by_shape(x->type, p.sub, p.wide, f);
+}
+
+int dedf_edge_attention_backward(const dedf_edge_attn* x, const double* norm, const float* out_f, const void* grad_out, void* d_alpha, void* d_value,
+                                 float* d_alpha_dot, float* d_edge_logits, float* d_bias_table, void* scratch, size_t scratch_bytes, void* stream) {
+    Plan p;
+    const int rc = make_plan(x, p);
+    if (rc != DEDF_OK) return rc;
+    if (p.a.n_dst > 0 && (!norm || !out_f || !grad_out)) return DEDF_ERR_INVALID;
+    if (scratch_bytes < backward_bytes(p) || (backward_bytes(p) > 0 && !scratch) || (reinterpret_cast<uintptr_t>(scratch) & 15)) return DEDF_ERR_INVALID;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int n_w = p.a.heads * p.a.k, columns = n_w + p.a.heads * p.a.n_buckets;
+    if (p.a.n_edges == 0) {          // no edge: the parameters' gradients are zero (a sum over no rows)
+        hipLaunchKernelGGL(k_column_sums, dim3((columns + 15) / 16), dim3(256), 0, st, (const float*)nullptr, 0, columns, d_alpha_dot, n_w, d_bias_table);
+        return hipGetLastError() == hipSuccess ? DEDF_OK : DEDF_ERR_RUNTIME;
+    }
+    BackArgs b{norm, (const float*)scratch, grad_out, whole_quads(grad_out, 0, p.a.heads * p.a.d, x->type), d_alpha, d_value, d_edge_logits,
+               d_alpha_dot || d_bias_table ? (float*)((char*)scratch + up16((size_t)p.a.n_dst * p.a.heads * 4)) : nullptr};
+    Backward f{p, b, out_f, (float*)scratch, d_alpha_dot, d_bias_table, st};
+    return by_shape(x->type, p.sub, p.wide, f);
+}
+
+}  // extern "C"
+#endif

@@ -1,0 +1,450 @@
+// Row operators on irreps features in their training form: the norms around a block fused with its dropout, gate and residual scale
+// (EquivariantLayerNormV2, reference equiformer/layer_norm.py:91-156; skips and projections' dropout, gnn_block.py:164-218), and dropout of whole
+// channels (EquivariantDropout, equiformer/drop.py:76-96), each with its backward pass.
+//
+//   u = post(y)          h = x + scale gate[group, channel] keep[row, channel] u          z = next(h)
+//   norm(f)[c] = w[channel] (f[c] - mean) r + bias:  mean over the scalars (degree 0 only), r = (mean of the degree's squares + eps)^-1/2
+// backward, p = dz w, n = the normalised value:  df = r (p - n mean(p n)), for the scalars minus its mean; sums over rows give the parameters' gradients
+//
+// A wave (four for wide rows) owns a row: a lane holds quads of 4 consecutive components in registers, the degree sums go through the wave once each.  Everything a
+// row needs is read once and its results written once, so memory bandwidth bounds both directions; the backward pass reads the inputs and computes the
+// forward values again instead of storing them.  All sums are in 32 bits over at most 2 048 components; sums over rows are kept per lane, folded per
+// workgroup and added in 64 bits in a fixed order.
+#pragma once
+#include "dedf_philox.h"
+
+namespace dedf {
+namespace rows {
+
+constexpr int kWaves = 4, kMostBlocks = 4;          // waves of a workgroup; degrees of a feature row
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+template <class T> struct Quad;
+template <> struct Quad<float> { typedef f4 type; };
+template <> struct Quad<_Float16> { typedef h4 type; };
+template <> struct Quad<__bf16> { typedef b4 type; };
+
+struct Shape {
+    int n_blocks, width, channels, scalars;          // scalars: channels of degree 0 (the first block), 0 if there is none
+    int start[kMostBlocks + 1];                      // first component of a block
+    int first[kMostBlocks];                          // first channel
+    int d[kMostBlocks];                              // components of a channel
+    float inverse[kMostBlocks];                      // 1 / components of a block
+};
+struct Args {
+    Shape s;
+    int n_rows, groups, slices, slice_rows;          // a unit of work: one slice of one group's consecutive rows
+    const void* x; const void* y;
+    const void* gate; int gate_f32;
+    const float* post_w; const float* post_b; const float* next_w; const float* next_b;
+    float scale, eps;
+    uint32_t threshold; float keep_scale;
+    const int64_t* rng;
+    int vec;
+    // forward
+    void* h; void* z; int64_t* rng_used;
+    // backward
+    const void* dh; const void* dz; void* dx; void* dy;
+    void* d_gate; float* gate_rows;                  // a group with one slice writes its gradient, else (unit, channels) sums
+    float* param_rows;                               // (workgroups, 4 channels): post weight, post bias, next weight, next bias
+};
+
+// sum over the wave, in every lane
+template <int CTRL, int ROWS> __device__ inline float dpp_add(float x) {
+    return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false));
+}
+__device__ inline float wave_sum(float x) {
+    x = dpp_add<0xB1, 0xf>(x);           // neighbours, pairs, halves of a row of 16, rows
+    x = dpp_add<0x4E, 0xf>(x);
+    x = dpp_add<0x141, 0xf>(x);
+    x = dpp_add<0x140, 0xf>(x);
+    x = dpp_add<0x142, 0xa>(x);          // row 0 into 1, 2 into 3; then row 1 into 2 and 3: the last lane holds the sum
+    x = dpp_add<0x143, 0xc>(x);
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+__device__ inline void wave_sync() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
+
+// a lane's components of a row and where they belong.  EVEN: blocks start on whole quads, so a quad has one degree.  WPR: waves that share a row (1; 4,
+// the whole workgroup, for rows over 512 components: one wave would have to spill its registers).
+template <class T, int NQ, bool EVEN, int WPR> struct Row {
+    typedef typename Quad<T>::type Raw;
+    const Shape& s; int lane, vec;        // lane: of the row's WPR x 64
+    float* own; float* exchange; int turn;
+    int block[NQ][EVEN ? 1 : 4];          // -1: no component
+    int channel[NQ][4];
+    __device__ Row(const Shape& shape, int vec_, char* lds) : s(shape), lane(threadIdx.x & (64 * WPR - 1)), vec(vec_), turn(0) {
+        own = (float*)(lds + threadIdx.x / (64 * WPR) * team_bytes(shape));
+        exchange = own + ((shape.width + 3) & ~3);
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = 4 * (j * 64 * WPR + lane) + i;
+                int b = -1, ch = 0;
+#pragma unroll
+                for (int k = 0; k < kMostBlocks; ++k)
+                    if (k < s.n_blocks && c >= s.start[k] && c < s.start[k + 1]) { b = k; ch = s.first[k] + (c - s.start[k]) / s.d[k]; }
+                channel[j][i] = ch;
+                if (!EVEN || i == 0) block[j][EVEN ? 0 : i] = b;
+            }
+    }
+    __device__ int of(int j, int i) const { return block[j][EVEN ? 0 : i]; }
+    __device__ void load(f4 (&f)[NQ], const void* p, int64_t row) const {
+        const T* at = (const T*)p + row * s.width;
+        Raw raw[NQ];
+        if (vec) {
+#pragma unroll
+            for (int j = 0; j < NQ; ++j) raw[j] = *(const Raw*)(at + min(4 * (j * 64 * WPR + lane), s.width - 4));
+#pragma unroll
+            for (int j = 0; j < NQ; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[j][i] = of(j, i) >= 0 ? (float)raw[j][i] : 0.0f;
+        } else {
+#pragma unroll
+            for (int j = 0; j < NQ; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { const int c = 4 * (j * 64 * WPR + lane) + i; f[j][i] = c < s.width ? (float)at[c] : 0.0f; }
+        }
+    }
+    __device__ void store(void* p, int64_t row, const f4 (&f)[NQ]) const {
+        T* at = (T*)p + row * s.width;
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+            const int c = 4 * (j * 64 * WPR + lane);
+            if (vec) { if (c < s.width) *(Raw*)(at + c) = Raw{(T)f[j][0], (T)f[j][1], (T)f[j][2], (T)f[j][3]}; }
+            else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) if (c + i < s.width) at[c + i] = (T)f[j][i];
+            }
+        }
+    }
+    // a channel's value on each of its components
+    __device__ void spread(f4 (&f)[NQ], const float* values, int n) const {
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[j][i] = of(j, i) >= 0 && channel[j][i] < n ? values[channel[j][i]] : 0.0f;
+    }
+    __device__ void sync() const { if constexpr (WPR == 1) wave_sync(); else __syncthreads(); }
+    // sums over the row's lanes, in every lane
+    template <int N> __device__ void row_sums(float (&v)[N]) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = wave_sum(v[k]);
+        if constexpr (WPR > 1) {          // (two buffers in turn: a wave that is one exchange ahead does not touch what another still reads)
+            float* at = exchange + turn * WPR * 8;
+            turn ^= 1;
+            if ((lane & 63) == 0)
+#pragma unroll
+                for (int k = 0; k < N; ++k) at[(lane >> 6) * 8 + k] = v[k];
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < N; ++k) { v[k] = 0.0f; for (int w = 0; w < WPR; ++w) v[k] += at[w * 8 + k]; }
+        }
+    }
+    // a lane's share of the sums over each block of f g
+    __device__ void block_parts(float (&part)[kMostBlocks], const f4 (&f)[NQ], const f4 (&g)[NQ]) const {
+#pragma unroll
+        for (int k = 0; k < kMostBlocks; ++k) part[k] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+            if constexpr (EVEN) {
+                const f4 m = f[j] * g[j];
+                const float q = (m[0] + m[1]) + (m[2] + m[3]);
+#pragma unroll
+                for (int k = 0; k < kMostBlocks; ++k) part[k] += block[j][0] == k ? q : 0.0f;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int k = 0; k < kMostBlocks; ++k) part[k] += of(j, i) == k ? f[j][i] * g[j][i] : 0.0f;
+            }
+        }
+    }
+    __device__ float scalar_part(const f4 (&f)[NQ]) const {
+        float part = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) part += of(j, i) == 0 ? f[j][i] : 0.0f;
+        return part;
+    }
+    __device__ float pick(const float (&v)[kMostBlocks], int j, int i) const {
+        const int b = of(j, i);
+        return b == 0 ? v[0] : b == 1 ? v[1] : b == 2 ? v[2] : v[3];
+    }
+    // f becomes its normalised value n, r the factor of each block
+    __device__ void normalise(f4 (&f)[NQ], float (&r)[kMostBlocks], float eps) {
+        if (s.scalars) {
+            float total[1] = {scalar_part(f)};
+            row_sums(total);
+            const float mean = total[0] * s.inverse[0];
+#pragma unroll
+            for (int j = 0; j < NQ; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) if (of(j, i) == 0) f[j][i] -= mean;
+        }
+        block_parts(r, f, f);
+        row_sums(r);
+#pragma unroll
+        for (int k = 0; k < kMostBlocks; ++k) if (k < s.n_blocks) r[k] = rsqrtf(r[k] * s.inverse[k] + eps);
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[j][i] *= pick(r, j, i);
+    }
+    // g: gradient of the normalised value n -> gradient of the value before the norm
+    __device__ void normalise_back(f4 (&g)[NQ], const f4 (&n)[NQ], const float (&r)[kMostBlocks]) {
+        float part[kMostBlocks], sums[kMostBlocks + 1], dot[kMostBlocks];
+        block_parts(part, g, n);
+#pragma unroll
+        for (int k = 0; k < kMostBlocks; ++k) sums[k] = part[k];
+        sums[kMostBlocks] = scalar_part(g);
+        row_sums(sums);
+        const float mean = sums[kMostBlocks] * s.inverse[0];
+#pragma unroll
+        for (int k = 0; k < kMostBlocks; ++k) dot[k] = sums[k] * s.inverse[k];
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) g[j][i] = pick(r, j, i) * (g[j][i] - (s.scalars && of(j, i) == 0 ? mean : 0.0f) - n[j][i] * pick(dot, j, i));
+    }
+    // dropout factors of a row, one word for each channel, through LDS
+    __device__ void keep(f4 (&f)[NQ], int64_t row, uint64_t offset, uint64_t seed, uint32_t threshold, float scale) const {
+        sync();
+        for (int g = lane; g < (s.channels + 3) >> 2; g += 64 * WPR) {
+            const Words x = dropout_words((uint32_t)row, (1u << 16) + g, offset, seed);
+            *(f4*)(own + 4 * g) = f4{x.w[0] >= threshold ? scale : 0.0f, x.w[1] >= threshold ? scale : 0.0f, x.w[2] >= threshold ? scale : 0.0f, x.w[3] >= threshold ? scale : 0.0f};
+        }
+        sync();
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[j][i] = own[channel[j][i]];
+    }
+    // components to LDS, from which folded() adds up a channel's
+    __device__ void fold(const f4 (&f)[NQ]) const {
+        sync();
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) if (4 * (j * 64 * WPR + lane) < s.width) *(f4*)(own + 4 * (j * 64 * WPR + lane)) = f[j];
+        sync();
+    }
+    __device__ float folded(const float* lds, int c) const {
+        int b = 0;
+        for (int k = 1; k < s.n_blocks; ++k) if (c >= s.first[k]) b = k;
+        float sum = 0.0f;
+        const int at = s.start[b] + (c - s.first[b]) * s.d[b];
+        for (int i = 0; i < s.d[b]; ++i) sum += lds[at + i];
+        return sum;
+    }
+    static __host__ __device__ size_t team_bytes(const Shape& s) { return ((size_t)(s.width + 3) >> 2) * 16 + (WPR > 1 ? 2 * WPR * 8 * 4 : 0); }
+};
+
+template <class T> __device__ inline float gate_at(const void* gate, int f32, int64_t i) { return f32 ? ((const float*)gate)[i] : (float)((const T*)gate)[i]; }
+
+template <class T, int NQ, bool EVEN, int WPR> __global__ __launch_bounds__(256) void k_norm_forward(Args P) {
+    extern __shared__ __align__(16) char lds[];
+    Row<T, NQ, EVEN, WPR> R(P.s, P.vec, lds);
+    if (P.rng_used && P.threshold && blockIdx.x == 0 && threadIdx.x < 2) P.rng_used[threadIdx.x] = P.rng[threadIdx.x];
+    constexpr int TEAMS = kWaves / WPR;
+    const int team = threadIdx.x / (64 * WPR);
+    uint64_t seed = 0, offset = 0;
+    if (P.threshold) { seed = (uint64_t)P.rng[0]; offset = (uint64_t)P.rng[1]; }
+    f4 pw[NQ], pb[NQ], nw[NQ], nb[NQ], gate[NQ];
+    if (P.post_w) { R.spread(pw, P.post_w, P.s.channels); R.spread(pb, P.post_b, P.s.scalars); }
+    if (P.z) { R.spread(nw, P.next_w, P.s.channels); R.spread(nb, P.next_b, P.s.scalars); }
+    const int units = P.groups * P.slices, group_rows = P.n_rows / P.groups;
+    for (int u = blockIdx.x * TEAMS + team; u < units; u += gridDim.x * TEAMS) {
+        const int g = u / P.slices, first = (u - g * P.slices) * P.slice_rows, last = min(first + P.slice_rows, group_rows);
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) gate[j][i] = P.scale * (P.gate ? gate_at<T>(P.gate, P.gate_f32, (int64_t)g * P.s.channels + R.channel[j][i]) : 1.0f);
+        for (int k = first; k < last; ++k) {
+            const int64_t row = (int64_t)g * group_rows + k;
+            f4 h[NQ], y[NQ];
+            R.load(h, P.x, row);
+            if (P.y) {
+                R.load(y, P.y, row);
+                if (P.post_w) {
+                    float r[kMostBlocks];
+                    R.normalise(y, r, P.eps);
+#pragma unroll
+                    for (int j = 0; j < NQ; ++j) y[j] = y[j] * pw[j] + pb[j];
+                }
+                if (P.threshold) {
+                    f4 m[NQ];
+                    R.keep(m, row, offset, seed, P.threshold, P.keep_scale);
+#pragma unroll
+                    for (int j = 0; j < NQ; ++j)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) y[j][i] = m[j][i] == 0.0f ? 0.0f : y[j][i] * m[j][i];
+                }
+#pragma unroll
+                for (int j = 0; j < NQ; ++j) h[j] += gate[j] * y[j];
+                R.store(P.h, row, h);
+            }
+            if (P.z) {
+                float r[kMostBlocks];
+                R.normalise(h, r, P.eps);
+#pragma unroll
+                for (int j = 0; j < NQ; ++j) h[j] = h[j] * nw[j] + nb[j];
+                R.store(P.z, row, h);
+            }
+        }
+    }
+}
+
+template <class T, int NQ, bool EVEN, int WPR> __global__ __launch_bounds__(256) void k_norm_backward(Args P) {
+    extern __shared__ __align__(16) char lds[];
+    typedef Row<T, NQ, EVEN, WPR> Rw;
+    Rw R(P.s, P.vec, lds);
+    constexpr int TEAMS = kWaves / WPR;
+    const int team = threadIdx.x / (64 * WPR), C = P.s.channels;
+    uint64_t seed = 0, offset = 0;
+    if (P.threshold) { seed = (uint64_t)P.rng[0]; offset = (uint64_t)P.rng[1]; }
+    const bool post = P.post_w != nullptr, next = P.dz != nullptr;
+    f4 pw[NQ], pb[NQ], nw[NQ], gate[NQ], d_pw[NQ], d_pb[NQ], d_nw[NQ], d_nb[NQ], d_gate[NQ];
+    if (post) { R.spread(pw, P.post_w, C); R.spread(pb, P.post_b, P.s.scalars); }
+    if (next) R.spread(nw, P.next_w, C);
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) d_pw[j] = d_pb[j] = d_nw[j] = d_nb[j] = f4{0, 0, 0, 0};
+    const int units = P.groups * P.slices, group_rows = P.n_rows / P.groups;
+    for (int u = blockIdx.x * TEAMS + team; u < units; u += gridDim.x * TEAMS) {
+        const int g = u / P.slices, slice = u - g * P.slices, first = slice * P.slice_rows, last = min(first + P.slice_rows, group_rows);
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+            d_gate[j] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) gate[j][i] = P.gate ? gate_at<T>(P.gate, P.gate_f32, (int64_t)g * C + R.channel[j][i]) : 1.0f;
+        }
+        for (int k = first; k < last; ++k) {
+            const int64_t row = (int64_t)g * group_rows + k;
+            f4 h[NQ], n[NQ], y[NQ], m[NQ], up[NQ];
+            float ry[kMostBlocks];
+            R.load(h, P.x, row);
+            if (P.y) R.load(y, P.y, row);
+            if (P.dh) R.load(up, P.dh, row);
+            else
+#pragma unroll
+                for (int j = 0; j < NQ; ++j) up[j] = f4{0, 0, 0, 0};
+            if (P.y) {
+                if (post) R.normalise(y, ry, P.eps);
+                if (P.threshold) R.keep(m, row, offset, seed, P.threshold, P.keep_scale);
+#pragma unroll
+                for (int j = 0; j < NQ; ++j) {
+                    if (!P.threshold) m[j] = f4{1.0f, 1.0f, 1.0f, 1.0f};
+                    m[j] *= P.scale;
+                    const f4 un = post ? y[j] * pw[j] + pb[j] : y[j];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) h[j][i] += m[j][i] == 0.0f ? 0.0f : gate[j][i] * m[j][i] * un[i];
+                }
+            }
+            if (next) {
+                f4 dz[NQ];
+                float r[kMostBlocks];
+                R.load(dz, P.dz, row);
+#pragma unroll
+                for (int j = 0; j < NQ; ++j) n[j] = h[j];
+                R.normalise(n, r, P.eps);
+#pragma unroll
+                for (int j = 0; j < NQ; ++j) {
+                    d_nw[j] += dz[j] * n[j];
+                    d_nb[j] += dz[j];
+                    dz[j] *= nw[j];
+                }
+                R.normalise_back(dz, n, r);
+#pragma unroll
+                for (int j = 0; j < NQ; ++j) up[j] += dz[j];
+            }
+            if (P.dx) R.store(P.dx, row, up);
+            if (!P.y) continue;
+#pragma unroll
+            for (int j = 0; j < NQ; ++j) {
+                const f4 un = post ? y[j] * pw[j] + pb[j] : y[j];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float t = m[j][i] == 0.0f ? 0.0f : m[j][i] * up[j][i];
+                    d_gate[j][i] += t == 0.0f ? 0.0f : t * un[i];
+                    up[j][i] = t * gate[j][i];
+                }
+                if (post) {
+                    d_pw[j] += up[j] * y[j];
+                    d_pb[j] += up[j];
+                    up[j] *= pw[j];
+                }
+            }
+            if (!P.dy) continue;
+            if (post) R.normalise_back(up, y, ry);
+            R.store(P.dy, row, up);
+        }
+        if (P.d_gate || P.gate_rows) {
+            R.fold(d_gate);
+            for (int c = R.lane; c < C; c += 64 * WPR) {
+                const float s = R.folded(R.own, c);
+                if (P.gate_rows) P.gate_rows[(int64_t)u * C + c] = s;
+                else if (P.gate_f32) ((float*)P.d_gate)[(int64_t)u * C + c] = s;
+                else ((T*)P.d_gate)[(int64_t)u * C + c] = (T)s;
+            }
+        }
+    }
+    if (!P.param_rows) return;
+    // the workgroup's sums, a parameter at a time
+#pragma unroll
+    for (int which = 0; which < 4; ++which) {
+        __syncthreads();
+        if (which == 0) R.fold(d_pw); else if (which == 1) R.fold(d_pb); else if (which == 2) R.fold(d_nw); else R.fold(d_nb);
+        __syncthreads();
+        for (int c = threadIdx.x; c < C; c += 256) {
+            float s = 0.0f;
+            for (int x = 0; x < TEAMS; ++x) s += R.folded((const float*)(lds + x * Rw::team_bytes(P.s)), c);
+            P.param_rows[((int64_t)blockIdx.x * 4 + which) * C + c] = s;
+        }
+    }
+}
+
+// x keep: forward and backward are the same map
+template <class T, int NQ, bool EVEN, int WPR> __global__ __launch_bounds__(256) void k_dropout(Args P) {
+    extern __shared__ __align__(16) char lds[];
+    Row<T, NQ, EVEN, WPR> R(P.s, P.vec, lds);
+    if (P.rng_used && P.threshold && blockIdx.x == 0 && threadIdx.x < 2) P.rng_used[threadIdx.x] = P.rng[threadIdx.x];
+    constexpr int TEAMS = kWaves / WPR;
+    const int team = threadIdx.x / (64 * WPR);
+    uint64_t seed = 0, offset = 0;
+    if (P.threshold) { seed = (uint64_t)P.rng[0]; offset = (uint64_t)P.rng[1]; }
+    for (int64_t row = blockIdx.x * TEAMS + team; row < P.n_rows; row += gridDim.x * TEAMS) {
+        f4 x[NQ], m[NQ];
+        R.load(x, P.x, row);
+        if (P.threshold) {
+            R.keep(m, row, offset, seed, P.threshold, P.keep_scale);
+#pragma unroll
+            for (int j = 0; j < NQ; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[j][i] = m[j][i] == 0.0f ? 0.0f : x[j][i] * m[j][i];
+        }
+        R.store(P.h, row, x);
+    }
+}
+
+// sums over `rows` rows of (rows, columns) in 64 bits, in order; 16 columns a workgroup, one of blockIdx.y matrices.  Output column c goes to
+// out[c / width] + c % width (an absent output is skipped), as 32 bits or as T.
+template <class T> __global__ __launch_bounds__(256) void k_row_sums(const float* x, int rows, int columns, int width, float* o0, float* o1, float* o2, float* o3, int n1, int n3, T* narrow) {
+    __shared__ double share[16][16];
+    const int c = blockIdx.x * 16 + (threadIdx.x & 15), r0 = threadIdx.x >> 4;
+    const float* m = x + (size_t)blockIdx.y * rows * columns;
+    double s = 0.0;
+    if (c < columns) for (int r = r0; r < rows; r += 16) s += (double)m[(size_t)r * columns + c];
+    share[r0][threadIdx.x & 15] = s;
+    __syncthreads();
+    if (r0 != 0 || c >= columns) return;
+    for (int r = 1; r < 16; ++r) s += share[r][threadIdx.x];
+    if (narrow) { narrow[(size_t)blockIdx.y * columns + c] = (T)(float)s; return; }
+    const int which = c / width, at = c - which * width;
+    float* o = which == 0 ? o0 : which == 1 ? o1 : which == 2 ? o2 : o3;
+    const int n = which == 1 ? n1 : which == 3 ? n3 : width;
+    if (o && at < n) o[(size_t)blockIdx.y * n + at] = (float)s;
+}
+
+}  // namespace rows
+}  // namespace dedf

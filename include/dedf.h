@@ -149,8 +149,9 @@ const char* dedf_version(void);
  * dedf_config [which = 0], dedf_schedule [1], dedf_stats [2], dedf_profile [3] for bindings that mirror the structs by hand (diffusion_edf_amd/_lib.py checks both).
  *   1  rounds 1-2.   2  round 3: dedf_config.unet_valid[4] (was [3]), dedf_stats.rtab_err / rtab_fallback, dedf_radius scratch arguments.
  *   3  round 4: dedf_abi_version / dedf_struct_size themselves; no struct change.   4  round 4: dedf_config.unet_narrow (appended).
- *   5  round 5: dedf_stats.sample_retries / edges_per_dst_capacity (appended).   6  round 5: dedf_config.query_time_encoding (appended). */
-#define DEDF_ABI_VERSION 6
+ *   5  round 5: dedf_stats.sample_retries / edges_per_dst_capacity (appended).   6  round 5: dedf_config.query_time_encoding (appended).
+ *   7  dedf_edge_attn, dedf_norm and the entry points of the training operators; no change of an older struct. */
+#define DEDF_ABI_VERSION 7
 int dedf_abi_version(void);
 size_t dedf_struct_size(int which);
 
@@ -293,6 +294,81 @@ int dedf_fps(const float* x, int n, int n_samples, int start, int* idx_out, void
 size_t dedf_radius_scratch_bytes(int n_dst);
 int dedf_radius(const float* x_src, int n_src, const float* x_dst, int n_dst, float r, int max_num_neighbors, int exclude_self,
                 int64_t edge_cap, int64_t* edge_dst, int64_t* edge_src, int64_t* n_edges, void* scratch, size_t scratch_bytes, void* stream);
+
+/* ---- Training operators (no handle; current device; device pointers; caller-owned scratch, 16-byte aligned; no synchronisation) -----------------
+ * They are what the reference's graph attention block consists of beside its linear layers, with gradients and dropout; the fused kernels above
+ * evaluate the same block for inference only.  Element types: features and activations in `type`, parameters and their gradients in float32, sums in 32
+ * or 64 bits.  Dropout draws from Philox4x32-10: key = rng[0], words of the counter = (edge, head / 4) or (row, 65536 + channel / 4), then
+ * rng[1] (64 bits); word head % 4 or channel % 4; kept iff word >= floor(dropout 2^32), then divided by 1 - dropout.  `rng` is read on the device, so a
+ * captured graph draws anew when its words change between replays; the forward call copies them to `rng_used` for the backward call. */
+#define DEDF_F32 0
+#define DEDF_F16 1
+#define DEDF_BF16 2
+
+/* Attention over edges sorted by destination: graph_attention.py:237-273 (SmoothLeakyReLU under normalize2mom, alpha_dot, scatter_logsumexp, alpha_drop,
+ * scatter), with a learned bias for buckets of the edge length:
+ *   t[e,h] = sum_k act(alpha[e,h,k]) alpha_dot[h,k] + edge_logits[e] + bias_table[b(edge_length[e]), h],   b(x) = number of boundaries <= x
+ *   out[n,h,:] = sum over the edges of n of softmax(t)[e,h] keep[e,h] value[e,h,:]
+ * An edge and head whose t is -inf, by its edge logit or its bucket's bias, takes no part, whatever alpha and value hold there; a row in which none does
+ * is zero.  Limits: n_edges < 2^31, heads <= 16, heads k <= 256, heads d <= 1024, n_buckets <= 1024, heads n_buckets <= 2048. */
+typedef struct dedf_edge_attn {
+    int64_t n_edges;
+    int n_dst, heads, k, d, type;
+    int n_buckets;                         /* 0: no length bias */
+    const void* alpha;                     /* (n_edges, heads, k); consecutive edges alpha_stride elements apart, the rest contiguous */
+    int64_t alpha_stride;
+    const void* value;                     /* (n_edges, heads, d); consecutive edges value_stride elements apart, the rest contiguous */
+    int64_t value_stride;
+    const float* alpha_dot;                /* (heads, k) */
+    const int32_t* dst;                    /* (n_edges) and rowptr (n_dst + 1): from dedf_edge_segments */
+    const int32_t* rowptr;
+    const float* edge_logits;              /* (n_edges) or NULL */
+    const float* edge_length;              /* (n_edges), bias_boundaries (n_buckets - 1, ascending), bias_table (n_buckets, heads) */
+    const float* bias_boundaries;
+    const float* bias_table;
+    double dropout;                        /* in [0, 1) */
+    const int64_t* rng;                    /* (2) seed, offset; may be NULL without dropout */
+} dedf_edge_attn;
+/* 32-bit destinations and row pointers of a sorted list; *bad (zeroed by the caller) is set if the list is not sorted or leaves [0, n_dst).  The
+ * attention reads in bounds whatever the list was, but what it computes from a bad one is undefined. */
+int dedf_edge_segments(const int64_t* edge_dst, int64_t n_edges, int n_dst, int32_t* dst, int32_t* rowptr, int32_t* bad, void* stream);
+size_t dedf_edge_attention_scratch_bytes(const dedf_edge_attn* a, int backward);
+/* out (n_dst, heads, d) in `type`; for the backward call, or NULL: out_f the same in float32, norm (n_dst, heads, 2)
+ * each row's largest logit and 1 / sum of exp(t - largest), rng_used (2) */
+int dedf_edge_attention(const dedf_edge_attn* a, void* out, float* out_f, double* norm, int64_t* rng_used, void* scratch, size_t scratch_bytes, void* stream);
+/* a->rng: the forward call's rng_used.  Gradients may be NULL: d_alpha, d_value contiguous in `type`, the others float32. */
+int dedf_edge_attention_backward(const dedf_edge_attn* a, const double* norm, const float* out_f, const void* grad_out, void* d_alpha, void* d_value,
+                                 float* d_alpha_dot, float* d_edge_logits, float* d_bias_table, void* scratch, size_t scratch_bytes, void* stream);
+
+/* The norms around a block with what stands between them (gnn_block.py:164-218; EquivariantLayerNormV2, equiformer/layer_norm.py:91-156):
+ *   u = post(y) (or y: no post_weight)     h = x + scale gate[group, channel] keep[row, channel] u     z = next(h) (if next_weight)
+ * The n_rows rows fall into `groups` runs of n_rows / groups consecutive rows, one gate row each.  y == NULL: z = next(x) alone, h is not written.
+ * Irreps: up to 4 blocks mul[b] x degree[b], degrees ascending, at most 2048 components.  Weights: one float for each channel, biases: for each
+ * channel of degree 0 (ignored without any). */
+typedef struct dedf_norm {
+    int type, n_rows, n_blocks, groups;
+    int mul[4], degree[4];
+    const void* x;                         /* (n_rows, components) */
+    const void* y;
+    const void* gate;                      /* (groups, channels) in `type`, or in float32 with gate_f = 1; NULL: none */
+    int gate_f;
+    float scale, eps;
+    const float* post_weight;
+    const float* post_bias;
+    const float* next_weight;
+    const float* next_bias;
+    double dropout;
+    const int64_t* rng;
+} dedf_norm;
+int dedf_norm_gate_residual(const dedf_norm* a, void* h, void* z, int64_t* rng_used, void* stream);
+size_t dedf_norm_scratch_bytes(const dedf_norm* a);          /* of the backward call */
+/* grad_h or grad_z may be NULL (zero), any gradient too; d_gate in the gate's type */
+int dedf_norm_gate_residual_backward(const dedf_norm* a, const void* grad_h, const void* grad_z, void* d_x, void* d_y, void* d_gate,
+                                     float* d_post_weight, float* d_post_bias, float* d_next_weight, float* d_next_bias,
+                                     void* scratch, size_t scratch_bytes, void* stream);
+/* out[row] = x[row] keep[row, channel] (EquivariantDropout, equiformer/drop.py:76-96); its own gradient on another tensor.  out may be x. */
+int dedf_channel_dropout(int type, int n_rows, int n_blocks, const int* mul, const int* degree, const void* x, double dropout, const int64_t* rng,
+                         void* out, int64_t* rng_used, void* stream);
 
 #ifdef __cplusplus
 }
