@@ -18,6 +18,9 @@
 #pragma once
 #include "dedf_philox.h"
 
+// products are fused into sums where it says so, not where the compiler likes: a result does not depend on the instantiation that alignment picks
+#pragma clang fp contract(off)
+
 namespace dedf {
 namespace attn {
 
@@ -40,7 +43,6 @@ struct Args {
     int n_dst, heads, k, d;
     const void* a; const void* v; const float* w;
     int64_t a_stride, v_stride;            // elements between the rows of two edges
-    int a_vec, v_vec;                      // rows start on whole quads (base, stride and width): one load per quad
     const int* dst; const int* rowptr;
     const float* logits; const float* length; const float* bounds; const float* table;
     int n_buckets;
@@ -49,16 +51,16 @@ struct Args {
     int range, n_waves;                    // edges per wave, waves
 };
 
-// quad of a row, as stored: one load where rows start on whole quads, else its `left` elements
-template <class T> __device__ inline typename Quad<T>::type whole_quad(const T* p) { return *(const typename Quad<T>::type*)p; }
-template <class T> __device__ inline typename Quad<T>::type part_quad(const T* p, int left) {
+// quad of a row, as stored: one access where rows consist of whole, aligned quads (VEC), else its `left` elements
+template <class T, bool VEC> __device__ inline typename Quad<T>::type load_quad(const T* p, int left) {
+    if constexpr (VEC) return *(const typename Quad<T>::type*)p;
     typename Quad<T>::type r = {(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f};
 #pragma unroll
     for (int i = 0; i < 4; ++i) if (i < left) r[i] = p[i];
     return r;
 }
-template <class T> __device__ inline void store_quad(T* p, f4 x, int vec, int left) {
-    if (vec) { *(typename Quad<T>::type*)p = typename Quad<T>::type{(T)x[0], (T)x[1], (T)x[2], (T)x[3]}; return; }
+template <class T, bool VEC> __device__ inline void store_quad(T* p, f4 x, int left) {
+    if constexpr (VEC) { *(typename Quad<T>::type*)p = typename Quad<T>::type{(T)x[0], (T)x[1], (T)x[2], (T)x[3]}; return; }
 #pragma unroll
     for (int i = 0; i < 4; ++i) if (i < left) p[i] = (T)x[i];
 }
@@ -74,7 +76,7 @@ __device__ inline float exp_d(double x) {
     return __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f((float)(y - n)), (int)n);
 }
 __device__ inline float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
-__device__ inline float act(float x) { return kActNorm * x * (0.2f + 0.8f * sigmoid(x)); }
+__device__ inline float act(float x) { return kActNorm * x * fmaf(0.8f, sigmoid(x), 0.2f); }
 
 // number of boundaries <= x in a sorted list
 __device__ inline int bucket_of(const float* bounds, int n, float x) {
@@ -86,8 +88,9 @@ __device__ inline int bucket_of(const float* bounds, int n, float x) {
 // what both directions share: the wave's place, its LDS, the batch's per-edge values, the logits
 //   SUB: a quad is cut into 4 / SUB parts that each lie inside one head (SUB 4: head widths divisible by 4; 2: even; 1: any)
 //   WIDE: up to 4 quads per lane (value rows of up to 1 024 channels), feature rows of up to 256
-template <class T, int SUB, bool WIDE> struct Wave {
+template <class T, int SUB, bool VEC, bool WIDE> struct Wave {
     static constexpr int NV = WIDE ? 4 : 1, NA = 4, GA = WIDE ? 4 : 16;      // GA edges x feature quads fill NA loads of a wave
+    static constexpr int R = WIDE ? 2 : 8;                                   // value rows in flight
     static constexpr int PARTS = 4 / SUB;
     static constexpr int kPart = SUB == 1 ? 2048 : 1024;                     // floats of the partial-sum buffer
     const Args& P;
@@ -97,13 +100,14 @@ template <class T, int SUB, bool WIDE> struct Wave {
     float* part; double* t; float* keep; const float* w; const float* bounds; const float* table;
     uint64_t seed, offset;
     int64_t base; int n;                                                     // the batch: edges base .. base + n - 1, n <= 16
+    uint32_t starts;                                                         // bit e: its edge e begins a row (or the batch)
     int* e_dst; int* e_bucket; float* e_logit;                               // its edges' destination, length bucket, edge logit
 
-    static __host__ __device__ size_t wave_bytes(int H) { return (size_t)kPart * 4 + (size_t)kBatch * (H + 1) * 12; }
+    static __host__ __device__ size_t wave_bytes(int H) { return (size_t)kPart * 4 + (size_t)kBatch * (H * 16 + 12); }
     static __host__ __device__ size_t shared_bytes(int HK, int H, int B) { return (((size_t)((HK + 3) & ~3) + (B ? B + (size_t)B * H : 0)) * 4 + 15) & ~(size_t)15; }
 
     __device__ Wave(const Args& p, char* lds, size_t own_bytes) : P(p) {
-        lane = threadIdx.x & 63; wave = threadIdx.x >> 6;
+        lane = threadIdx.x & 63; wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);          // (known to be uniform: row addresses stay scalar)
         H = p.heads; K = p.k; D = p.d; HK = H * K; HD = H * D;
         qa = (HK + 3) >> 2; qv = (HD + 3) >> 2;
         sub_a = (K & 3) ? 1 : 4; n_sub_a = K / sub_a;
@@ -118,21 +122,28 @@ template <class T, int SUB, bool WIDE> struct Wave {
         table = s;
         char* mine = lds + shared_bytes(HK, H, B) + wave * own_bytes;
         t = (double*)mine; part = (float*)(mine + (size_t)kBatch * H * 8); keep = part + kPart;
-        e_logit = keep + kBatch * H; e_dst = (int*)(e_logit + kBatch); e_bucket = e_dst + kBatch;
+        e_logit = keep + 2 * kBatch * H; e_dst = (int*)(e_logit + kBatch); e_bucket = e_dst + kBatch;
         seed = offset = 0;
         if (p.threshold) { seed = (uint64_t)p.rng[0]; offset = (uint64_t)p.rng[1]; }
         const int64_t id = (int64_t)blockIdx.x * kWaves + wave;
         e0 = min(id * p.range, p.n_edges); e1 = min(e0 + p.range, p.n_edges);
         __syncthreads();
     }
-    __device__ void load_edges(int64_t b) {
+    // per-edge values of the batch at b: requested early (into registers of the first 16 lanes), put into LDS when the batch begins
+    struct Edge { int dst; float logit, length; };
+    __device__ Edge request(int64_t b) const {
+        const int64_t e = min(b + (lane & (kBatch - 1)), e1 - 1);          // (places behind the last edge repeat it)
+        return Edge{P.dst[e], P.logits ? P.logits[e] : 0.0f, P.n_buckets ? P.length[e] : 0.0f};
+    }
+    __device__ void begin(int64_t b, const Edge& x) {
         base = b; n = (int)min((int64_t)kBatch, e1 - b);
-        if (lane < kBatch) {          // (places behind the last edge repeat it)
-            const int64_t e = b + min(lane, n - 1);
-            e_dst[lane] = P.dst[e];
-            e_logit[lane] = P.logits ? P.logits[e] : 0.0f;
-            e_bucket[lane] = P.n_buckets ? bucket_of(bounds, P.n_buckets - 1, P.length[e]) : 0;
+        if (lane < kBatch) {
+            e_dst[lane] = x.dst;
+            e_logit[lane] = x.logit;
+            e_bucket[lane] = P.n_buckets ? bucket_of(bounds, P.n_buckets - 1, x.length) : 0;
         }
+        const int before = __shfl_up(x.dst, 1);
+        starts = (uint32_t)__ballot(lane < n && (lane == 0 || x.dst != before));
     }
     // feature quad i of the edges e_first .. e_first + GA - 1: its edge (relative to e_first) and quad; false if there is none
     __device__ bool a_place(int i, int e_first, int& e, int& q) const {
@@ -140,68 +151,32 @@ template <class T, int SUB, bool WIDE> struct Wave {
         e = (int)((idx * inv_qa) >> 16); q = idx - e * qa;
         return e < GA && e_first + e < n;
     }
-    // Loads go out together and unconditionally (places that do not exist repeat the batch's last edge or the row's last quad): a branch around each
-    // would make the wave wait for one row at a time.
+    // Loads go out unconditionally (places that do not exist repeat an edge or the row's last quad): a branch around each would make the wave wait
+    // for one row at a time.
     typedef typename Quad<T>::type Raw;
-    __device__ void load_a(Raw (&a)[NA], int e_first) const {
-        const T* row = (const T*)P.a;
-        if (P.a_vec) {
+    __device__ void load_a(Raw (&a)[NA], int64_t base, int n, int e_first) const {
 #pragma unroll
-            for (int i = 0; i < NA; ++i) {
-                int e, q;
-                a_place(i, e_first, e, q);
-                a[i] = whole_quad<T>(row + (base + min(e_first + e, n - 1)) * P.a_stride + 4 * q);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < NA; ++i) {
-                int e, q;
-                a_place(i, e_first, e, q);
-                a[i] = part_quad<T>(row + (base + min(e_first + e, n - 1)) * P.a_stride + 4 * q, HK - 4 * q);
-            }
+        for (int i = 0; i < NA; ++i) {
+            const int idx = i * 64 + lane, e = (int)((idx * inv_qa) >> 16), q = idx - e * qa;
+            a[i] = load_quad<T, VEC>((const T*)P.a + (base + min(e_first + e, n - 1)) * P.a_stride + 4 * q, HK - 4 * q);
         }
     }
-    template <int G> __device__ void load_v(Raw (&v)[G][NV], int e_first) const {
-        const T* row = (const T*)P.v;
-        if (P.v_vec) {
+    // the lane's quads of a row of H D elements
+    __device__ void load_row(Raw (&v)[NV], const T* row) const {
 #pragma unroll
-            for (int e = 0; e < G; ++e)
-#pragma unroll
-                for (int j = 0; j < NV; ++j) v[e][j] = whole_quad<T>(row + (base + min(e_first + e, n - 1)) * P.v_stride + 4 * min(j * 64 + lane, qv - 1));
-        } else {
-#pragma unroll
-            for (int e = 0; e < G; ++e)
-#pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    const int q = min(j * 64 + lane, qv - 1);
-                    v[e][j] = part_quad<T>(row + (base + min(e_first + e, n - 1)) * P.v_stride + 4 * q, HD - 4 * q);
-                }
+        for (int j = 0; j < NV; ++j) {
+            const int q = min(j * 64 + lane, qv - 1);
+            v[j] = load_quad<T, VEC>(row + 4 * q, HD - 4 * q);
         }
     }
-    // rows of a (n_dst, H D) tensor at the edges' destinations
-    template <int G> __device__ void load_at_dst(Raw (&v)[G][NV], const T* rows, int vec, int e_first) const {
-        if (vec) {
-#pragma unroll
-            for (int e = 0; e < G; ++e)
-#pragma unroll
-                for (int j = 0; j < NV; ++j) v[e][j] = whole_quad<T>(rows + (int64_t)__builtin_amdgcn_readfirstlane(e_dst[min(e_first + e, n - 1)]) * HD + 4 * min(j * 64 + lane, qv - 1));
-        } else {
-#pragma unroll
-            for (int e = 0; e < G; ++e)
-#pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    const int q = min(j * 64 + lane, qv - 1);
-                    v[e][j] = part_quad<T>(rows + (int64_t)__builtin_amdgcn_readfirstlane(e_dst[min(e_first + e, n - 1)]) * HD + 4 * q, HD - 4 * q);
-                }
-        }
-    }
+    __device__ const T* value_row(int64_t e) const { return (const T*)P.v + min(e, e1 - 1) * P.v_stride; }
     __device__ float dropped(int64_t edge, int h) const {
         if (!P.threshold) return 1.0f;
         const Words x = dropout_words((uint32_t)edge, (uint32_t)(h >> 2), offset, seed);
         const uint32_t lo = h & 1 ? x.w[1] : x.w[0], hi = h & 1 ? x.w[3] : x.w[2];
         return (h & 2 ? hi : lo) >= P.threshold ? P.keep_scale : 0.0f;
     }
-    // t of the edges e_first .. e_first + GA - 1 (and their dropout factors) into LDS
+    // t of the edges e_first .. e_first + GA - 1 into LDS
     __device__ void logits(const Raw (&a)[NA], int e_first) {
         const int subs = sub_a == 4 ? qa : 4 * qa;
         wave_sync();
@@ -212,9 +187,9 @@ template <class T, int SUB, bool WIDE> struct Wave {
             const f4 wq = *(const f4*)(w + 4 * q);
             f4 x;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = 4 * q + j < HK ? act((float)a[i][j]) * wq[j] : 0.0f;
-            if (sub_a == 4) part[e * subs + q] = (x[0] + x[1]) + (x[2] + x[3]);
-            else *(f4*)(part + e * subs + 4 * q) = x;
+            for (int j = 0; j < 4; ++j) x[j] = act((float)a[i][j]);          // (0 where the row has no such element)
+            if (sub_a == 4) part[e * subs + q] = fmaf(x[3], wq[3], fmaf(x[2], wq[2], fmaf(x[1], wq[1], x[0] * wq[0])));
+            else *(f4*)(part + e * subs + 4 * q) = x * wq;
         }
         wave_sync();
         for (int idx = lane; idx < GA * H; idx += 64) {
@@ -227,7 +202,6 @@ template <class T, int SUB, bool WIDE> struct Wave {
             if (l == -__builtin_inff()) x = -__builtin_inf();          // a masked edge takes no part whatever its features hold
             if (x == __builtin_inf()) x = __builtin_nan("");
             t[eb * H + h] = x;
-            keep[eb * H + h] = eb < n ? dropped(base + eb, h) : 0.0f;
         }
     }
 };
@@ -240,9 +214,10 @@ template <int NV, int PARTS> struct Row {
     __device__ void clear() {
         for (int j = 0; j < NV; ++j) { acc[j] = f4{0, 0, 0, 0}; for (int p = 0; p < PARTS; ++p) { m[j][p] = -__builtin_inf(); sum[j][p] = 0.0f; } }
     }
-    // another (weighted) term with logit x: weight of the old sum and of the term
+    // a sum relative to x comes in (x = -inf: an empty one): factors of the old sum and of the new one
     __device__ static void weights(double& m, double x, float& w_old, float& w_new) {
-        if (x > m || x != x) { w_old = m == -__builtin_inf() ? 0.0f : exp_d(m - x); w_new = 1.0f; if (x != x) w_old = w_new = __builtin_nanf(""); m = x; }
+        if (x == -__builtin_inf()) w_old = w_new = 1.0f;          // nothing (or NaN, which its sum holds)
+        else if (x > m) { w_old = m == -__builtin_inf() ? 0.0f : exp_d(m - x); w_new = 1.0f; m = x; }
         else { w_old = 1.0f; w_new = exp_d(x - m); }
     }
 };
@@ -251,10 +226,9 @@ template <int NV, int PARTS> struct Row {
 // first row, slot 1 its last one.
 template <int NV, int PARTS> struct Record { f4 acc[NV]; double m[NV][PARTS]; float sum[NV][PARTS]; };
 
-template <class T, int SUB, bool WIDE> __device__ inline void
+template <class T, int SUB, bool VEC, bool WIDE> __device__ inline void
 finish_row(const Args& P, int row, const Row<WIDE ? 4 : 1, 4 / SUB>& r, int lane, int qv, int HD, T* out, float* out32, double* norm) {
     constexpr int NV = WIDE ? 4 : 1, PARTS = 4 / SUB;
-    const int vec = (HD & 3) == 0;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int q = j * 64 + lane;
@@ -268,14 +242,14 @@ finish_row(const Args& P, int row, const Row<WIDE ? 4 : 1, 4 / SUB>& r, int lane
             const int c = 4 * q + p * SUB;
             if (norm && c < HD && c % P.d == 0) *(d2*)(norm + 2 * ((int64_t)row * P.heads + c / P.d)) = d2{r.m[j][p], (double)inv};
         }
-        store_quad(out + (int64_t)row * HD + 4 * q, o, vec, HD - 4 * q);
-        if (out32) store_quad(out32 + (int64_t)row * HD + 4 * q, o, vec, HD - 4 * q);
+        store_quad<T, VEC>(out + (int64_t)row * HD + 4 * q, o, HD - 4 * q);
+        if (out32) store_quad<float, VEC>(out32 + (int64_t)row * HD + 4 * q, o, HD - 4 * q);
     }
 }
 
-template <class T, int SUB, bool WIDE> __global__ __launch_bounds__(256)
+template <class T, int SUB, bool VEC, bool WIDE> __global__ __launch_bounds__(256)
 void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, int64_t* rng_used) {
-    typedef Wave<T, SUB, WIDE> W;
+    typedef Wave<T, SUB, VEC, WIDE> W;
     constexpr int NV = W::NV, PARTS = W::PARTS, GA = W::GA;
     extern __shared__ __align__(16) char lds[];
     if (rng_used && P.threshold && blockIdx.x == 0 && threadIdx.x < 2) rng_used[threadIdx.x] = P.rng[threadIdx.x];
@@ -293,7 +267,7 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
         }
         return;
     }
-    W w(P, lds, W::wave_bytes(P.heads));
+    W w(P, lds, W::wave_bytes(P.heads) + (size_t)kBatch * P.heads * 8);
     if (w.e0 >= w.e1) return;
     const int lane = w.lane, H = w.H, HD = w.HD, qv = w.qv;
     int head[NV][PARTS];
@@ -312,36 +286,79 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
             Record<NV, PARTS> x;
             for (int j = 0; j < NV; ++j) { x.acc[j] = r.acc[j]; for (int p = 0; p < PARTS; ++p) { x.m[j][p] = r.m[j][p]; x.sum[j][p] = r.sum[j][p]; } }
             rec[first_row ? 0 : 64] = x;
-        } else finish_row<T, SUB, WIDE>(P, cur, r, lane, qv, HD, out, out32, norm);
+        } else finish_row<T, SUB, VEC, WIDE>(P, cur, r, lane, qv, HD, out, out32, norm);
     };
+    float2* share = (float2*)w.keep;                       // [16][H] share of the piece, and that share times the dropout factor
+    double* top = (double*)(w.e_bucket + kBatch);          // [16][H] largest logit of the piece
+    typename W::Edge edge = w.request(w.e0);
+    // R value rows are always in flight: a row's registers are loaded again, R edges ahead, as soon as it has been added
+    constexpr int R = W::R;
+    typename W::Raw a[W::NA], v[R][NV];
+    w.load_a(a, w.e0, (int)min((int64_t)kBatch, w.e1 - w.e0), 0);
+#pragma unroll
+    for (int i = 0; i < R; ++i) w.load_row(v[i], w.value_row(w.e0 + i));
     for (int64_t base = w.e0; base < w.e1; base += kBatch) {
-        w.load_edges(base);
+        w.begin(base, edge);
+        edge = w.request(min(base + kBatch, w.e1 - 1));
         for (int g = 0; g < kBatch && g < w.n; g += GA) {
-            typename W::Raw a[W::NA], v[GA][NV];
-            w.load_a(a, g);
-            w.template load_v<GA>(v, g);
             w.logits(a, g);
+            // the next features are on their way while this group is summed up
+            if (g + GA < kBatch && g + GA < w.n) w.load_a(a, base, w.n, g + GA);
+            else if (base + kBatch < w.e1) w.load_a(a, base + kBatch, (int)min((int64_t)kBatch, w.e1 - base - kBatch), 0);
             wave_sync();
+            // a "piece" is what one row has in this group: shares relative to the piece's own maximum
+            const uint32_t starts = (w.starts >> g) | 1u;
+            const int live = min(GA, w.n - g);
+#pragma unroll 1
+            for (int idx = lane; idx < GA * H; idx += 64) {
+                const int e = (int)((idx * w.inv_h) >> 16), h = idx - e * H;
+                const uint32_t upto = starts & ((2u << e) - 1u), after = starts & ~((2u << e) - 1u);
+                const int from = 31 - __builtin_clz(upto), to = min(after ? __builtin_ctz(after) : GA, live);
+                double most = -__builtin_inf();
 #pragma unroll
-            for (int e = 0; e < GA; ++e) if (g + e < w.n) {
-                const int d = __builtin_amdgcn_readfirstlane(w.e_dst[g + e]);
-                if (d != cur) { flush(false); cur = d; first_row = false; r.clear(); }
+                for (int k = 0; k < GA; ++k) {
+                    const double o = w.t[(g + k) * H + h];
+                    if (k >= from && k < to) most = __builtin_fmax(most, o);
+                }
+                const double x = w.t[(g + e) * H + h];
+                const float p = x == -__builtin_inf() ? 0.0f : exp_d(x - most);
+                share[(g + e) * H + h] = float2{p, e < live ? p * w.dropped(base + g + e, h) : 0.0f};
+                top[(g + e) * H + h] = most;
+            }
+            wave_sync();
+            float scale[NV][PARTS];
+#pragma unroll 1
+            for (int s = 0; s < GA; s += R)
 #pragma unroll
-                for (int j = 0; j < NV; ++j)
+            for (int i = 0; i < R; ++i) {
+                const int e = s + i;
+                if (g + e < w.n) {
+                    if ((starts >> e) & 1u) {
+                        const int d = __builtin_amdgcn_readfirstlane(w.e_dst[g + e]);
+                        if (d != cur) { flush(false); cur = d; first_row = false; r.clear(); }
 #pragma unroll
-                    for (int p = 0; p < PARTS; ++p) {
-                        const double x = w.t[(g + e) * H + head[j][p]];
-                        if (x == -__builtin_inf()) continue;
-                        const float kp = w.keep[(g + e) * H + head[j][p]];
-                        float w_old, w_new;
-                        Row<NV, PARTS>::weights(r.m[j][p], x, w_old, w_new);
-                        r.sum[j][p] = r.sum[j][p] * w_old + w_new;
+                        for (int j = 0; j < NV; ++j)
 #pragma unroll
-                        for (int i = 0; i < SUB; ++i) {
-                            const float old = r.acc[j][p * SUB + i] * w_old;
-                            r.acc[j][p * SUB + i] = kp != 0.0f ? old + w_new * kp * (float)v[e][j][p * SUB + i] : old;
-                        }
+                            for (int p = 0; p < PARTS; ++p) {
+                                float w_old;
+                                Row<NV, PARTS>::weights(r.m[j][p], top[(g + e) * H + head[j][p]], w_old, scale[j][p]);
+                                r.sum[j][p] *= w_old;
+#pragma unroll
+                                for (int c = 0; c < SUB; ++c) r.acc[j][p * SUB + c] *= w_old;
+                            }
                     }
+#pragma unroll
+                    for (int j = 0; j < NV; ++j)
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p) {
+                            const float2 f = share[(g + e) * H + head[j][p]];
+                            const float k = f.y * scale[j][p];
+                            r.sum[j][p] = fmaf(f.x, scale[j][p], r.sum[j][p]);
+#pragma unroll
+                            for (int c = 0; c < SUB; ++c) r.acc[j][p * SUB + c] = k == 0.0f ? r.acc[j][p * SUB + c] : fmaf(k, (float)v[i][j][p * SUB + c], r.acc[j][p * SUB + c]);
+                        }
+                }
+                w.load_row(v[i], w.value_row(base + g + e + R));
             }
             wave_sync();
         }
@@ -351,7 +368,7 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
 
 // Rows that cross ranges: workgroup b looks at the border between ranges b and b + 1, and joins a row whose first crossing that is.  Each wave joins
 // every fourth record, then the four are joined in order.
-template <class T, int SUB, bool WIDE> __global__ __launch_bounds__(256)
+template <class T, int SUB, bool VEC, bool WIDE> __global__ __launch_bounds__(256)
 void k_attn_merge(Args P, T* out, float* out32, double* norm, const void* records) {
     constexpr int NV = WIDE ? 4 : 1, PARTS = 4 / SUB;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, H = P.heads, HD = H * P.d, qv = (HD + 3) >> 2;
@@ -369,12 +386,11 @@ void k_attn_merge(Args P, T* out, float* out32, double* norm, const void* record
         for (int j = 0; j < NV; ++j)
 #pragma unroll
             for (int p = 0; p < PARTS; ++p) {
-                if (m[j][p] == -__builtin_inf()) continue;
                 float w_old, w_new;
                 Row<NV, PARTS>::weights(r.m[j][p], m[j][p], w_old, w_new);
-                r.sum[j][p] = r.sum[j][p] * w_old + sum[j][p] * w_new;
+                r.sum[j][p] = fmaf(sum[j][p], w_new, r.sum[j][p] * w_old);
 #pragma unroll
-                for (int i = 0; i < SUB; ++i) r.acc[j][p * SUB + i] = r.acc[j][p * SUB + i] * w_old + acc[j][p * SUB + i] * w_new;
+                for (int i = 0; i < SUB; ++i) r.acc[j][p * SUB + i] = fmaf(acc[j][p * SUB + i], w_new, r.acc[j][p * SUB + i] * w_old);
             }
     };
 #pragma unroll 2
@@ -390,7 +406,7 @@ void k_attn_merge(Args P, T* out, float* out32, double* norm, const void* record
     __syncthreads();
     if (wave > 0) return;
     for (int o = 0; o < kWaves - 1; ++o) join(share[o][lane].acc, share[o][lane].m, share[o][lane].sum);
-    finish_row<T, SUB, WIDE>(P, row, r, lane, qv, HD, out, out32, norm);
+    finish_row<T, SUB, VEC, WIDE>(P, row, r, lane, qv, HD, out, out32, norm);
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------------------------------
@@ -404,7 +420,7 @@ void k_attn_delta(int64_t n_rows, int H, int D, const T* grad, const float* out3
     const T* g = grad + row * HD; const float* o = out32 + row * HD;
     for (int h = 0; h < H; ++h) {
         float s = 0.0f;
-        for (int c = lane; c < D; c += 64) s += (float)g[h * D + c] * o[h * D + c];
+        for (int c = lane; c < D; c += 64) s = fmaf((float)g[h * D + c], o[h * D + c], s);
 #pragma unroll
         for (int x = 32; x >= 1; x >>= 1) s += __shfl_xor(s, x, 64);
         if (lane == 0) delta[row * H + h] = s;
@@ -412,15 +428,15 @@ void k_attn_delta(int64_t n_rows, int H, int D, const T* grad, const float* out3
 }
 
 struct BackArgs {
-    const double* norm; const float* delta; const void* grad; int grad_vec;
+    const double* norm; const float* delta; const void* grad;
     void* da; void* dv; float* dl;          // any of them may be null
     float* param_rows;                      // (workgroups, H K + B H) sums of dw and dT, or null
 };
 
-template <class T, int SUB, bool WIDE> __global__ __launch_bounds__(256)
+template <class T, int SUB, bool VEC, bool WIDE> __global__ __launch_bounds__(256)
 void k_attn_backward(Args P, BackArgs B) {
-    typedef Wave<T, SUB, WIDE> W;
-    constexpr int NV = W::NV, NA = W::NA, PARTS = W::PARTS, GA = W::GA, GV = WIDE ? 2 : 8;      // GV value rows at a time
+    typedef Wave<T, SUB, VEC, WIDE> W;
+    constexpr int NV = W::NV, NA = W::NA, PARTS = W::PARTS, GA = W::GA, R = W::R;
     extern __shared__ __align__(16) char lds[];
     const int BH = P.n_buckets * P.heads;
     const size_t own = W::wave_bytes(P.heads) + (size_t)kBatch * P.heads * 4 + (size_t)((BH + 1) & ~1) * 4;
@@ -444,87 +460,114 @@ void k_attn_backward(Args P, BackArgs B) {
         head_a[i] = min(4 * q / P.k, H - 1);
     }
 
-    for (int64_t base = w.e0; base < w.e1; base += kBatch) {
-        w.load_edges(base);
-        for (int g = 0; g < kBatch && g < w.n; g += GA) {
-            typename W::Raw a[NA];
-            w.load_a(a, g);
-            w.logits(a, g);
-            wave_sync();
-            for (int idx = lane; idx < GA * H; idx += 64) {          // t becomes p
-                const int e = (int)((idx * w.inv_h) >> 16), h = idx - e * H, eb = g + e;
-                if (eb >= w.n) continue;
-                const double x = w.t[eb * H + h];
-                const d2 at = *(const d2*)(B.norm + 2 * ((int64_t)w.e_dst[eb] * H + h));
-                w.t[eb * H + h] = x == -__builtin_inf() ? 0.0 : (double)(exp_d(x - at[0]) * (float)at[1]);
-            }
+    if (w.e0 < w.e1) {
+        // value rows and the upper gradient at their destinations, R edges ahead; a batch's per-edge values and features one batch ahead
+        typename W::Edge edge = w.request(w.e0), next = edge;
+        typename W::Raw a[NA], a_next[NA], v[R][NV], up[R][NV];
+        w.load_a(a_next, w.e0, (int)min((int64_t)kBatch, w.e1 - w.e0), 0);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            w.load_row(v[i], w.value_row(w.e0 + i));
+            w.load_row(up[i], (const T*)B.grad + (int64_t)__builtin_amdgcn_readlane(edge.dst, i) * HD);
+        }
+        for (int64_t base = w.e0; base < w.e1; base += kBatch) {
+            w.begin(base, edge);
+            next = w.request(min(base + kBatch, w.e1 - 1));
             wave_sync();
 #pragma unroll 1
-            for (int s = g; s < g + GA && s < w.n; s += GV) {
-                typename W::Raw v[GV][NV], up[GV][NV];
-                w.template load_v<GV>(v, s);
-                w.template load_at_dst<GV>(up, (const T*)B.grad, B.grad_vec, s);
+            for (int g = 0; g < kBatch && g < w.n; g += GA) {
+#pragma unroll
+                for (int i = 0; i < NA; ++i) a[i] = a_next[i];
+                if (g + GA < kBatch && g + GA < w.n) w.load_a(a_next, base, w.n, g + GA);
+                else if (base + kBatch < w.e1) w.load_a(a_next, base + kBatch, (int)min((int64_t)kBatch, w.e1 - base - kBatch), 0);
+                const int pairs = min(GA, w.n - g) * H;
+                // the first 64 of the group's edges and heads (all of them for up to 4 heads): what their rows keep, on its way early
+                d2 norm0 = {0.0, 0.0};
+                {
+                    const int at = w.e_dst[g + (int)((min(lane, pairs - 1) * w.inv_h) >> 16)] * H + min(lane, pairs - 1) % H;
+                    norm0 = *(const d2*)(B.norm + 2 * (int64_t)at);
+                }
+                w.logits(a, g);
                 wave_sync();
+                for (int idx = lane; idx < pairs; idx += 64) {          // t becomes p
+                    const int e = (int)((idx * w.inv_h) >> 16), h = idx - e * H, eb = g + e;
+                    const double x = w.t[eb * H + h];
+                    const d2 at = idx == lane ? norm0 : *(const d2*)(B.norm + 2 * ((int64_t)w.e_dst[eb] * H + h));
+                    w.t[eb * H + h] = x == -__builtin_inf() ? 0.0 : (double)(exp_d(x - at[0]) * (float)at[1]);
+                    w.keep[eb * H + h] = w.dropped(base + eb, h);
+                }
+                wave_sync();
+#pragma unroll 1
+                for (int s = g; s < g + GA && s < w.n; s += R) {
 #pragma unroll
-                for (int e = 0; e < GV; ++e) if (s + e < w.n) {
+                    for (int i = 0; i < R; ++i) {
+                        if (s + i < w.n) {
 #pragma unroll
-                    for (int j = 0; j < NV; ++j) {
-                        const int q = j * 64 + lane;
-                        if (q >= qv) continue;
-                        f4 o;
+                            for (int j = 0; j < NV; ++j) {
+                                const int q = j * 64 + lane;
+                                f4 o;
+                                float dot[PARTS];
 #pragma unroll
-                        for (int p = 0; p < PARTS; ++p) {
-                            const int at = (s + e) * H + head[j][p];
-                            const float f = (float)w.t[at] * w.keep[at];
-                            float dot = 0.0f;
+                                for (int p = 0; p < PARTS; ++p) {
+                                    const int at = (s + i) * H + head[j][p];
+                                    const float f = (float)w.t[at] * w.keep[at];
+                                    dot[p] = 0.0f;
 #pragma unroll
-                            for (int i = 0; i < SUB; ++i) {
-                                const int c = p * SUB + i;
-                                const float u = (float)up[e][j][c];
-                                o[c] = f == 0.0f ? 0.0f : f * u;
-                                dot += (float)v[e][j][c] * u;
+                                    for (int k = 0; k < SUB; ++k) {
+                                        const int c = p * SUB + k;
+                                        const float u = (float)up[i][j][c];
+                                        o[c] = f == 0.0f ? 0.0f : f * u;
+                                        dot[p] = fmaf((float)v[i][j][c], u, dot[p]);
+                                    }
+                                }
+                                if (q < qv) {
+#pragma unroll
+                                    for (int p = 0; p < PARTS; ++p) w.part[i * subs + q * PARTS + p] = dot[p];
+                                    if (B.dv) store_quad<T, VEC>((T*)B.dv + (base + s + i) * HD + 4 * q, o, HD - 4 * q);
+                                }
                             }
-                            w.part[e * subs + q * PARTS + p] = dot;
                         }
-                        if (B.dv) store_quad((T*)B.dv + (base + s + e) * HD + 4 * q, o, (HD & 3) == 0, HD - 4 * q);
+                        const int ahead = s + i + R, dst = ahead < kBatch ? __builtin_amdgcn_readlane(edge.dst, ahead) : __builtin_amdgcn_readlane(next.dst, ahead - kBatch);
+                        w.load_row(v[i], w.value_row(base + ahead));
+                        w.load_row(up[i], (const T*)B.grad + (int64_t)dst * HD);
                     }
+                    wave_sync();
+                    const int last = min(s + R, w.n) - g;
+                    for (int idx = lane + (s - g) * H, k = lane; idx < last * H; idx += 64, k += 64) {
+                        const int i = (int)((k * w.inv_h) >> 16), h = k - i * H, eb = s + i;
+                        float dot = 0.0f;
+                        for (int c = 0; c < per_head; ++c) dot += w.part[i * subs + h * per_head + c];
+                        const float p = (float)w.t[eb * H + h], kp = w.keep[eb * H + h];
+                        dt[eb * H + h] = p == 0.0f ? 0.0f : p * ((kp == 0.0f ? 0.0f : kp * dot) - B.delta[(int64_t)w.e_dst[eb] * H + h]);
+                    }
+                    wave_sync();
                 }
+                if (B.dl && lane < GA && g + lane < w.n) {
+                    float s = 0.0f;
+                    for (int h = 0; h < H; ++h) s += dt[(g + lane) * H + h];
+                    B.dl[base + g + lane] = s;
+                }
+#pragma unroll
+                for (int i = 0; i < NA; ++i) {
+                    int e, q;
+                    if (!w.a_place(i, g, e, q)) continue;
+                    const f4 wq = *(const f4*)(w.w + 4 * q);
+                    f4 o;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int h = w.sub_a == 4 ? head_a[i] : min((4 * q + j) / P.k, H - 1);
+                        const float f = dt[(g + e) * H + h], x = (float)a[i][j], sg = sigmoid(x);
+                        const float slope = kActNorm * fmaf(0.8f * sg, fmaf(x, 1.0f - sg, 1.0f), 0.2f);
+                        o[j] = f == 0.0f ? 0.0f : f * wq[j] * slope;
+                        dw[i][j] = f == 0.0f ? dw[i][j] : fmaf(f, kActNorm * x * fmaf(0.8f, sg, 0.2f), dw[i][j]);
+                    }
+                    if (B.da) store_quad<T, VEC>((T*)B.da + (base + g + e) * HK + 4 * q, o, HK - 4 * q);
+                }
+                if (BH && B.param_rows && lane < H)          // in the edges' order: lane h alone adds to the sums of its head
+                    for (int e = 0; e < GA && g + e < w.n; ++e) bins[w.e_bucket[g + e] * H + lane] += dt[(g + e) * H + lane];
                 wave_sync();
-                for (int idx = lane; idx < GV * H; idx += 64) {
-                    const int e = (int)((idx * w.inv_h) >> 16), h = idx - e * H, eb = s + e;
-                    if (eb >= w.n) continue;
-                    float dot = 0.0f;
-                    for (int i = 0; i < per_head; ++i) dot += w.part[e * subs + h * per_head + i];
-                    const float p = (float)w.t[eb * H + h], kp = w.keep[eb * H + h];
-                    const float dp = kp == 0.0f ? 0.0f : kp * dot;
-                    dt[eb * H + h] = p == 0.0f ? 0.0f : p * (dp - B.delta[(int64_t)w.e_dst[eb] * H + h]);
-                }
             }
-            wave_sync();
-            if (B.dl && lane < GA && g + lane < w.n) {
-                float s = 0.0f;
-                for (int h = 0; h < H; ++h) s += dt[(g + lane) * H + h];
-                B.dl[base + g + lane] = s;
-            }
-#pragma unroll
-            for (int i = 0; i < NA; ++i) {
-                int e, q;
-                if (!w.a_place(i, g, e, q)) continue;
-                const f4 wq = *(const f4*)(w.w + 4 * q);
-                f4 o;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int h = w.sub_a == 4 ? head_a[i] : min((4 * q + j) / P.k, H - 1);
-                    const float f = dt[(g + e) * H + h], x = (float)a[i][j], sg = sigmoid(x);
-                    const float slope = kActNorm * (0.2f + 0.8f * sg * (1.0f + x * (1.0f - sg)));
-                    o[j] = f == 0.0f ? 0.0f : f * wq[j] * slope;
-                    dw[i][j] += f == 0.0f ? 0.0f : f * kActNorm * x * (0.2f + 0.8f * sg);
-                }
-                if (B.da) store_quad((T*)B.da + (base + g + e) * HK + 4 * q, o, (HK & 3) == 0, HK - 4 * q);
-            }
-            if (BH && B.param_rows && lane < H)          // in the edges' order: lane h alone adds to the sums of its head
-                for (int e = 0; e < GA && g + e < w.n; ++e) bins[w.e_bucket[g + e] * H + lane] += dt[(g + e) * H + lane];
-            wave_sync();
+            edge = next;
         }
     }
     if (!B.param_rows) return;
