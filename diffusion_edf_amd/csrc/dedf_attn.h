@@ -26,6 +26,10 @@ namespace attn {
 
 constexpr int kBatch = 16;                 // edges per step of a wave
 constexpr int kWaves = 4;                  // waves per workgroup
+// Waves a SIMD holds, by the registers of each instantiation; a launch has as many waves as are resident at once, each with one range of edges.  More
+// waves than that run in two rounds, of which the second is half empty: 1.97 M edges, float32, backward with 2 048 waves 0.95 ms, with 3 072 1.13 ms.
+constexpr int forward_waves(int nv, int sub, int bytes) { return nv == 1 ? (bytes == 2 && sub > 1 ? 4 : 3) : nv == 2 ? (sub == 4 ? 3 : sub) : (sub == 4 ? 2 : 1); }
+constexpr int kBackwardWaves = 2;
 constexpr float kActNorm = 1.531320475574866f;
 constexpr double kLog2e = 1.4426950408889634;
 
@@ -86,11 +90,12 @@ __device__ inline int bucket_of(const float* bounds, int n, float x) {
 }
 
 // what both directions share: the wave's place, its LDS, the batch's per-edge values, the logits
-//   SUB: a quad is cut into 4 / SUB parts that each lie inside one head (SUB 4: head widths divisible by 4; 2: even; 1: any)
-//   WIDE: up to 4 quads per lane (value rows of up to 1 024 channels), feature rows of up to 256
-template <class T, int SUB, bool VEC, bool WIDE> struct Wave {
-    static constexpr int NV = WIDE ? 4 : 1, NA = 4, GA = WIDE ? 4 : 16;      // GA edges x feature quads fill NA loads of a wave
-    static constexpr int R = WIDE ? 2 : 8;                                   // value rows in flight
+//   SUB: a quad is cut into 4 / SUB parts that each lie inside one head (4: head widths divisible by 4; 2: even; 1: any)
+//   VEC: rows consist of whole, aligned quads
+//   NV: quads of a value row a lane holds: 1 (up to 256 channels) or 2 (512), with feature rows of up to 64, or 4 (1 024) with feature rows of up to 256
+template <class T, int SUB, bool VEC, int NV> struct Wave {
+    static constexpr int NA = 4, GA = NV == 4 ? 4 : 16;                      // GA edges x feature quads fill NA loads of a wave
+    static constexpr int R = 8 / NV;                                         // value rows in flight
     static constexpr int PARTS = 4 / SUB;
     static constexpr int kPart = SUB == 1 ? 2048 : 1024;                     // floats of the partial-sum buffer
     const Args& P;
@@ -226,9 +231,9 @@ template <int NV, int PARTS> struct Row {
 // first row, slot 1 its last one.
 template <int NV, int PARTS> struct Record { f4 acc[NV]; double m[NV][PARTS]; float sum[NV][PARTS]; };
 
-template <class T, int SUB, bool VEC, bool WIDE> __device__ inline void
-finish_row(const Args& P, int row, const Row<WIDE ? 4 : 1, 4 / SUB>& r, int lane, int qv, int HD, T* out, float* out32, double* norm) {
-    constexpr int NV = WIDE ? 4 : 1, PARTS = 4 / SUB;
+template <class T, int SUB, bool VEC, int NV> __device__ inline void
+finish_row(const Args& P, int row, const Row<NV, 4 / SUB>& r, int lane, int qv, int HD, T* out, float* out32, double* norm) {
+    constexpr int PARTS = 4 / SUB;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int q = j * 64 + lane;
@@ -247,10 +252,10 @@ finish_row(const Args& P, int row, const Row<WIDE ? 4 : 1, 4 / SUB>& r, int lane
     }
 }
 
-template <class T, int SUB, bool VEC, bool WIDE> __global__ __launch_bounds__(256)
+template <class T, int SUB, bool VEC, int NV> __global__ __launch_bounds__(256, forward_waves(NV, SUB, sizeof(T)))
 void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, int64_t* rng_used) {
-    typedef Wave<T, SUB, VEC, WIDE> W;
-    constexpr int NV = W::NV, PARTS = W::PARTS, GA = W::GA;
+    typedef Wave<T, SUB, VEC, NV> W;
+    constexpr int PARTS = W::PARTS, GA = W::GA;
     extern __shared__ __align__(16) char lds[];
     if (rng_used && P.threshold && blockIdx.x == 0 && threadIdx.x < 2) rng_used[threadIdx.x] = P.rng[threadIdx.x];
     const int edge_blocks = (P.n_waves + kWaves - 1) / kWaves;
@@ -286,7 +291,7 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
             Record<NV, PARTS> x;
             for (int j = 0; j < NV; ++j) { x.acc[j] = r.acc[j]; for (int p = 0; p < PARTS; ++p) { x.m[j][p] = r.m[j][p]; x.sum[j][p] = r.sum[j][p]; } }
             rec[first_row ? 0 : 64] = x;
-        } else finish_row<T, SUB, VEC, WIDE>(P, cur, r, lane, qv, HD, out, out32, norm);
+        } else finish_row<T, SUB, VEC, NV>(P, cur, r, lane, qv, HD, out, out32, norm);
     };
     float2* share = (float2*)w.keep;                       // [16][H] share of the piece, and that share times the dropout factor
     double* top = (double*)(w.e_bucket + kBatch);          // [16][H] largest logit of the piece
@@ -368,9 +373,9 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
 
 // Rows that cross ranges: workgroup b looks at the border between ranges b and b + 1, and joins a row whose first crossing that is.  Each wave joins
 // every fourth record, then the four are joined in order.
-template <class T, int SUB, bool VEC, bool WIDE> __global__ __launch_bounds__(256)
+template <class T, int SUB, bool VEC, int NV> __global__ __launch_bounds__(256)
 void k_attn_merge(Args P, T* out, float* out32, double* norm, const void* records) {
-    constexpr int NV = WIDE ? 4 : 1, PARTS = 4 / SUB;
+    constexpr int PARTS = 4 / SUB;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, H = P.heads, HD = H * P.d, qv = (HD + 3) >> 2;
     const int64_t border = ((int64_t)blockIdx.x + 1) * P.range;
     const int row = P.dst[border];
@@ -406,7 +411,7 @@ void k_attn_merge(Args P, T* out, float* out32, double* norm, const void* record
     __syncthreads();
     if (wave > 0) return;
     for (int o = 0; o < kWaves - 1; ++o) join(share[o][lane].acc, share[o][lane].m, share[o][lane].sum);
-    finish_row<T, SUB, VEC, WIDE>(P, row, r, lane, qv, HD, out, out32, norm);
+    finish_row<T, SUB, VEC, NV>(P, row, r, lane, qv, HD, out, out32, norm);
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------------------------------
@@ -433,10 +438,10 @@ struct BackArgs {
     float* param_rows;                      // (workgroups, H K + B H) sums of dw and dT, or null
 };
 
-template <class T, int SUB, bool VEC, bool WIDE> __global__ __launch_bounds__(256)
+template <class T, int SUB, bool VEC, int NV> __global__ __launch_bounds__(256, kBackwardWaves)
 void k_attn_backward(Args P, BackArgs B) {
-    typedef Wave<T, SUB, VEC, WIDE> W;
-    constexpr int NV = W::NV, NA = W::NA, PARTS = W::PARTS, GA = W::GA, R = W::R;
+    typedef Wave<T, SUB, VEC, NV> W;
+    constexpr int NA = W::NA, PARTS = W::PARTS, GA = W::GA, R = W::R;
     extern __shared__ __align__(16) char lds[];
     const int BH = P.n_buckets * P.heads;
     const size_t own = W::wave_bytes(P.heads) + (size_t)kBatch * P.heads * 4 + (size_t)((BH + 1) & ~1) * 4;

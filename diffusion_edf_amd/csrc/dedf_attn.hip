@@ -10,25 +10,25 @@ using namespace dedf::attn;
 namespace dedf {
 namespace attn {
 
-struct Plan { Args a; bool wide; int sub; size_t record, lds_forward, lds_backward; int blocks; };
+struct Plan { Args a; int nv, sub; size_t record, lds_forward, lds_backward; int blocks; };
 
 struct Forward {
     const Plan& p; void* out; float* out32; double* norm; int64_t* rng_used; void* records; hipStream_t st;
-    template <class T, int SUB, bool VEC, bool WIDE> int run() {
-        if (p.lds_forward > 65536 && hipFuncSetAttribute((const void*)k_attn_forward<T, SUB, VEC, WIDE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds_forward) != hipSuccess) return DEDF_ERR_RUNTIME;
+    template <class T, int SUB, bool VEC, int NV> int run() {
+        if (p.lds_forward > 65536 && hipFuncSetAttribute((const void*)k_attn_forward<T, SUB, VEC, NV>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds_forward) != hipSuccess) return DEDF_ERR_RUNTIME;
         const int empty_blocks = (p.a.n_dst + 64 * kWaves - 1) / (64 * kWaves);
-        hipLaunchKernelGGL((k_attn_forward<T, SUB, VEC, WIDE>), dim3(p.blocks + empty_blocks), dim3(256), p.lds_forward, st, p.a, (T*)out, out32, norm, records, rng_used);
-        if (p.a.n_waves > 1) hipLaunchKernelGGL((k_attn_merge<T, SUB, VEC, WIDE>), dim3(p.a.n_waves - 1), dim3(256), 0, st, p.a, (T*)out, out32, norm, (const void*)records);
+        hipLaunchKernelGGL((k_attn_forward<T, SUB, VEC, NV>), dim3(p.blocks + empty_blocks), dim3(256), p.lds_forward, st, p.a, (T*)out, out32, norm, records, rng_used);
+        if (p.a.n_waves > 1) hipLaunchKernelGGL((k_attn_merge<T, SUB, VEC, NV>), dim3(p.a.n_waves - 1), dim3(256), 0, st, p.a, (T*)out, out32, norm, (const void*)records);
         return hipGetLastError() == hipSuccess ? DEDF_OK : DEDF_ERR_RUNTIME;
     }
 };
 struct Backward {
     const Plan& p; BackArgs b; const float* out32; float* delta; float* d_alpha_dot; float* d_table; hipStream_t st;
-    template <class T, int SUB, bool VEC, bool WIDE> int run() {
-        if (p.lds_backward > 65536 && hipFuncSetAttribute((const void*)k_attn_backward<T, SUB, VEC, WIDE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds_backward) != hipSuccess) return DEDF_ERR_RUNTIME;
+    template <class T, int SUB, bool VEC, int NV> int run() {
+        if (p.lds_backward > 65536 && hipFuncSetAttribute((const void*)k_attn_backward<T, SUB, VEC, NV>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds_backward) != hipSuccess) return DEDF_ERR_RUNTIME;
         const Args& a = p.a;
         hipLaunchKernelGGL((k_attn_delta<T>), dim3((a.n_dst + kWaves - 1) / kWaves), dim3(256), 0, st, (int64_t)a.n_dst, a.heads, a.d, (const T*)b.grad, out32, delta);
-        hipLaunchKernelGGL((k_attn_backward<T, SUB, VEC, WIDE>), dim3(p.blocks), dim3(256), p.lds_backward, st, a, b);
+        hipLaunchKernelGGL((k_attn_backward<T, SUB, VEC, NV>), dim3(p.blocks), dim3(256), p.lds_backward, st, a, b);
         if (b.param_rows) {
             const int n_w = a.heads * a.k, columns = n_w + a.heads * a.n_buckets;
             hipLaunchKernelGGL(k_column_sums, dim3((columns + 15) / 16), dim3(256), 0, st, (const float*)b.param_rows, p.blocks, columns, d_alpha_dot, n_w, d_table);
@@ -37,16 +37,14 @@ struct Backward {
     }
 };
 
-template <class T, class F> int launch(int sub, bool wide, F f) {          // sub 0: rows that do not consist of whole, aligned quads
-    switch (sub) {
-        case 4: return wide ? f.template run<T, 4, true, true>() : f.template run<T, 4, true, false>();
-        case 2: return wide ? f.template run<T, 2, true, true>() : f.template run<T, 2, true, false>();
-        case 1: return wide ? f.template run<T, 1, true, true>() : f.template run<T, 1, true, false>();
-        default: return wide ? f.template run<T, 1, false, true>() : f.template run<T, 1, false, false>();
-    }
+template <class T, int SUB, bool VEC, class F> int by_width(int nv, F& f) {
+    return nv == 1 ? f.template run<T, SUB, VEC, 1>() : nv == 2 ? f.template run<T, SUB, VEC, 2>() : f.template run<T, SUB, VEC, 4>();
+}
+template <class T, class F> int launch(int sub, int nv, F f) {          // sub 0: rows that do not consist of whole, aligned quads
+    return sub == 4 ? by_width<T, 4, true>(nv, f) : sub == 2 ? by_width<T, 2, true>(nv, f) : sub == 1 ? by_width<T, 1, true>(nv, f) : by_width<T, 1, false>(nv, f);
 }
 
-#define DEDF_LAUNCHES(T, PREFIX) PREFIX template int launch<T, Forward>(int, bool, Forward); PREFIX template int launch<T, Backward>(int, bool, Backward);
+#define DEDF_LAUNCHES(T, PREFIX) PREFIX template int launch<T, Forward>(int, int, Forward); PREFIX template int launch<T, Backward>(int, int, Backward);
 #ifndef DEDF_ELEMENT
 DEDF_LAUNCHES(float, extern) DEDF_LAUNCHES(_Float16, extern) DEDF_LAUNCHES(__bf16, extern)
 #elif DEDF_ELEMENT == 0
@@ -63,10 +61,8 @@ DEDF_LAUNCHES(__bf16, )
 #ifndef DEDF_ELEMENT
 namespace {
 
-constexpr int kMostWaves = 3072;          // 256 CUs x 12: what is resident at once
+constexpr int kSimds = 1024;          // 256 CUs of 4
 constexpr size_t kMostLds = 160 * 1024;
-
-
 
 size_t element(int type) { return type == DEDF_F32 ? 4 : 2; }
 bool whole_quads(const void* p, int64_t stride, int width, int type) {
@@ -75,7 +71,7 @@ bool whole_quads(const void* p, int64_t stride, int width, int type) {
 }
 
 // `tensors`: the call's other tensors of (edges or rows, heads, k or d) in the element type
-int make_plan(const dedf_edge_attn* x, Plan& p, std::initializer_list<const void*> tensors = {}) {
+int make_plan(const dedf_edge_attn* x, bool backward, Plan& p, std::initializer_list<const void*> tensors) {
     if (!x || x->n_edges < 0 || x->n_dst < 0 || x->heads < 1 || x->k < 1 || x->d < 1 || x->n_buckets < 0) return DEDF_ERR_INVALID;
     if (x->type != DEDF_F32 && x->type != DEDF_F16 && x->type != DEDF_BF16) return DEDF_ERR_UNSUPPORTED;
     if (x->n_edges >= (int64_t)1 << 31 || x->heads > 16 || x->k > 256 || x->d > 1024 || x->heads * x->k > 256 || x->heads * x->d > 1024) return DEDF_ERR_UNSUPPORTED;
@@ -94,20 +90,21 @@ int make_plan(const dedf_edge_attn* x, Plan& p, std::initializer_list<const void
     a.n_buckets = x->n_buckets;
     a.threshold = (uint32_t)std::floor(x->dropout * 4294967296.0);
     a.keep_scale = (float)(1.0 / (1.0 - x->dropout)); a.rng = x->rng;
-    const int64_t even = (a.n_edges + kMostWaves - 1) / kMostWaves;
-    a.range = (int)std::max<int64_t>(kBatch, (even + kBatch - 1) / kBatch * kBatch);
-    a.n_waves = (int)((a.n_edges + a.range - 1) / a.range);
     bool whole = whole_quads(a.a, a.a_stride, a.heads * a.k, x->type) && whole_quads(a.v, a.v_stride, a.heads * a.d, x->type);
     for (const void* t : tensors) whole = whole && whole_quads(t, 0, 0, x->type);
     p.sub = !whole ? 0 : x->d % 4 == 0 ? 4 : x->d % 2 == 0 ? 2 : 1;
-    p.wide = a.heads * a.k > 64 || a.heads * a.d > 256;
+    p.nv = a.heads * a.k > 64 || a.heads * a.d > 512 ? 4 : a.heads * a.d > 256 ? 2 : 1;
+    const int most = kSimds * (backward ? kBackwardWaves : forward_waves(p.nv, p.sub ? p.sub : 1, (int)element(x->type)));
+    const int64_t even = (a.n_edges + most - 1) / most;
+    a.range = (int)std::max<int64_t>(kBatch, (even + kBatch - 1) / kBatch * kBatch);
+    a.n_waves = (int)((a.n_edges + a.range - 1) / a.range);
     p.blocks = (a.n_waves + kWaves - 1) / kWaves;
-    const auto record = [](auto r) { return sizeof(r) * 64 * 2; };
-    p.record = p.wide ? (p.sub == 4 ? record(Record<4, 1>{}) : p.sub == 2 ? record(Record<4, 2>{}) : record(Record<4, 4>{}))
-                      : (p.sub == 4 ? record(Record<1, 1>{}) : p.sub == 2 ? record(Record<1, 2>{}) : record(Record<1, 4>{}));
-    const size_t own = p.sub <= 1 ? Wave<float, 1, true, false>::wave_bytes(a.heads) : Wave<float, 4, true, false>::wave_bytes(a.heads);          // (whatever the type and width)
+    const int parts = p.sub == 4 ? 1 : p.sub == 2 ? 2 : 4;          // (as the kernels' Record<nv, parts>)
+    p.record = (size_t)(p.nv * 16 + p.nv * parts * 12 + 15) / 16 * 16 * 64 * 2;
+    static_assert(sizeof(Record<1, 1>) == 32 && sizeof(Record<1, 4>) == 64 && sizeof(Record<2, 2>) == 80 && sizeof(Record<4, 4>) == 256, "records are as large as computed here");
+    const size_t own = p.sub <= 1 ? Wave<float, 1, true, 1>::wave_bytes(a.heads) : Wave<float, 4, true, 1>::wave_bytes(a.heads);          // (whatever the type and width)
     const int BH = a.n_buckets * a.heads;
-    const size_t shared = Wave<float, 4, true, false>::shared_bytes(a.heads * a.k, a.heads, a.n_buckets);
+    const size_t shared = Wave<float, 4, true, 1>::shared_bytes(a.heads * a.k, a.heads, a.n_buckets);
     p.lds_forward = shared + kWaves * (own + (size_t)kBatch * a.heads * 8);
     p.lds_backward = shared + kWaves * ((own + (size_t)kBatch * a.heads * 4 + (size_t)((BH + 1) & ~1) * 4 + 15) & ~(size_t)15);
     if (p.lds_forward > kMostLds || p.lds_backward > kMostLds) return DEDF_ERR_UNSUPPORTED;
@@ -115,8 +112,8 @@ int make_plan(const dedf_edge_attn* x, Plan& p, std::initializer_list<const void
 }
 size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 size_t forward_bytes(const Plan& p) { return (size_t)p.blocks * kWaves * p.record; }
-template <class F> int by_shape(int type, int sub, bool wide, F f) {
-    return type == DEDF_F32 ? launch<float>(sub, wide, f) : type == DEDF_F16 ? launch<_Float16>(sub, wide, f) : launch<__bf16>(sub, wide, f);
+template <class F> int by_shape(int type, int sub, int nv, F f) {
+    return type == DEDF_F32 ? launch<float>(sub, nv, f) : type == DEDF_F16 ? launch<_Float16>(sub, nv, f) : launch<__bf16>(sub, nv, f);
 }
 size_t backward_bytes(const Plan& p) {
     return up16((size_t)p.a.n_dst * p.a.heads * 4) + (size_t)p.blocks * (p.a.heads * (p.a.k + p.a.n_buckets)) * 4;
@@ -136,24 +133,27 @@ int dedf_edge_segments(const int64_t* edge_dst, int64_t n_edges, int n_dst, int3
 
 size_t dedf_edge_attention_scratch_bytes(const dedf_edge_attn* x, int backward) {
     Plan p;
-    if (make_plan(x, p) != DEDF_OK) return 0;
-    return backward ? backward_bytes(p) : forward_bytes(p);
+    if (make_plan(x, backward != 0, p, {}) != DEDF_OK) return 0;
+    if (backward) return backward_bytes(p);
+    // (outputs that are not aligned to whole quads choose another instantiation: room for either)
+    const size_t aligned = forward_bytes(p);
+    return make_plan(x, false, p, {reinterpret_cast<const void*>(1)}) == DEDF_OK ? std::max(aligned, forward_bytes(p)) : aligned;
 }
 
 int dedf_edge_attention(const dedf_edge_attn* x, void* out, float* out_f, double* norm, int64_t* rng_used, void* scratch, size_t scratch_bytes, void* stream) {
     Plan p;
-    const int rc = make_plan(x, p, {out, out_f});
+    const int rc = make_plan(x, false, p, {out, out_f});
     if (rc != DEDF_OK) return rc;
     if (p.a.n_dst == 0) return DEDF_OK;
     if (!out || scratch_bytes < forward_bytes(p) || (forward_bytes(p) > 0 && !scratch) || (reinterpret_cast<uintptr_t>(scratch) & 15)) return DEDF_ERR_INVALID;
     Forward f{p, out, out_f, norm, rng_used, scratch, static_cast<hipStream_t>(stream)};
-    return by_shape(x->type, p.sub, p.wide, f);
+    return by_shape(x->type, p.sub, p.nv, f);
 }
 
 int dedf_edge_attention_backward(const dedf_edge_attn* x, const double* norm, const float* out_f, const void* grad_out, void* d_alpha, void* d_value,
                                  float* d_alpha_dot, float* d_edge_logits, float* d_bias_table, void* scratch, size_t scratch_bytes, void* stream) {
     Plan p;
-    const int rc = make_plan(x, p, {grad_out, d_alpha, d_value});
+    const int rc = make_plan(x, true, p, {grad_out, d_alpha, d_value});
     if (rc != DEDF_OK) return rc;
     if (p.a.n_dst > 0 && (!norm || !out_f || !grad_out)) return DEDF_ERR_INVALID;
     if (scratch_bytes < backward_bytes(p) || (backward_bytes(p) > 0 && !scratch) || (reinterpret_cast<uintptr_t>(scratch) & 15)) return DEDF_ERR_INVALID;
@@ -166,7 +166,7 @@ int dedf_edge_attention_backward(const dedf_edge_attn* x, const double* norm, co
     BackArgs b{norm, (const float*)scratch, grad_out, d_alpha, d_value, d_edge_logits,
                d_alpha_dot || d_bias_table ? (float*)((char*)scratch + up16((size_t)p.a.n_dst * p.a.heads * 4)) : nullptr};
     Backward f{p, b, out_f, (float*)scratch, d_alpha_dot, d_bias_table, st};
-    return by_shape(x->type, p.sub, p.wide, f);
+    return by_shape(x->type, p.sub, p.nv, f);
 }
 
 }  // extern "C"
