@@ -18,6 +18,10 @@ namespace rows {
 
 constexpr int kWaves = 4, kMostBlocks = 4;          // waves of a workgroup; degrees of a feature row
 
+// Waves a SIMD holds, by registers; a launch of the norms has as many workgroups as are resident at once, which share out the rows evenly
+constexpr int forward_waves(int nq) { return nq == 1 ? 6 : 4; }
+constexpr int backward_waves(int nq) { return nq == 1 ? 4 : 2; }
+
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b4 __attribute__((ext_vector_type(4)));
@@ -31,7 +35,8 @@ struct Shape {
     int start[kMostBlocks + 1];                      // first component of a block
     int first[kMostBlocks];                          // first channel
     int d[kMostBlocks];                              // components of a channel
-    float inverse[kMostBlocks];                      // 1 / components of a block
+    int divide[kMostBlocks];                         // (x divide) >> 16 = x / d for components x of a block
+    float inverse[kMostBlocks];                      // 1 / components of a block; 0 and an empty range for a block that is not there
 };
 struct Args {
     Shape s;
@@ -42,7 +47,6 @@ struct Args {
     float scale, eps;
     uint32_t threshold; float keep_scale;
     const int64_t* rng;
-    int vec;
     // forward
     void* h; void* z; int64_t* rng_used;
     // backward
@@ -51,32 +55,36 @@ struct Args {
     float* param_rows;                               // (workgroups, 4 channels): post weight, post bias, next weight, next bias
 };
 
-// sum over the wave, in every lane
-template <int CTRL, int ROWS> __device__ inline float dpp_add(float x) {
-    return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false));
+// sums over the wave, in every lane.  Step by step for all of them: each step waits for the one before, and N chains fill each other's waits.
+template <int CTRL, int ROWS, int N> __device__ inline void dpp_add(float (&x)[N]) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) x[k] += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x[k]), CTRL, ROWS, 0xf, false));
 }
-__device__ inline float wave_sum(float x) {
-    x = dpp_add<0xB1, 0xf>(x);           // neighbours, pairs, halves of a row of 16, rows
-    x = dpp_add<0x4E, 0xf>(x);
-    x = dpp_add<0x141, 0xf>(x);
-    x = dpp_add<0x140, 0xf>(x);
-    x = dpp_add<0x142, 0xa>(x);          // row 0 into 1, 2 into 3; then row 1 into 2 and 3: the last lane holds the sum
-    x = dpp_add<0x143, 0xc>(x);
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+template <int N> __device__ inline void wave_sums(float (&x)[N]) {
+    dpp_add<0xB1, 0xf>(x);           // neighbours, pairs, halves of a row of 16, rows
+    dpp_add<0x4E, 0xf>(x);
+    dpp_add<0x141, 0xf>(x);
+    dpp_add<0x140, 0xf>(x);
+    dpp_add<0x142, 0xa>(x);          // row 0 into 1, 2 into 3; then row 1 into 2 and 3: the last lane holds the sum
+    dpp_add<0x143, 0xc>(x);
+#pragma unroll
+    for (int k = 0; k < N; ++k) x[k] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x[k]), 63));
 }
 __device__ inline void wave_sync() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
 
-// a lane's components of a row and where they belong.  EVEN: blocks start on whole quads, so a quad has one degree.  WPR: waves that share a row (1; 4,
-// the whole workgroup, for rows over 512 components: one wave would have to spill its registers).
-template <class T, int NQ, bool EVEN, int WPR> struct Row {
+// a lane's components of a row and where they belong.  FAST: blocks start on whole, aligned quads, so a quad has one degree and is one access.  WPR:
+// waves that share a row (1; 4, the whole workgroup, for rows over 512 components: one wave would have to spill its registers).  Lanes behind the row's end
+// repeat its last quad; they belong to no block and are not stored.
+template <class T, int NQ, bool FAST, int WPR> struct Row {
     typedef typename Quad<T>::type Raw;
-    const Shape& s; int lane, vec;        // lane: of the row's WPR x 64
+    const Shape& s; int lane;             // of the row's WPR x 64
     float* own; float* exchange; int turn;
-    int block[NQ][EVEN ? 1 : 4];          // -1: no component
+    int64_t held;                         // row whose dropout words LDS holds (and the next one's, where two rows fit)
+    int block[NQ][FAST ? 1 : 4];          // -1: no component
     int channel[NQ][4];
-    __device__ Row(const Shape& shape, int vec_, char* lds) : s(shape), lane(threadIdx.x & (64 * WPR - 1)), vec(vec_), turn(0) {
-        own = (float*)(lds + threadIdx.x / (64 * WPR) * team_bytes(shape));
-        exchange = own + ((shape.width + 3) & ~3);
+    __device__ Row(const Shape& shape, char* lds, int team) : s(shape), lane(threadIdx.x & (64 * WPR - 1)), turn(0), held(-2) {
+        own = (float*)(lds + team * team_bytes(shape));
+        exchange = own + own_floats(shape);
 #pragma unroll
         for (int j = 0; j < NQ; ++j)
 #pragma unroll
@@ -84,23 +92,24 @@ template <class T, int NQ, bool EVEN, int WPR> struct Row {
                 const int c = 4 * (j * 64 * WPR + lane) + i;
                 int b = -1, ch = 0;
 #pragma unroll
-                for (int k = 0; k < kMostBlocks; ++k)
-                    if (k < s.n_blocks && c >= s.start[k] && c < s.start[k + 1]) { b = k; ch = s.first[k] + (c - s.start[k]) / s.d[k]; }
+                for (int k = 0; k < kMostBlocks; ++k) {
+                    const bool in = (c >= s.start[k]) & (c < s.start[k + 1]);
+                    b = in ? k : b;
+                    ch = in ? s.first[k] + (((c - s.start[k]) * s.divide[k]) >> 16) : ch;
+                }
                 channel[j][i] = ch;
-                if (!EVEN || i == 0) block[j][EVEN ? 0 : i] = b;
+                if (!FAST || i == 0) block[j][FAST ? 0 : i] = b;
             }
     }
-    __device__ int of(int j, int i) const { return block[j][EVEN ? 0 : i]; }
+    __device__ int of(int j, int i) const { return block[j][FAST ? 0 : i]; }
     __device__ void load(f4 (&f)[NQ], const void* p, int64_t row) const {
         const T* at = (const T*)p + row * s.width;
-        Raw raw[NQ];
-        if (vec) {
+        if constexpr (FAST) {
+            Raw raw[NQ];
 #pragma unroll
             for (int j = 0; j < NQ; ++j) raw[j] = *(const Raw*)(at + min(4 * (j * 64 * WPR + lane), s.width - 4));
 #pragma unroll
-            for (int j = 0; j < NQ; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) f[j][i] = of(j, i) >= 0 ? (float)raw[j][i] : 0.0f;
+            for (int j = 0; j < NQ; ++j) f[j] = f4{(float)raw[j][0], (float)raw[j][1], (float)raw[j][2], (float)raw[j][3]};
         } else {
 #pragma unroll
             for (int j = 0; j < NQ; ++j)
@@ -113,25 +122,27 @@ template <class T, int NQ, bool EVEN, int WPR> struct Row {
 #pragma unroll
         for (int j = 0; j < NQ; ++j) {
             const int c = 4 * (j * 64 * WPR + lane);
-            if (vec) { if (c < s.width) *(Raw*)(at + c) = Raw{(T)f[j][0], (T)f[j][1], (T)f[j][2], (T)f[j][3]}; }
+            if constexpr (FAST) { if (c < s.width) *(Raw*)(at + c) = Raw{(T)f[j][0], (T)f[j][1], (T)f[j][2], (T)f[j][3]}; }
             else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) if (c + i < s.width) at[c + i] = (T)f[j][i];
             }
         }
     }
-    // a channel's value on each of its components
+    // a channel's value on each of its components; channels from n on have 0
     __device__ void spread(f4 (&f)[NQ], const float* values, int n) const {
 #pragma unroll
-        for (int j = 0; j < NQ; ++j)
+        for (int j = 0; j < NQ; ++j) {
+            f[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (n > 0)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) f[j][i] = of(j, i) >= 0 && channel[j][i] < n ? values[channel[j][i]] : 0.0f;
+                for (int i = 0; i < 4; ++i) { const float x = values[min(channel[j][i], n - 1)]; f[j][i] = channel[j][i] < n ? x : 0.0f; }
+        }
     }
     __device__ void sync() const { if constexpr (WPR == 1) wave_sync(); else __syncthreads(); }
     // sums over the row's lanes, in every lane
     template <int N> __device__ void row_sums(float (&v)[N]) {
-#pragma unroll
-        for (int k = 0; k < N; ++k) v[k] = wave_sum(v[k]);
+        wave_sums(v);
         if constexpr (WPR > 1) {          // (two buffers in turn: a wave that is one exchange ahead does not touch what another still reads)
             float* at = exchange + turn * WPR * 8;
             turn ^= 1;
@@ -149,7 +160,7 @@ template <class T, int NQ, bool EVEN, int WPR> struct Row {
         for (int k = 0; k < kMostBlocks; ++k) part[k] = 0.0f;
 #pragma unroll
         for (int j = 0; j < NQ; ++j) {
-            if constexpr (EVEN) {
+            if constexpr (FAST) {
                 const f4 m = f[j] * g[j];
                 const float q = (m[0] + m[1]) + (m[2] + m[3]);
 #pragma unroll
@@ -188,7 +199,7 @@ template <class T, int NQ, bool EVEN, int WPR> struct Row {
         block_parts(r, f, f);
         row_sums(r);
 #pragma unroll
-        for (int k = 0; k < kMostBlocks; ++k) if (k < s.n_blocks) r[k] = rsqrtf(r[k] * s.inverse[k] + eps);
+        for (int k = 0; k < kMostBlocks; ++k) r[k] = rsqrtf(r[k] * s.inverse[k] + eps);
 #pragma unroll
         for (int j = 0; j < NQ; ++j)
 #pragma unroll
@@ -210,21 +221,28 @@ template <class T, int NQ, bool EVEN, int WPR> struct Row {
 #pragma unroll
             for (int i = 0; i < 4; ++i) g[j][i] = pick(r, j, i) * (g[j][i] - (s.scalars && of(j, i) == 0 ? mean : 0.0f) - n[j][i] * pick(dot, j, i));
     }
-    // dropout factors of a row, one word for each channel, through LDS
-    __device__ void keep(f4 (&f)[NQ], int64_t row, uint64_t offset, uint64_t seed, uint32_t threshold, float scale) const {
-        sync();
-        for (int g = lane; g < (s.channels + 3) >> 2; g += 64 * WPR) {
-            const Words x = dropout_words((uint32_t)row, (1u << 16) + g, offset, seed);
-            *(f4*)(own + 4 * g) = f4{x.w[0] >= threshold ? scale : 0.0f, x.w[1] >= threshold ? scale : 0.0f, x.w[2] >= threshold ? scale : 0.0f, x.w[3] >= threshold ? scale : 0.0f};
+    // dropout factors of a row, one word for each channel, through LDS: of this row and the next at once where both fit into the row's lanes
+    __device__ void keep(f4 (&f)[NQ], int64_t row, uint64_t offset, uint64_t seed, uint32_t threshold, float scale) {
+        const int groups = (s.channels + 3) >> 2, rows = two_rows(s) ? 2 : 1;
+        if (row != held && (rows == 1 || row != held + 1)) {
+            sync();
+            for (int idx = lane; idx < rows * groups; idx += 64 * WPR) {
+                const int next = idx >= groups, g = idx - (next ? groups : 0);
+                const Words x = dropout_words((uint32_t)(row + next), (1u << 16) + g, offset, seed);
+                *(f4*)(own + 4 * idx) = f4{x.w[0] >= threshold ? scale : 0.0f, x.w[1] >= threshold ? scale : 0.0f, x.w[2] >= threshold ? scale : 0.0f, x.w[3] >= threshold ? scale : 0.0f};
+            }
+            held = row;
+            sync();
         }
-        sync();
+        const float* at = own + (row == held ? 0 : 4 * groups);
 #pragma unroll
         for (int j = 0; j < NQ; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) f[j][i] = own[channel[j][i]];
+            for (int i = 0; i < 4; ++i) f[j][i] = at[channel[j][i]];
     }
     // components to LDS, from which folded() adds up a channel's
-    __device__ void fold(const f4 (&f)[NQ]) const {
+    __device__ void fold(const f4 (&f)[NQ]) {
+        held = -2;
         sync();
 #pragma unroll
         for (int j = 0; j < NQ; ++j) if (4 * (j * 64 * WPR + lane) < s.width) *(f4*)(own + 4 * (j * 64 * WPR + lane)) = f[j];
@@ -238,17 +256,22 @@ template <class T, int NQ, bool EVEN, int WPR> struct Row {
         for (int i = 0; i < s.d[b]; ++i) sum += lds[at + i];
         return sum;
     }
-    static __host__ __device__ size_t team_bytes(const Shape& s) { return ((size_t)(s.width + 3) >> 2) * 16 + (WPR > 1 ? 2 * WPR * 8 * 4 : 0); }
+    static __host__ __device__ bool two_rows(const Shape& s) { return s.channels <= 128; }
+    static __host__ __device__ int own_floats(const Shape& s) {
+        const int c = (s.channels + 3) & ~3, w = (s.width + 3) & ~3, k = two_rows(s) ? 2 * c : c;
+        return w > k ? w : k;
+    }
+    static __host__ __device__ size_t team_bytes(const Shape& s) { return (size_t)own_floats(s) * 4 + (WPR > 1 ? 2 * WPR * 8 * 4 : 0); }
 };
 
 template <class T> __device__ inline float gate_at(const void* gate, int f32, int64_t i) { return f32 ? ((const float*)gate)[i] : (float)((const T*)gate)[i]; }
 
-template <class T, int NQ, bool EVEN, int WPR> __global__ __launch_bounds__(256) void k_norm_forward(Args P) {
+template <class T, int NQ, bool FAST, int WPR> __global__ __launch_bounds__(256, forward_waves(NQ)) void k_norm_forward(Args P) {
     extern __shared__ __align__(16) char lds[];
-    Row<T, NQ, EVEN, WPR> R(P.s, P.vec, lds);
     if (P.rng_used && P.threshold && blockIdx.x == 0 && threadIdx.x < 2) P.rng_used[threadIdx.x] = P.rng[threadIdx.x];
     constexpr int TEAMS = kWaves / WPR;
-    const int team = threadIdx.x / (64 * WPR);
+    const int team = __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * WPR));          // (known to be uniform: row addresses stay scalar)
+    Row<T, NQ, FAST, WPR> R(P.s, lds, team);
     uint64_t seed = 0, offset = 0;
     if (P.threshold) { seed = (uint64_t)P.rng[0]; offset = (uint64_t)P.rng[1]; }
     f4 pw[NQ], pb[NQ], nw[NQ], nb[NQ], gate[NQ];
@@ -296,12 +319,12 @@ template <class T, int NQ, bool EVEN, int WPR> __global__ __launch_bounds__(256)
     }
 }
 
-template <class T, int NQ, bool EVEN, int WPR> __global__ __launch_bounds__(256) void k_norm_backward(Args P) {
+template <class T, int NQ, bool FAST, int WPR> __global__ __launch_bounds__(256, backward_waves(NQ)) void k_norm_backward(Args P) {
     extern __shared__ __align__(16) char lds[];
-    typedef Row<T, NQ, EVEN, WPR> Rw;
-    Rw R(P.s, P.vec, lds);
+    typedef Row<T, NQ, FAST, WPR> Rw;
     constexpr int TEAMS = kWaves / WPR;
-    const int team = threadIdx.x / (64 * WPR), C = P.s.channels;
+    const int team = __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * WPR)), C = P.s.channels;
+    Rw R(P.s, lds, team);
     uint64_t seed = 0, offset = 0;
     if (P.threshold) { seed = (uint64_t)P.rng[0]; offset = (uint64_t)P.rng[1]; }
     const bool post = P.post_w != nullptr, next = P.dz != nullptr;
@@ -405,15 +428,16 @@ template <class T, int NQ, bool EVEN, int WPR> __global__ __launch_bounds__(256)
 }
 
 // x keep: forward and backward are the same map
-template <class T, int NQ, bool EVEN, int WPR> __global__ __launch_bounds__(256) void k_dropout(Args P) {
+template <class T, int NQ, bool FAST, int WPR> __global__ __launch_bounds__(256) void k_dropout(Args P) {
     extern __shared__ __align__(16) char lds[];
-    Row<T, NQ, EVEN, WPR> R(P.s, P.vec, lds);
     if (P.rng_used && P.threshold && blockIdx.x == 0 && threadIdx.x < 2) P.rng_used[threadIdx.x] = P.rng[threadIdx.x];
     constexpr int TEAMS = kWaves / WPR;
-    const int team = threadIdx.x / (64 * WPR);
+    const int team = __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * WPR));          // (known to be uniform: row addresses stay scalar)
+    Row<T, NQ, FAST, WPR> R(P.s, lds, team);
     uint64_t seed = 0, offset = 0;
     if (P.threshold) { seed = (uint64_t)P.rng[0]; offset = (uint64_t)P.rng[1]; }
-    for (int64_t row = blockIdx.x * TEAMS + team; row < P.n_rows; row += gridDim.x * TEAMS) {
+    const int64_t first = ((int64_t)blockIdx.x * TEAMS + team) * P.slice_rows, last = min(first + P.slice_rows, (int64_t)P.n_rows);
+    for (int64_t row = first; row < last; ++row) {
         f4 x[NQ], m[NQ];
         R.load(x, P.x, row);
         if (P.threshold) {

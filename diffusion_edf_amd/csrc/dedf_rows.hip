@@ -9,35 +9,40 @@ using namespace dedf::rows;
 namespace {
 
 constexpr int kMostWidth = 2048;
-constexpr int kForwardBlocks = 2048, kBackwardBlocks = 768;
+constexpr int kCus = 256, kDropoutBlocks = 2048;
+int quads(int width) { return width <= 256 || (width > 512 && width <= 1024) ? 1 : 2; }          // of a lane, as by_width
+int norm_blocks(bool backward, int width) { return kCus * (backward ? backward_waves(quads(width)) : forward_waves(quads(width))); }          // (a workgroup has a wave on each SIMD)
 
 size_t element(int type) { return type == DEDF_F32 ? 4 : 2; }
 bool shared_rows(int width) { return width > 512; }          // a row has the whole workgroup
 
-template <class T, bool EVEN, class F> int by_width(int width, F& f) {
-    return width <= 256 ? f.template run<T, 1, EVEN, 1>() : width <= 512 ? f.template run<T, 2, EVEN, 1>()
-         : width <= 1024 ? f.template run<T, 1, EVEN, 4>() : f.template run<T, 2, EVEN, 4>();
+template <class T, bool FAST, class F> int by_width(int width, F& f) {
+    return width <= 256 ? f.template run<T, 1, FAST, 1>() : width <= 512 ? f.template run<T, 2, FAST, 1>()
+         : width <= 1024 ? f.template run<T, 1, FAST, 4>() : f.template run<T, 2, FAST, 4>();
 }
 
-int make_shape(int n_blocks, const int* mul, const int* degree, Shape& s, bool& even) {
+// `whole`: blocks start on whole quads
+int make_shape(int n_blocks, const int* mul, const int* degree, Shape& s, bool& whole) {
     if (n_blocks < 1 || !mul || !degree) return DEDF_ERR_INVALID;
     if (n_blocks > kMostBlocks) return DEDF_ERR_UNSUPPORTED;
     s = Shape{};
     s.n_blocks = n_blocks;
-    even = true;
+    whole = true;
     int64_t width = 0, channels = 0;
-    for (int b = 0; b < n_blocks; ++b) {
-        if (mul[b] < 1 || degree[b] < 0 || (b > 0 && degree[b] <= degree[b - 1])) return DEDF_ERR_INVALID;
-        if (mul[b] > kMostWidth || degree[b] > 7) return DEDF_ERR_UNSUPPORTED;
-        s.start[b] = (int)width; s.first[b] = (int)channels; s.d[b] = 2 * degree[b] + 1;
-        s.inverse[b] = 1.0f / (float)(mul[b] * s.d[b]);
-        even = even && width % 4 == 0;
-        width += (int64_t)mul[b] * s.d[b]; channels += mul[b];
+    for (int b = 0; b < kMostBlocks; ++b) {
+        const bool there = b < n_blocks;
+        if (there && (mul[b] < 1 || degree[b] < 0 || (b > 0 && degree[b] <= degree[b - 1]))) return DEDF_ERR_INVALID;
+        if (there && (mul[b] > kMostWidth || degree[b] > 7)) return DEDF_ERR_UNSUPPORTED;
+        const int m = there ? mul[b] : 0, d = there ? 2 * degree[b] + 1 : 1;
+        s.start[b] = (int)width; s.first[b] = (int)channels; s.d[b] = d;
+        s.divide[b] = (65536 + d - 1) / d;          // (exact for x d < 65536: x < 2048, d <= 15)
+        s.inverse[b] = there ? 1.0f / (float)(m * d) : 0.0f;
+        width += (int64_t)m * d; channels += m;
         s.start[b + 1] = (int)width;
+        whole = whole && width % 4 == 0;
     }
     if (width > kMostWidth) return DEDF_ERR_UNSUPPORTED;
     s.width = (int)width; s.channels = (int)channels; s.scalars = degree[0] == 0 ? mul[0] : 0;
-    even = even && width % 4 == 0;
     return DEDF_OK;
 }
 
@@ -53,11 +58,11 @@ int grid(const Args& a, int most) {
     return (int)std::min<int64_t>(most, ((int64_t)a.groups * a.slices + teams - 1) / teams);
 }
 
-int make_args(const dedf_norm* x, Args& a, bool& even, int waves) {
+int make_args(const dedf_norm* x, bool backward, Args& a, bool& fast) {
     if (!x || x->n_rows < 0) return DEDF_ERR_INVALID;
     if (x->type != DEDF_F32 && x->type != DEDF_F16 && x->type != DEDF_BF16) return DEDF_ERR_UNSUPPORTED;
     a = Args{};
-    const int rc = make_shape(x->n_blocks, x->mul, x->degree, a.s, even);
+    const int rc = make_shape(x->n_blocks, x->mul, x->degree, a.s, fast);
     if (rc != DEDF_OK) return rc;
     const int groups = x->gate ? x->groups : 1;
     if (x->n_rows > 0 && (!x->x || groups < 1 || groups > x->n_rows || x->n_rows % groups != 0)) return DEDF_ERR_INVALID;
@@ -69,11 +74,10 @@ int make_args(const dedf_norm* x, Args& a, bool& even, int waves) {
     a.post_w = x->post_weight; a.post_b = x->post_bias; a.next_w = x->next_weight; a.next_b = x->next_bias;
     a.scale = x->scale; a.eps = x->eps;
     a.threshold = (uint32_t)std::floor(x->dropout * 4294967296.0); a.keep_scale = (float)(1.0 / (1.0 - x->dropout)); a.rng = x->rng;
-    if (a.n_rows > 0) cut(a, waves);
+    if (a.n_rows > 0) cut(a, norm_blocks(backward, a.s.width) * (shared_rows(a.s.width) ? 1 : kWaves));
     return DEDF_OK;
 }
-bool on_quads(int type, std::initializer_list<const void*> all, int width) {
-    if (width % 4 != 0) return false;
+bool on_quads(int type, std::initializer_list<const void*> all) {
     for (const void* p : all) if (reinterpret_cast<uintptr_t>(p) % (4 * element(type)) != 0) return false;
     return true;
 }
@@ -88,16 +92,16 @@ namespace rows {
 
 struct NormForward {
     const Args& a; hipStream_t st;
-    template <class T, int NQ, bool EVEN, int WPR> int run() {
-        hipLaunchKernelGGL((k_norm_forward<T, NQ, EVEN, WPR>), dim3(grid(a, kForwardBlocks)), dim3(256), lds_bytes(a), st, a);
+    template <class T, int NQ, bool FAST, int WPR> int run() {
+        hipLaunchKernelGGL((k_norm_forward<T, NQ, FAST, WPR>), dim3(grid(a, norm_blocks(false, a.s.width))), dim3(256), lds_bytes(a), st, a);
         return hipGetLastError() == hipSuccess ? DEDF_OK : DEDF_ERR_RUNTIME;
     }
 };
 struct NormBackward {
     const Args& a; hipStream_t st; float* post_w; float* post_b; float* next_w; float* next_b;
-    template <class T, int NQ, bool EVEN, int WPR> int run() {
-        const int blocks = grid(a, kBackwardBlocks), C = a.s.channels;
-        hipLaunchKernelGGL((k_norm_backward<T, NQ, EVEN, WPR>), dim3(blocks), dim3(256), lds_bytes(a), st, a);
+    template <class T, int NQ, bool FAST, int WPR> int run() {
+        const int blocks = grid(a, norm_blocks(true, a.s.width)), C = a.s.channels;
+        hipLaunchKernelGGL((k_norm_backward<T, NQ, FAST, WPR>), dim3(blocks), dim3(256), lds_bytes(a), st, a);
         if (a.param_rows)
             hipLaunchKernelGGL(k_row_sums<T>, dim3((4 * C + 15) / 16), dim3(256), 0, st, (const float*)a.param_rows, blocks, 4 * C, C, post_w, post_b, next_w, next_b, a.s.scalars, a.s.scalars, (T*)nullptr);
         if (a.gate_rows)
@@ -108,13 +112,16 @@ struct NormBackward {
 };
 struct Dropout {
     const Args& a; hipStream_t st;
-    template <class T, int NQ, bool EVEN, int WPR> int run() {
-        const int teams = kWaves / WPR;
-        hipLaunchKernelGGL((k_dropout<T, NQ, EVEN, WPR>), dim3(std::min(kForwardBlocks, (a.n_rows + teams - 1) / teams)), dim3(256), lds_bytes(a), st, a);
+    template <class T, int NQ, bool FAST, int WPR> int run() {
+        constexpr int teams = kWaves / WPR;
+        Args b = a;
+        b.slice_rows = (a.n_rows + kDropoutBlocks * teams - 1) / (kDropoutBlocks * teams);
+        const int slices = (a.n_rows + b.slice_rows - 1) / b.slice_rows;
+        hipLaunchKernelGGL((k_dropout<T, NQ, FAST, WPR>), dim3((slices + teams - 1) / teams), dim3(256), lds_bytes(a), st, b);
         return hipGetLastError() == hipSuccess ? DEDF_OK : DEDF_ERR_RUNTIME;
     }
 };
-template <class T, class F> int launch(int width, bool even, F f) { return even ? by_width<T, true>(width, f) : by_width<T, false>(width, f); }
+template <class T, class F> int launch(int width, bool fast, F f) { return fast ? by_width<T, true>(width, f) : by_width<T, false>(width, f); }
 
 #define DEDF_LAUNCHES(T, PREFIX) \
     PREFIX template int launch<T, NormForward>(int, bool, NormForward); PREFIX template int launch<T, NormBackward>(int, bool, NormBackward); PREFIX template int launch<T, Dropout>(int, bool, Dropout);
@@ -134,10 +141,10 @@ DEDF_LAUNCHES(__bf16, )
 #ifndef DEDF_ELEMENT
 namespace {
 
-template <class F> int by_shape(int type, int width, bool even, F f) {
-    return type == DEDF_F32 ? launch<float>(width, even, f) : type == DEDF_F16 ? launch<_Float16>(width, even, f) : launch<__bf16>(width, even, f);
+template <class F> int by_shape(int type, int width, bool fast, F f) {
+    return type == DEDF_F32 ? launch<float>(width, fast, f) : type == DEDF_F16 ? launch<_Float16>(width, fast, f) : launch<__bf16>(width, fast, f);
 }
-size_t param_bytes(const Args& a) { return (size_t)grid(a, kBackwardBlocks) * 4 * a.s.channels * 4; }
+size_t param_bytes(const Args& a) { return (size_t)grid(a, norm_blocks(true, a.s.width)) * 4 * a.s.channels * 4; }
 size_t gate_bytes(const Args& a) { return a.gate && a.slices > 1 ? (size_t)a.groups * a.slices * a.s.channels * 4 : 0; }
 size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
@@ -146,28 +153,28 @@ size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 extern "C" {
 
 int dedf_norm_gate_residual(const dedf_norm* x, void* h, void* z, int64_t* rng_used, void* stream) {
-    Args a; bool even;
-    const int rc = make_args(x, a, even, kForwardBlocks * kWaves);
+    Args a; bool fast;
+    const int rc = make_args(x, false, a, fast);
     if (rc != DEDF_OK) return rc;
     if (a.n_rows == 0) return DEDF_OK;          // (tensors without elements may have no address)
     if ((x->y != nullptr) != (h != nullptr) || (x->next_weight != nullptr) != (z != nullptr) || (!h && !z)) return DEDF_ERR_INVALID;
     a.h = h; a.z = z; a.rng_used = rng_used;
-    a.vec = on_quads(x->type, {a.x, a.y, h, z}, a.s.width);
+    fast = fast && on_quads(x->type, {a.x, a.y, h, z});
     NormForward f{a, static_cast<hipStream_t>(stream)};
-    return by_shape(x->type, a.s.width, even, f);
+    return by_shape(x->type, a.s.width, fast, f);
 }
 
 size_t dedf_norm_scratch_bytes(const dedf_norm* x) {
-    Args a; bool even;
-    if (make_args(x, a, even, kBackwardBlocks * kWaves) != DEDF_OK || a.n_rows == 0) return 0;
+    Args a; bool fast;
+    if (make_args(x, true, a, fast) != DEDF_OK || a.n_rows == 0) return 0;
     return up16(param_bytes(a)) + gate_bytes(a);
 }
 
 int dedf_norm_gate_residual_backward(const dedf_norm* x, const void* grad_h, const void* grad_z, void* d_x, void* d_y, void* d_gate,
                                      float* d_post_weight, float* d_post_bias, float* d_next_weight, float* d_next_bias,
                                      void* scratch, size_t scratch_bytes, void* stream) {
-    Args a; bool even;
-    const int rc = make_args(x, a, even, kBackwardBlocks * kWaves);
+    Args a; bool fast;
+    const int rc = make_args(x, true, a, fast);
     if (rc != DEDF_OK) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const bool params = d_post_weight || d_post_bias || d_next_weight || d_next_bias;
@@ -183,24 +190,24 @@ int dedf_norm_gate_residual_backward(const dedf_norm* x, const void* grad_h, con
     a.dh = grad_h; a.dz = grad_z; a.dx = d_x; a.dy = d_y; a.d_gate = d_gate;
     a.gate_rows = d_gate && a.slices > 1 ? (float*)((char*)scratch + up16(param_bytes(a))) : nullptr;
     a.param_rows = params ? (float*)scratch : nullptr;
-    a.vec = on_quads(x->type, {a.x, a.y, grad_h, grad_z, d_x, d_y}, a.s.width);
+    fast = fast && on_quads(x->type, {a.x, a.y, grad_h, grad_z, d_x, d_y});
     NormBackward f{a, st, d_post_weight, d_post_bias, d_next_weight, d_next_bias};
-    return by_shape(x->type, a.s.width, even, f);
+    return by_shape(x->type, a.s.width, fast, f);
 }
 
 int dedf_channel_dropout(int type, int n_rows, int n_blocks, const int* mul, const int* degree, const void* x, double dropout, const int64_t* rng,
                          void* out, int64_t* rng_used, void* stream) {
-    Args a{}; bool even;
+    Args a{}; bool fast;
     if (type != DEDF_F32 && type != DEDF_F16 && type != DEDF_BF16) return DEDF_ERR_UNSUPPORTED;
-    const int rc = make_shape(n_blocks, mul, degree, a.s, even);
+    const int rc = make_shape(n_blocks, mul, degree, a.s, fast);
     if (rc != DEDF_OK) return rc;
     if (n_rows < 0 || (n_rows > 0 && (!x || !out)) || !(dropout >= 0.0 && dropout < 1.0) || (dropout > 0.0 && !rng)) return DEDF_ERR_INVALID;
     if (n_rows == 0) return DEDF_OK;
     a.n_rows = n_rows; a.x = x; a.h = out; a.rng_used = rng_used;
     a.threshold = (uint32_t)std::floor(dropout * 4294967296.0); a.keep_scale = (float)(1.0 / (1.0 - dropout)); a.rng = rng;
-    a.vec = on_quads(type, {x, out}, a.s.width);
+    fast = fast && on_quads(type, {x, out});
     Dropout f{a, static_cast<hipStream_t>(stream)};
-    return by_shape(type, a.s.width, even, f);
+    return by_shape(type, a.s.width, fast, f);
 }
 
 }  // extern "C"
