@@ -597,18 +597,29 @@ void k_attn_backward(Args P, BackArgs B) {
     }
 }
 
-// column sums of (rows, columns) in 64 bits, in order: 16 columns a workgroup
-static __global__ __launch_bounds__(256) void k_column_sums(const float* x, int rows, int columns, float* first, int n_first, float* second) {
-    __shared__ double share[16][16];
+// column sums of (rows, columns) in 64 bits, in a fixed order: 16 columns a workgroup; the first n_first go to `first`, the rest to `second`
+static __global__ __launch_bounds__(1024) void k_column_sums(const float* x, int rows, int columns, float* first, int n_first, float* second) {
+    __shared__ double share[64][17];
     const int c = blockIdx.x * 16 + (threadIdx.x & 15), r0 = threadIdx.x >> 4;
+    const float* m = x + c;
     double s = 0.0;
-    if (c < columns) for (int r = r0; r < rows; r += 16) s += (double)x[(size_t)r * columns + c];
+    if (c < columns) {
+        int r = r0;
+        for (; r + 3 * 64 < rows; r += 4 * 64) {
+            const float a = m[(size_t)r * columns], b = m[(size_t)(r + 64) * columns], d = m[(size_t)(r + 128) * columns], e = m[(size_t)(r + 192) * columns];
+            s += ((double)a + (double)b) + ((double)d + (double)e);
+        }
+        for (; r < rows; r += 64) s += (double)m[(size_t)r * columns];
+    }
     share[r0][threadIdx.x & 15] = s;
-    __syncthreads();
+    for (int half = 32; half >= 1; half >>= 1) {
+        __syncthreads();
+        if (r0 < half) share[r0][threadIdx.x & 15] += share[r0 + half][threadIdx.x & 15];
+    }
     if (r0 != 0 || c >= columns) return;
-    for (int r = 1; r < 16; ++r) s += share[r][threadIdx.x];
-    if (c < n_first) { if (first) first[c] = (float)s; }
-    else if (second) second[c - n_first] = (float)s;
+    const float v = (float)share[0][threadIdx.x & 15];
+    if (c < n_first) { if (first) first[c] = v; }
+    else if (second) second[c - n_first] = v;
 }
 
 // ---- the sorted edge list -------------------------------------------------------------------------------------------------------------------

@@ -31,7 +31,7 @@ struct Backward {
         hipLaunchKernelGGL((k_attn_backward<T, SUB, VEC, NV>), dim3(p.blocks), dim3(256), p.lds_backward, st, a, b);
         if (b.param_rows) {
             const int n_w = a.heads * a.k, columns = n_w + a.heads * a.n_buckets;
-            hipLaunchKernelGGL(k_column_sums, dim3((columns + 15) / 16), dim3(256), 0, st, (const float*)b.param_rows, p.blocks, columns, d_alpha_dot, n_w, d_table);
+            hipLaunchKernelGGL(k_column_sums, dim3((columns + 15) / 16), dim3(1024), 0, st, (const float*)b.param_rows, p.blocks, columns, d_alpha_dot, n_w, d_table);
         }
         return hipGetLastError() == hipSuccess ? DEDF_OK : DEDF_ERR_RUNTIME;
     }
@@ -160,7 +160,7 @@ int dedf_edge_attention_backward(const dedf_edge_attn* x, const double* norm, co
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int n_w = p.a.heads * p.a.k, columns = n_w + p.a.heads * p.a.n_buckets;
     if (p.a.n_edges == 0) {          // no edge: the parameters' gradients are zero (a sum over no rows)
-        hipLaunchKernelGGL(k_column_sums, dim3((columns + 15) / 16), dim3(256), 0, st, (const float*)nullptr, 0, columns, d_alpha_dot, n_w, d_bias_table);
+        hipLaunchKernelGGL(k_column_sums, dim3((columns + 15) / 16), dim3(1024), 0, st, (const float*)nullptr, 0, columns, d_alpha_dot, n_w, d_bias_table);
         return hipGetLastError() == hipSuccess ? DEDF_OK : DEDF_ERR_RUNTIME;
     }
     BackArgs b{norm, (const float*)scratch, grad_out, d_alpha, d_value, d_edge_logits,

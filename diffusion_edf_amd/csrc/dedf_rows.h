@@ -52,23 +52,37 @@ struct Args {
     // backward
     const void* dh; const void* dz; void* dx; void* dy;
     void* d_gate; float* gate_rows;                  // a group with one slice writes its gradient, else (unit, channels) sums
-    float* param_rows;                               // (workgroups, 4 channels): post weight, post bias, next weight, next bias
+    float* param_rows; int n_params;                 // (workgroups, n_params channels): post weight, post bias, next weight, next bias; the gate of one group
 };
 
-// sums over the wave, in every lane.  Step by step for all of them: each step waits for the one before, and N chains fill each other's waits.
-template <int CTRL, int ROWS, int N> __device__ inline void dpp_add(float (&x)[N]) {
-#pragma unroll
-    for (int k = 0; k < N; ++k) x[k] += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x[k]), CTRL, ROWS, 0xf, false));
+template <int CTRL> __device__ inline float dpp(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
 }
-template <int N> __device__ inline void wave_sums(float (&x)[N]) {
-    dpp_add<0xB1, 0xf>(x);           // neighbours, pairs, halves of a row of 16, rows
-    dpp_add<0x4E, 0xf>(x);
-    dpp_add<0x141, 0xf>(x);
-    dpp_add<0x140, 0xf>(x);
-    dpp_add<0x142, 0xa>(x);          // row 0 into 1, 2 into 3; then row 1 into 2 and 3: the last lane holds the sum
-    dpp_add<0x143, 0xc>(x);
-#pragma unroll
-    for (int k = 0; k < N; ++k) x[k] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x[k]), 63));
+// x of the rows of 16 lanes added in pairs, then of the halves of the wave: every lane gets the sum over the lanes with its place in a row
+__device__ inline float add_rows(float x) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+    x = __builtin_bit_cast(float, (unsigned)a[0]) + __builtin_bit_cast(float, (unsigned)a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+    return __builtin_bit_cast(float, (unsigned)b[0]) + __builtin_bit_cast(float, (unsigned)b[1]);
+}
+// sum over the wave, in every lane
+__device__ inline float wave_sum(float x) {
+    x += dpp<0xB1>(x);           // neighbours, pairs, halves of a row, rows
+    x += dpp<0x4E>(x);
+    x += dpp<0x141>(x);
+    x += dpp<0x140>(x);
+    return add_rows(x);
+}
+// four sums over the wave at once: lane i gets the sum of v[i % 4].  The first two steps halve the number of values a lane carries instead of adding
+// all four in every lane.
+__device__ inline float wave_sums4(const float (&v)[4], int lane) {
+    const bool odd = lane & 1, upper = lane & 2;
+    const float a = (odd ? v[1] : v[0]) + dpp<0xB1>(odd ? v[0] : v[1]);
+    const float b = (odd ? v[3] : v[2]) + dpp<0xB1>(odd ? v[2] : v[3]);
+    float c = (upper ? b : a) + dpp<0x4E>(upper ? a : b);
+    c += dpp<0x124>(c);          // the other quads of a row: rotations by 4 and 8
+    c += dpp<0x128>(c);
+    return add_rows(c);
 }
 __device__ inline void wave_sync() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
 
@@ -82,6 +96,7 @@ template <class T, int NQ, bool FAST, int WPR> struct Row {
     int64_t held;                         // row whose dropout words LDS holds (and the next one's, where two rows fit)
     int block[NQ][FAST ? 1 : 4];          // -1: no component
     int channel[NQ][4];
+    float inverse[NQ][FAST ? 1 : 4];      // 1 / components of the block
     __device__ Row(const Shape& shape, char* lds, int team) : s(shape), lane(threadIdx.x & (64 * WPR - 1)), turn(0), held(-2) {
         own = (float*)(lds + team * team_bytes(shape));
         exchange = own + own_floats(shape);
@@ -91,14 +106,16 @@ template <class T, int NQ, bool FAST, int WPR> struct Row {
             for (int i = 0; i < 4; ++i) {
                 const int c = 4 * (j * 64 * WPR + lane) + i;
                 int b = -1, ch = 0;
+                float inv = 0.0f;
 #pragma unroll
                 for (int k = 0; k < kMostBlocks; ++k) {
                     const bool in = (c >= s.start[k]) & (c < s.start[k + 1]);
                     b = in ? k : b;
+                    inv = in ? s.inverse[k] : inv;
                     ch = in ? s.first[k] + (((c - s.start[k]) * s.divide[k]) >> 16) : ch;
                 }
                 channel[j][i] = ch;
-                if (!FAST || i == 0) block[j][FAST ? 0 : i] = b;
+                if (!FAST || i == 0) { block[j][FAST ? 0 : i] = b; inverse[j][FAST ? 0 : i] = inv; }
             }
     }
     __device__ int of(int j, int i) const { return block[j][FAST ? 0 : i]; }
@@ -140,20 +157,6 @@ template <class T, int NQ, bool FAST, int WPR> struct Row {
         }
     }
     __device__ void sync() const { if constexpr (WPR == 1) wave_sync(); else __syncthreads(); }
-    // sums over the row's lanes, in every lane
-    template <int N> __device__ void row_sums(float (&v)[N]) {
-        wave_sums(v);
-        if constexpr (WPR > 1) {          // (two buffers in turn: a wave that is one exchange ahead does not touch what another still reads)
-            float* at = exchange + turn * WPR * 8;
-            turn ^= 1;
-            if ((lane & 63) == 0)
-#pragma unroll
-                for (int k = 0; k < N; ++k) at[(lane >> 6) * 8 + k] = v[k];
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < N; ++k) { v[k] = 0.0f; for (int w = 0; w < WPR; ++w) v[k] += at[w * 8 + k]; }
-        }
-    }
     // a lane's share of the sums over each block of f g
     __device__ void block_parts(float (&part)[kMostBlocks], const f4 (&f)[NQ], const f4 (&g)[NQ]) const {
 #pragma unroll
@@ -181,45 +184,82 @@ template <class T, int NQ, bool FAST, int WPR> struct Row {
             for (int i = 0; i < 4; ++i) part += of(j, i) == 0 ? f[j][i] : 0.0f;
         return part;
     }
-    __device__ float pick(const float (&v)[kMostBlocks], int j, int i) const {
-        const int b = of(j, i);
-        return b == 0 ? v[0] : b == 1 ? v[1] : b == 2 ? v[2] : v[3];
-    }
-    // f becomes its normalised value n, r the factor of each block
-    __device__ void normalise(f4 (&f)[NQ], float (&r)[kMostBlocks], float eps) {
-        if (s.scalars) {
-            float total[1] = {scalar_part(f)};
-            row_sums(total);
-            const float mean = total[0] * s.inverse[0];
+    typedef float PerQuad[NQ][FAST ? 1 : 4];
+    static __device__ float at(const PerQuad& v, int j, int i) { return v[j][FAST ? 0 : i]; }
+    // the blocks' sums of parts (by block) and the scalars' sum of one more value: each component's own block's sum, and the latter
+    __device__ float sums(PerQuad& own_sum, const float (&part)[kMostBlocks], float scalar) {
+        float c = wave_sums4(part, lane);
+        scalar = wave_sum(scalar);
+        if constexpr (WPR > 1) {          // (two buffers in turn: a wave that is one exchange ahead does not touch what another still reads)
+            float* to = exchange + turn * WPR * 8;
+            turn ^= 1;
+            if ((lane & 63) < 4) to[(lane >> 6) * 8 + (lane & 3)] = c;
+            if ((lane & 63) == 4) to[(lane >> 6) * 8 + 4] = scalar;
+            __syncthreads();
+            scalar = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WPR; ++w) scalar += to[w * 8 + 4];
 #pragma unroll
             for (int j = 0; j < NQ; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) if (of(j, i) == 0) f[j][i] -= mean;
-        }
-        block_parts(r, f, f);
-        row_sums(r);
+                for (int i = 0; i < (FAST ? 1 : 4); ++i) {
+                    own_sum[j][i] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kMostBlocks; ++k) r[k] = rsqrtf(r[k] * s.inverse[k] + eps);
+                    for (int w = 0; w < WPR; ++w) own_sum[j][i] += to[w * 8 + (block[j][i] & 3)];
+                }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NQ; ++j)
+#pragma unroll
+                for (int i = 0; i < (FAST ? 1 : 4); ++i) own_sum[j][i] = __shfl(c, (lane & ~3) | (block[j][i] & 3));
+        }
+        return scalar;
+    }
+    // the sum of one value alone
+    __device__ float sum(float x) {
+        x = wave_sum(x);
+        if constexpr (WPR > 1) {
+            float* to = exchange + turn * WPR * 8;
+            turn ^= 1;
+            if ((lane & 63) == 0) to[(lane >> 6) * 8] = x;
+            __syncthreads();
+            x = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WPR; ++w) x += to[w * 8];
+        }
+        return x;
+    }
+    // f becomes its normalised value n, r the factor of each component's block
+    __device__ void normalise(f4 (&f)[NQ], PerQuad& r, float eps) {
+        if (s.scalars) {
+            const float mean = sum(scalar_part(f)) * s.inverse[0];
+#pragma unroll
+            for (int j = 0; j < NQ; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[j][i] -= of(j, i) == 0 ? mean : 0.0f;
+        }
+        float part[kMostBlocks];
+        block_parts(part, f, f);
+        sums(r, part, 0.0f);
 #pragma unroll
         for (int j = 0; j < NQ; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) f[j][i] *= pick(r, j, i);
+            for (int i = 0; i < (FAST ? 1 : 4); ++i) r[j][i] = __builtin_amdgcn_rsqf(fmaf(r[j][i], inverse[j][i], eps));
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[j][i] *= at(r, j, i);
     }
     // g: gradient of the normalised value n -> gradient of the value before the norm
-    __device__ void normalise_back(f4 (&g)[NQ], const f4 (&n)[NQ], const float (&r)[kMostBlocks]) {
-        float part[kMostBlocks], sums[kMostBlocks + 1], dot[kMostBlocks];
+    __device__ void normalise_back(f4 (&g)[NQ], const f4 (&n)[NQ], const PerQuad& r) {
+        float part[kMostBlocks];
+        PerQuad dot;
         block_parts(part, g, n);
-#pragma unroll
-        for (int k = 0; k < kMostBlocks; ++k) sums[k] = part[k];
-        sums[kMostBlocks] = scalar_part(g);
-        row_sums(sums);
-        const float mean = sums[kMostBlocks] * s.inverse[0];
-#pragma unroll
-        for (int k = 0; k < kMostBlocks; ++k) dot[k] = sums[k] * s.inverse[k];
+        const float scalar = sums(dot, part, scalar_part(g)), mean = s.scalars ? scalar * s.inverse[0] : 0.0f;
 #pragma unroll
         for (int j = 0; j < NQ; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) g[j][i] = pick(r, j, i) * (g[j][i] - (s.scalars && of(j, i) == 0 ? mean : 0.0f) - n[j][i] * pick(dot, j, i));
+            for (int i = 0; i < 4; ++i) g[j][i] = at(r, j, i) * (g[j][i] - (of(j, i) == 0 ? mean : 0.0f) - n[j][i] * (at(dot, j, i) * at(inverse, j, i)));
     }
     // dropout factors of a row, one word for each channel, through LDS: of this row and the next at once where both fit into the row's lanes
     __device__ void keep(f4 (&f)[NQ], int64_t row, uint64_t offset, uint64_t seed, uint32_t threshold, float scale) {
@@ -291,7 +331,7 @@ template <class T, int NQ, bool FAST, int WPR> __global__ __launch_bounds__(256,
             if (P.y) {
                 R.load(y, P.y, row);
                 if (P.post_w) {
-                    float r[kMostBlocks];
+                    typename Row<T, NQ, FAST, WPR>::PerQuad r;
                     R.normalise(y, r, P.eps);
 #pragma unroll
                     for (int j = 0; j < NQ; ++j) y[j] = y[j] * pw[j] + pb[j];
@@ -309,7 +349,7 @@ template <class T, int NQ, bool FAST, int WPR> __global__ __launch_bounds__(256,
                 R.store(P.h, row, h);
             }
             if (P.z) {
-                float r[kMostBlocks];
+                typename Row<T, NQ, FAST, WPR>::PerQuad r;
                 R.normalise(h, r, P.eps);
 #pragma unroll
                 for (int j = 0; j < NQ; ++j) h[j] = h[j] * nw[j] + nb[j];
@@ -332,20 +372,20 @@ template <class T, int NQ, bool FAST, int WPR> __global__ __launch_bounds__(256,
     if (post) { R.spread(pw, P.post_w, C); R.spread(pb, P.post_b, P.s.scalars); }
     if (next) R.spread(nw, P.next_w, C);
 #pragma unroll
-    for (int j = 0; j < NQ; ++j) d_pw[j] = d_pb[j] = d_nw[j] = d_nb[j] = f4{0, 0, 0, 0};
+    for (int j = 0; j < NQ; ++j) d_pw[j] = d_pb[j] = d_nw[j] = d_nb[j] = d_gate[j] = f4{0, 0, 0, 0};
     const int units = P.groups * P.slices, group_rows = P.n_rows / P.groups;
     for (int u = blockIdx.x * TEAMS + team; u < units; u += gridDim.x * TEAMS) {
         const int g = u / P.slices, slice = u - g * P.slices, first = slice * P.slice_rows, last = min(first + P.slice_rows, group_rows);
 #pragma unroll
         for (int j = 0; j < NQ; ++j) {
-            d_gate[j] = f4{0, 0, 0, 0};
+            if (P.n_params < 5) d_gate[j] = f4{0, 0, 0, 0};
 #pragma unroll
             for (int i = 0; i < 4; ++i) gate[j][i] = P.gate ? gate_at<T>(P.gate, P.gate_f32, (int64_t)g * C + R.channel[j][i]) : 1.0f;
         }
         for (int k = first; k < last; ++k) {
             const int64_t row = (int64_t)g * group_rows + k;
             f4 h[NQ], n[NQ], y[NQ], m[NQ], up[NQ];
-            float ry[kMostBlocks];
+            typename Rw::PerQuad ry;
             R.load(h, P.x, row);
             if (P.y) R.load(y, P.y, row);
             if (P.dh) R.load(up, P.dh, row);
@@ -366,7 +406,7 @@ template <class T, int NQ, bool FAST, int WPR> __global__ __launch_bounds__(256,
             }
             if (next) {
                 f4 dz[NQ];
-                float r[kMostBlocks];
+                typename Rw::PerQuad r;
                 R.load(dz, P.dz, row);
 #pragma unroll
                 for (int j = 0; j < NQ; ++j) n[j] = h[j];
@@ -402,7 +442,7 @@ template <class T, int NQ, bool FAST, int WPR> __global__ __launch_bounds__(256,
             if (post) R.normalise_back(up, y, ry);
             R.store(P.dy, row, up);
         }
-        if (P.d_gate || P.gate_rows) {
+        if (P.n_params < 5 && (P.d_gate || P.gate_rows)) {
             R.fold(d_gate);
             for (int c = R.lane; c < C; c += 64 * WPR) {
                 const float s = R.folded(R.own, c);
@@ -414,15 +454,18 @@ template <class T, int NQ, bool FAST, int WPR> __global__ __launch_bounds__(256,
     }
     if (!P.param_rows) return;
     // the workgroup's sums, a parameter at a time
+#pragma unroll 1
+    for (int which = 0; which < P.n_params; ++which) {
+        f4 d[NQ];
 #pragma unroll
-    for (int which = 0; which < 4; ++which) {
+        for (int j = 0; j < NQ; ++j) d[j] = which == 0 ? d_pw[j] : which == 1 ? d_pb[j] : which == 2 ? d_nw[j] : which == 3 ? d_nb[j] : d_gate[j];
         __syncthreads();
-        if (which == 0) R.fold(d_pw); else if (which == 1) R.fold(d_pb); else if (which == 2) R.fold(d_nw); else R.fold(d_nb);
+        R.fold(d);
         __syncthreads();
         for (int c = threadIdx.x; c < C; c += 256) {
             float s = 0.0f;
             for (int x = 0; x < TEAMS; ++x) s += R.folded((const float*)(lds + x * Rw::team_bytes(P.s)), c);
-            P.param_rows[((int64_t)blockIdx.x * 4 + which) * C + c] = s;
+            P.param_rows[((int64_t)blockIdx.x * P.n_params + which) * C + c] = s;
         }
     }
 }
@@ -451,23 +494,33 @@ template <class T, int NQ, bool FAST, int WPR> __global__ __launch_bounds__(256)
     }
 }
 
-// sums over `rows` rows of (rows, columns) in 64 bits, in order; 16 columns a workgroup, one of blockIdx.y matrices.  Output column c goes to
-// out[c / width] + c % width (an absent output is skipped), as 32 bits or as T.
-template <class T> __global__ __launch_bounds__(256) void k_row_sums(const float* x, int rows, int columns, int width, float* o0, float* o1, float* o2, float* o3, int n1, int n3, T* narrow) {
-    __shared__ double share[16][16];
+// sums over `rows` rows of (rows, columns) in 64 bits, in a fixed order; 16 columns a workgroup, one of blockIdx.y matrices.  Column c is element
+// c % width of output c / width: its first n elements are written, as 32 bits or as T.
+struct Outputs { void* to[5]; int n[5]; int narrow[5]; };
+template <class T> __global__ __launch_bounds__(1024) void k_row_sums(const float* x, int rows, int columns, int width, Outputs out) {
+    __shared__ double share[64][17];
     const int c = blockIdx.x * 16 + (threadIdx.x & 15), r0 = threadIdx.x >> 4;
-    const float* m = x + (size_t)blockIdx.y * rows * columns;
+    const float* m = x + (size_t)blockIdx.y * rows * columns + c;
     double s = 0.0;
-    if (c < columns) for (int r = r0; r < rows; r += 16) s += (double)m[(size_t)r * columns + c];
+    if (c < columns) {
+        int r = r0;
+        for (; r + 3 * 64 < rows; r += 4 * 64) {
+            const float a = m[(size_t)r * columns], b = m[(size_t)(r + 64) * columns], d = m[(size_t)(r + 128) * columns], e = m[(size_t)(r + 192) * columns];
+            s += ((double)a + (double)b) + ((double)d + (double)e);
+        }
+        for (; r < rows; r += 64) s += (double)m[(size_t)r * columns];
+    }
     share[r0][threadIdx.x & 15] = s;
-    __syncthreads();
+    for (int half = 32; half >= 1; half >>= 1) {
+        __syncthreads();
+        if (r0 < half) share[r0][threadIdx.x & 15] += share[r0 + half][threadIdx.x & 15];
+    }
     if (r0 != 0 || c >= columns) return;
-    for (int r = 1; r < 16; ++r) s += share[r][threadIdx.x];
-    if (narrow) { narrow[(size_t)blockIdx.y * columns + c] = (T)(float)s; return; }
     const int which = c / width, at = c - which * width;
-    float* o = which == 0 ? o0 : which == 1 ? o1 : which == 2 ? o2 : o3;
-    const int n = which == 1 ? n1 : which == 3 ? n3 : width;
-    if (o && at < n) o[(size_t)blockIdx.y * n + at] = (float)s;
+    if (!out.to[which] || at >= out.n[which]) return;
+    const float v = (float)share[0][threadIdx.x & 15];
+    const size_t to = (size_t)blockIdx.y * out.n[which] + at;
+    if (out.narrow[which]) ((T*)out.to[which])[to] = (T)v; else ((float*)out.to[which])[to] = v;
 }
 
 }  // namespace rows

@@ -68,7 +68,7 @@ int make_args(const dedf_norm* x, bool backward, Args& a, bool& fast) {
     if (x->n_rows > 0 && (!x->x || groups < 1 || groups > x->n_rows || x->n_rows % groups != 0)) return DEDF_ERR_INVALID;
     if (x->n_rows > 0 && !x->y && (x->gate || x->post_weight || x->dropout != 0.0)) return DEDF_ERR_INVALID;
     if (a.s.scalars > 0 && ((x->post_weight && !x->post_bias) || (x->next_weight && !x->next_bias))) return DEDF_ERR_INVALID;
-    if (!(x->dropout >= 0.0 && x->dropout < 1.0) || (x->dropout > 0.0 && !x->rng) || !(x->eps > 0.0f)) return DEDF_ERR_INVALID;
+    if (!(x->dropout >= 0.0 && x->dropout < 1.0) || (x->dropout > 0.0 && !x->rng) || !(x->eps >= 1e-30f)) return DEDF_ERR_INVALID;
     a.n_rows = x->n_rows; a.groups = std::max(1, groups);
     a.x = x->x; a.y = x->y; a.gate = x->gate; a.gate_f32 = x->type == DEDF_F32 || x->gate_f;
     a.post_w = x->post_weight; a.post_b = x->post_bias; a.next_w = x->next_weight; a.next_b = x->next_bias;
@@ -102,11 +102,12 @@ struct NormBackward {
     template <class T, int NQ, bool FAST, int WPR> int run() {
         const int blocks = grid(a, norm_blocks(true, a.s.width)), C = a.s.channels;
         hipLaunchKernelGGL((k_norm_backward<T, NQ, FAST, WPR>), dim3(blocks), dim3(256), lds_bytes(a), st, a);
+        const int narrow = a.gate_f32 ? 0 : 1;
         if (a.param_rows)
-            hipLaunchKernelGGL(k_row_sums<T>, dim3((4 * C + 15) / 16), dim3(256), 0, st, (const float*)a.param_rows, blocks, 4 * C, C, post_w, post_b, next_w, next_b, a.s.scalars, a.s.scalars, (T*)nullptr);
+            hipLaunchKernelGGL(k_row_sums<T>, dim3((a.n_params * C + 15) / 16), dim3(1024), 0, st, (const float*)a.param_rows, blocks, a.n_params * C, C,
+                               Outputs{{post_w, post_b, next_w, next_b, a.d_gate}, {C, a.s.scalars, C, a.s.scalars, C}, {0, 0, 0, 0, narrow}});
         if (a.gate_rows)
-            hipLaunchKernelGGL(k_row_sums<T>, dim3((C + 15) / 16, a.groups), dim3(256), 0, st, (const float*)a.gate_rows, a.slices, C, C,
-                               a.gate_f32 ? (float*)a.d_gate : nullptr, (float*)nullptr, (float*)nullptr, (float*)nullptr, 0, 0, a.gate_f32 ? (T*)nullptr : (T*)a.d_gate);
+            hipLaunchKernelGGL(k_row_sums<T>, dim3((C + 15) / 16, a.groups), dim3(1024), 0, st, (const float*)a.gate_rows, a.slices, C, C, Outputs{{a.d_gate}, {C}, {narrow}});
         return hipGetLastError() == hipSuccess ? DEDF_OK : DEDF_ERR_RUNTIME;
     }
 };
@@ -144,8 +145,8 @@ namespace {
 template <class F> int by_shape(int type, int width, bool fast, F f) {
     return type == DEDF_F32 ? launch<float>(width, fast, f) : type == DEDF_F16 ? launch<_Float16>(width, fast, f) : launch<__bf16>(width, fast, f);
 }
-size_t param_bytes(const Args& a) { return (size_t)grid(a, norm_blocks(true, a.s.width)) * 4 * a.s.channels * 4; }
-size_t gate_bytes(const Args& a) { return a.gate && a.slices > 1 ? (size_t)a.groups * a.slices * a.s.channels * 4 : 0; }
+size_t param_bytes(const Args& a) { return (size_t)grid(a, norm_blocks(true, a.s.width)) * 5 * a.s.channels * 4; }
+size_t gate_bytes(const Args& a) { return a.gate && a.groups > 1 && a.slices > 1 ? (size_t)a.groups * a.slices * a.s.channels * 4 : 0; }
 size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
 }  // namespace
@@ -180,16 +181,18 @@ int dedf_norm_gate_residual_backward(const dedf_norm* x, const void* grad_h, con
     const bool params = d_post_weight || d_post_bias || d_next_weight || d_next_bias;
     if (a.n_rows == 0) {          // no row: the parameters' gradients are zero (a sum over no rows); the caller's gate gradient has no element
         const int C = a.s.channels;
-        if (params) hipLaunchKernelGGL(k_row_sums<float>, dim3((4 * C + 15) / 16), dim3(256), 0, st, (const float*)nullptr, 0, 4 * C, C, d_post_weight, d_post_bias,
-                                       d_next_weight, d_next_bias, a.s.scalars, a.s.scalars, (float*)nullptr);
+        if (params) hipLaunchKernelGGL(k_row_sums<float>, dim3((4 * C + 15) / 16), dim3(1024), 0, st, (const float*)nullptr, 0, 4 * C, C,
+                                       Outputs{{d_post_weight, d_post_bias, d_next_weight, d_next_bias, nullptr}, {C, a.s.scalars, C, a.s.scalars, 0}, {}});
         return hipGetLastError() == hipSuccess ? DEDF_OK : DEDF_ERR_RUNTIME;
     }
     if ((!grad_h && !grad_z) || (grad_z && !x->next_weight) || (d_y && !x->y) || (d_gate && !x->gate)) return DEDF_ERR_INVALID;
     const size_t need = up16(param_bytes(a)) + gate_bytes(a);
     if (!scratch || scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 15)) return DEDF_ERR_INVALID;
     a.dh = grad_h; a.dz = grad_z; a.dx = d_x; a.dy = d_y; a.d_gate = d_gate;
-    a.gate_rows = d_gate && a.slices > 1 ? (float*)((char*)scratch + up16(param_bytes(a))) : nullptr;
-    a.param_rows = params ? (float*)scratch : nullptr;
+    const bool shared_gate = d_gate && a.groups == 1;          // a gradient like the norms' weights
+    a.gate_rows = d_gate && !shared_gate && a.slices > 1 ? (float*)((char*)scratch + up16(param_bytes(a))) : nullptr;
+    a.param_rows = params || shared_gate ? (float*)scratch : nullptr;
+    a.n_params = shared_gate ? 5 : 4;
     fast = fast && on_quads(x->type, {a.x, a.y, grad_h, grad_z, d_x, d_y});
     NormBackward f{a, st, d_post_weight, d_post_bias, d_next_weight, d_next_bias};
     return by_shape(x->type, a.s.width, fast, f);

@@ -105,8 +105,8 @@ def norm_gate_residual(x: torch.Tensor, y: torch.Tensor, irreps, scale: float = 
         gate = gate.contiguous()
     post_weight, post_bias = _check_affine("post", post_weight, post_bias, shape)
     next_weight, next_bias = _check_affine("next", next_weight, next_bias, shape)
-    if not eps > 0.0:
-        raise ValueError(f"eps {eps}: positive")
+    if not eps >= 1e-30:
+        raise ValueError(f"eps {eps}: at least 1e-30")
     p = check_dropout(dropout, rng, x.device)
     rng = rng.contiguous() if p > 0.0 else None
     check_gpu("norm_gate_residual", x, y, gate, post_weight, post_bias, next_weight, next_bias)
@@ -120,8 +120,8 @@ def equivariant_layer_norm(x: torch.Tensor, irreps, weight: torch.Tensor, bias: 
     weight, bias = _check_affine("next", weight, bias, shape)
     if weight is None:
         raise ValueError(f"weight: float32 ({shape.channels},)")
-    if not eps > 0.0:
-        raise ValueError(f"eps {eps}: positive")
+    if not eps >= 1e-30:
+        raise ValueError(f"eps {eps}: at least 1e-30")
     check_gpu("equivariant_layer_norm", x, weight, bias)
     return _run(shape, x.contiguous(), None, None, None, None, weight, bias, 1.0, float(eps), 0.0, None)[1]
 
