@@ -75,46 +75,34 @@ def check_dropout(p: float, rng: Optional[torch.Tensor], device: torch.device) -
 def check_gpu(what: str, *tensors) -> torch.device:
     """-> the one GPU that all tensors (None among them) are on"""
     dev = tensors[0].device
-    if any(t is not None and t.device != dev for t in tensors):
-        raise ValueError(f"{what}: tensors on different devices")
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what}: tensors on different devices")
     if dev.type != "cuda":
         raise RuntimeError(f"{what} needs GPU tensors: the product has no CPU path")
     return dev
 
 
-class on_device:
-    """``torch.cuda.device`` where it is not the current one already"""
-
-    def __init__(self, device: torch.device):
-        self.index, self.inner = device.index, None
-
-    def __enter__(self):
-        if self.index is not None and self.index != torch.cuda.current_device():
-            self.inner = torch.cuda.device(self.index)
-            self.inner.__enter__()
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *a):
-        if self.inner is not None:
-            self.inner.__exit__(*a)
+def launch(what: str, device: torch.device, call, *args) -> None:
+    """``call(*args, stream)`` on the device's current stream (with the device current: the library launches there); raises for what it returns"""
+    if device.index == torch.cuda.current_device():
+        rc = call(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = call(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if rc != _lib.OK:
+        raise (ValueError if rc == _lib.ERR_INVALID else NotImplementedError if rc == _lib.ERR_UNSUPPORTED else RuntimeError)(f"{what} failed ({rc})")
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-def check_rc(what: str, rc: int) -> None:
-    if rc == _lib.OK:
-        return
-    raise (ValueError if rc == _lib.ERR_INVALID else NotImplementedError if rc == _lib.ERR_UNSUPPORTED else RuntimeError)(f"{what} failed ({rc})")
-
-
 def _launch(x: torch.Tensor, shape: RowShape, p: float, rng: Optional[torch.Tensor], keep_rng: bool):
     out = torch.empty_like(x)
     used = torch.empty(2, dtype=torch.int64, device=x.device) if keep_rng else None
-    with on_device(x.device) as stream:
-        check_rc("dedf_channel_dropout", _lib.load().dedf_channel_dropout(TYPES[x.dtype], len(x), len(shape.blocks), shape.mul, shape.degree, x.data_ptr(), p,
-                                                                          ptr(rng), out.data_ptr(), ptr(used), stream))
+    launch("dedf_channel_dropout", x.device, _lib.load().dedf_channel_dropout, TYPES[x.dtype], x.shape[0], len(shape.blocks), shape.mul, shape.degree,
+           x.data_ptr(), p, ptr(rng), out.data_ptr(), ptr(used))
     return out, used
 
 

@@ -11,7 +11,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from .drop import TYPES, check_dropout, check_gpu, check_rc, on_device, ptr
+from .drop import TYPES, check_dropout, check_gpu, launch, ptr
 
 
 class EdgeSegments:
@@ -32,8 +32,7 @@ class EdgeSegments:
         self.rowptr = torch.empty(n_dst + 1, dtype=torch.int32, device=dev)
         bad = torch.zeros(1, dtype=torch.int32, device=dev)
         edge_dst = edge_dst.contiguous()
-        with on_device(dev) as stream:
-            check_rc("dedf_edge_segments", _lib.load().dedf_edge_segments(ptr(edge_dst), self.n_edges, n_dst, ptr(self.dst), ptr(self.rowptr), ptr(bad), stream))
+        launch("dedf_edge_segments", dev, _lib.load().dedf_edge_segments, ptr(edge_dst), self.n_edges, n_dst, ptr(self.dst), ptr(self.rowptr), ptr(bad))
         if bad.item():
             raise ValueError(f"edge_dst is not ascending or leaves [0, {n_dst})")
 
@@ -49,7 +48,7 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 
 
 def _struct(seg: EdgeSegments, alpha, value, alpha_dot, logits, length, bounds, table, p, rng) -> _lib.DedfEdgeAttn:
-    return _lib.DedfEdgeAttn(seg.n_edges, seg.n_dst, alpha.shape[1], alpha.shape[2], value.shape[2], TYPES[value.dtype], 0 if table is None else len(table),
+    return _lib.DedfEdgeAttn(seg.n_edges, seg.n_dst, alpha.shape[1], alpha.shape[2], value.shape[2], TYPES[value.dtype], 0 if table is None else table.shape[0],
                              ptr(alpha), alpha.stride(0), ptr(value), value.stride(0), ptr(alpha_dot), ptr(seg.dst), ptr(seg.rowptr), ptr(logits), ptr(length),
                              ptr(bounds), ptr(table), p, ptr(rng))
 
@@ -65,8 +64,7 @@ def _forward(seg, alpha, value, alpha_dot, logits, length, bounds, table, p, rng
         norm = torch.empty(seg.n_dst, H, 2, dtype=torch.float64, device=dev)
         used = torch.empty(2, dtype=torch.int64, device=dev) if p > 0.0 else None
     scratch = torch.empty(lib.dedf_edge_attention_scratch_bytes(C.byref(a), 0), dtype=torch.uint8, device=dev)
-    with on_device(dev) as stream:
-        check_rc("dedf_edge_attention", lib.dedf_edge_attention(C.byref(a), ptr(out), ptr(out_f), ptr(norm), ptr(used), ptr(scratch), scratch.numel(), stream))
+    launch("dedf_edge_attention", dev, lib.dedf_edge_attention, C.byref(a), ptr(out), ptr(out_f), ptr(norm), ptr(used), ptr(scratch), scratch.numel())
     return out, out_f, norm, used
 
 
@@ -90,9 +88,8 @@ class _EdgeAttention(torch.autograd.Function):
         d_dot, d_logits, d_table = (torch.empty_like(t) if n else None for n, t in zip(need[2:5], (alpha_dot, logits, table)))
         lib = _lib.load()
         scratch = torch.empty(lib.dedf_edge_attention_scratch_bytes(C.byref(a), 1), dtype=torch.uint8, device=dev)
-        with on_device(dev) as stream:
-            check_rc("dedf_edge_attention_backward", lib.dedf_edge_attention_backward(
-                C.byref(a), ptr(norm), ptr(out_f), ptr(grad), ptr(d_alpha), ptr(d_value), ptr(d_dot), ptr(d_logits), ptr(d_table), ptr(scratch), scratch.numel(), stream))
+        launch("dedf_edge_attention_backward", dev, lib.dedf_edge_attention_backward, C.byref(a), ptr(norm), ptr(out_f), ptr(grad), ptr(d_alpha), ptr(d_value),
+               ptr(d_dot), ptr(d_logits), ptr(d_table), ptr(scratch), scratch.numel())
         return d_alpha, d_value, d_dot, d_logits, d_table, None, None, None, None, None
 
 

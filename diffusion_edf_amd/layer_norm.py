@@ -9,11 +9,11 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .drop import RowShape, TYPES, check_dropout, check_gpu, check_rc, check_rows, on_device, ptr, row_shape
+from .drop import RowShape, TYPES, check_dropout, check_gpu, check_rows, launch, ptr, row_shape
 
 
 def _struct(shape: RowShape, x, y, gate, scale, eps, post_w, post_b, next_w, next_b, p, rng) -> _lib.DedfNorm:
-    return _lib.DedfNorm(TYPES[x.dtype], len(x), len(shape.blocks), 1 if gate is None else len(gate), shape.mul, shape.degree, x.data_ptr(), ptr(y), ptr(gate),
+    return _lib.DedfNorm(TYPES[x.dtype], x.shape[0], len(shape.blocks), 1 if gate is None else gate.shape[0], shape.mul, shape.degree, x.data_ptr(), ptr(y), ptr(gate),
                          int(gate is not None and gate.dtype == torch.float32), scale, eps, ptr(post_w), ptr(post_b), ptr(next_w), ptr(next_b), p, ptr(rng))
 
 
@@ -22,8 +22,7 @@ def _forward(shape, x, y, gate, scale, eps, post_w, post_b, next_w, next_b, p, r
     h = torch.empty_like(x) if y is not None else None
     z = torch.empty_like(x) if next_w is not None else None
     used = torch.empty(2, dtype=torch.int64, device=x.device) if keep_rng and p > 0.0 else None
-    with on_device(x.device) as stream:
-        check_rc("dedf_norm_gate_residual", _lib.load().dedf_norm_gate_residual(C.byref(a), ptr(h), ptr(z), ptr(used), stream))
+    launch("dedf_norm_gate_residual", x.device, _lib.load().dedf_norm_gate_residual, C.byref(a), ptr(h), ptr(z), ptr(used))
     return h, z, used
 
 
@@ -50,9 +49,8 @@ class _NormGateResidual(torch.autograd.Function):
         params = [torch.empty_like(t) if n else None for n, t in zip(need[3:7], (post_w, post_b, next_w, next_b))]
         lib = _lib.load()
         scratch = torch.empty(lib.dedf_norm_scratch_bytes(C.byref(a)), dtype=torch.uint8, device=x.device)
-        with on_device(x.device) as stream:
-            check_rc("dedf_norm_gate_residual_backward", lib.dedf_norm_gate_residual_backward(
-                C.byref(a), ptr(grad_h), ptr(grad_z), ptr(d_x), ptr(d_y), ptr(d_gate), *map(ptr, params), ptr(scratch), scratch.numel(), stream))
+        launch("dedf_norm_gate_residual_backward", x.device, lib.dedf_norm_gate_residual_backward, C.byref(a), ptr(grad_h), ptr(grad_z), ptr(d_x), ptr(d_y),
+               ptr(d_gate), *map(ptr, params), scratch.data_ptr(), scratch.numel())
         return (d_x, d_y, d_gate, *params, None, None, None, None, None)
 
 
