@@ -5,7 +5,7 @@
 //   p      = softmax of t over the edges of a destination; an edge and head with t = -inf takes no part
 //   P      = p m / (1 - q)                        m from Philox4x32-10, key = seed, counter = (edge, head / 4, offset), word head % 4
 //   out[n,h,:] = sum_e P v[e,h,:]
-// backward, from a row and head's maximum M and sum Z = sum exp(t - M) alone (the probabilities are recomputed, the mask is drawn again):
+// backward, from a logit M near a row and head's largest and 1 / Z, Z = sum exp(t - M), alone (the probabilities are recomputed, the mask is drawn again):
 //   p = exp(t - M) / Z   dP = m/(1-q) (dout . v)   delta = dout . out   dt = p (dP - delta)
 //   dv = P dout   dl = sum_h dt   dT[b,h] = sum dt   dw = sum_e dt act(a)   da = dt w act'(a)
 //
@@ -181,8 +181,8 @@ template <class T, int SUB, bool VEC, int NV> struct Wave {
         const uint32_t lo = h & 1 ? x.w[1] : x.w[0], hi = h & 1 ? x.w[3] : x.w[2];
         return (h & 2 ? hi : lo) >= P.threshold ? P.keep_scale : 0.0f;
     }
-    // t of the edges e_first .. e_first + GA - 1 into LDS
-    __device__ void logits(const Raw (&a)[NA], int e_first) {
+    // sums over a quad (or single products) of act(a) w for the edges e_first .. e_first + GA - 1, into LDS
+    __device__ void partial_logits(const Raw (&a)[NA], int e_first) {
         const int subs = sub_a == 4 ? qa : 4 * qa;
         wave_sync();
 #pragma unroll
@@ -197,19 +197,22 @@ template <class T, int SUB, bool VEC, int NV> struct Wave {
             else *(f4*)(part + e * subs + 4 * q) = x * wq;
         }
         wave_sync();
-        for (int idx = lane; idx < GA * H; idx += 64) {
-            const int e = (int)((idx * inv_h) >> 16), h = idx - e * H, eb = e_first + e;
-            float s = 0.0f;
-            for (int i = 0; i < n_sub_a; ++i) s += part[e * subs + h * n_sub_a + i];
-            const float l = e_logit[eb];
-            double x = (double)s + (double)l;
-            if (P.n_buckets) { const float b = table[e_bucket[eb] * H + h]; x = b == -__builtin_inff() ? (double)b : x + (double)b; }
-            if (l == -__builtin_inff()) x = -__builtin_inf();          // a masked edge takes no part whatever its features hold
-            if (x == __builtin_inf()) x = __builtin_nan("");
-            t[eb * H + h] = x;
-        }
+    }
+    // t of edge e_first + e and head h
+    __device__ double logit(int e_first, int e, int h) const {
+        const int subs = sub_a == 4 ? qa : 4 * qa, eb = e_first + e;
+        float s = 0.0f;
+        for (int i = 0; i < n_sub_a; ++i) s += part[e * subs + h * n_sub_a + i];
+        const float l = e_logit[eb];
+        double x = (double)s + (double)l;
+        if (P.n_buckets) { const float b = table[e_bucket[eb] * H + h]; x = b == -__builtin_inff() ? (double)b : x + (double)b; }
+        if (l == -__builtin_inff()) x = -__builtin_inf();          // a masked edge takes no part whatever its features hold
+        return x == __builtin_inf() ? __builtin_nan("") : x;
     }
 };
+
+// a value of another lane of the row of 16: rotations by 4 (0x124) and 8, the neighbour (0xB1), the other pair (0x4E), the mirrored half (0x141)
+template <int CTRL> __device__ inline float ror(float x) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true)); }
 
 // ---- forward --------------------------------------------------------------------------------------------------------------------------------
 
@@ -294,7 +297,7 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
         } else finish_row<T, SUB, VEC, NV>(P, cur, r, lane, qv, HD, out, out32, norm);
     };
     float2* share = (float2*)w.keep;                       // [16][H] share of the piece, and that share times the dropout factor
-    double* top = (double*)(w.e_bucket + kBatch);          // [16][H] largest logit of the piece
+    double* top = (double*)(w.e_bucket + kBatch);          // [16][H] logit that the shares are relative to
     typename W::Edge edge = w.request(w.e0);
     // R value rows are always in flight: a row's registers are loaded again, R edges ahead, as soon as it has been added
     constexpr int R = W::R;
@@ -306,38 +309,65 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
         w.begin(base, edge);
         edge = w.request(min(base + kBatch, w.e1 - 1));
         for (int g = 0; g < kBatch && g < w.n; g += GA) {
-            w.logits(a, g);
+            w.partial_logits(a, g);
             // the next features are on their way while this group is summed up
             if (g + GA < kBatch && g + GA < w.n) w.load_a(a, base, w.n, g + GA);
             else if (base + kBatch < w.e1) w.load_a(a, base + kBatch, (int)min((int64_t)kBatch, w.e1 - base - kBatch), 0);
-            wave_sync();
-            // a "piece" is what one row has in this group: shares relative to the piece's own maximum
+            // A "piece" is what one row has in this group.  Shares are relative to a logit that every lane of a head agrees on; any within e^60 of the piece's
+            // own largest keeps full precision.
             const uint32_t starts = (w.starts >> g) | 1u;
             const int live = min(GA, w.n - g);
-#pragma unroll 1
-            for (int idx = lane; idx < GA * H; idx += 64) {
-                const int e = (int)((idx * w.inv_h) >> 16), h = idx - e * H;
-                const uint32_t upto = starts & ((2u << e) - 1u), after = starts & ~((2u << e) - 1u);
-                const int from = 31 - __builtin_clz(upto), to = min(after ? __builtin_ctz(after) : GA, live);
-                double most = -__builtin_inf();
-#pragma unroll
-                for (int k = 0; k < GA; ++k) {
-                    const double o = w.t[(g + k) * H + h];
-                    if (k >= from && k < to) most = __builtin_fmax(most, o);
+            bool near = false;
+            uint64_t some = ~(uint64_t)0;          // bit 4 e: edge e takes part somewhere
+            bool select = true;                    // an edge may take part in one head and not in another
+            if (GA == 16 && H == 4) {
+                // one edge and head a lane: the largest and smallest logits of the group, through the wave
+                const int e = lane >> 2, h = lane & 3;
+                const double x = w.logit(g, e, h);
+                const bool in = e < live && x != -__builtin_inf();
+                float most = in ? (float)x : -__builtin_inff(), least = in ? (float)x : __builtin_inff();
+                most = fmaxf(most, ror<0x124>(most)); least = fminf(least, ror<0x124>(least));
+                most = fmaxf(most, ror<0x128>(most)); least = fminf(least, ror<0x128>(least));
+                most = fmaxf(most, __shfl_xor(most, 16)); least = fminf(least, __shfl_xor(least, 16));
+                most = fmaxf(most, __shfl_xor(most, 32)); least = fminf(least, __shfl_xor(least, 32));
+                near = __ballot(most != -__builtin_inff() && !(most - least <= 60.0f && fabsf(most) <= 1e6f)) == 0;
+                if (near) {
+                    const float p = in ? exp_d(x - (double)most) : 0.0f;
+                    share[(g + e) * 4 + h] = float2{p, in ? p * w.dropped(base + g + e, h) : 0.0f};
+                    top[(g + e) * 4 + h] = (double)most;
+                    const uint64_t b = __ballot(in), heads = 0x1111111111111111ull;
+                    some = b | b >> 1 | b >> 2 | b >> 3;
+                    select = ((some ^ (b & b >> 1 & b >> 2 & b >> 3)) & heads) != 0;
+                } else w.t[(g + e) * 4 + h] = x;
+            } else {
+                for (int idx = lane; idx < GA * H; idx += 64) {
+                    const int e = (int)((idx * w.inv_h) >> 16), h = idx - e * H;
+                    w.t[(g + e) * H + h] = w.logit(g, e, h);
                 }
-                const double x = w.t[(g + e) * H + h];
-                const float p = x == -__builtin_inf() ? 0.0f : exp_d(x - most);
-                share[(g + e) * H + h] = float2{p, e < live ? p * w.dropped(base + g + e, h) : 0.0f};
-                top[(g + e) * H + h] = most;
             }
             wave_sync();
+            if (!near) {          // relative to the piece's own largest logit
+#pragma unroll 1
+                for (int idx = lane; idx < GA * H; idx += 64) {
+                    const int e = (int)((idx * w.inv_h) >> 16), h = idx - e * H;
+                    const uint32_t upto = starts & ((2u << e) - 1u), after = starts & ~((2u << e) - 1u);
+                    const int from = 31 - __builtin_clz(upto), to = min(after ? __builtin_ctz(after) : GA, live);
+                    double most = -__builtin_inf();
+                    for (int k = from; k < to; ++k) most = __builtin_fmax(most, w.t[(g + k) * H + h]);
+                    const double x = w.t[(g + e) * H + h];
+                    const float p = e >= live || x == -__builtin_inf() ? 0.0f : exp_d(x - most);
+                    share[(g + e) * H + h] = float2{p, e < live ? p * w.dropped(base + g + e, h) : 0.0f};
+                    top[(g + e) * H + h] = most;
+                }
+                wave_sync();
+            }
             float scale[NV][PARTS];
 #pragma unroll 1
             for (int s = 0; s < GA; s += R)
 #pragma unroll
             for (int i = 0; i < R; ++i) {
                 const int e = s + i;
-                if (g + e < w.n) {
+                if (e < live) {
                     if ((starts >> e) & 1u) {
                         const int d = __builtin_amdgcn_readfirstlane(w.e_dst[g + e]);
                         if (d != cur) { flush(false); cur = d; first_row = false; r.clear(); }
@@ -352,6 +382,7 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
                                 for (int c = 0; c < SUB; ++c) r.acc[j][p * SUB + c] *= w_old;
                             }
                     }
+                    if (GA != 16 || (some >> ((4 * e) & 63)) & 1)
 #pragma unroll
                     for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -360,7 +391,11 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
                             const float k = f.y * scale[j][p];
                             r.sum[j][p] = fmaf(f.x, scale[j][p], r.sum[j][p]);
 #pragma unroll
-                            for (int c = 0; c < SUB; ++c) r.acc[j][p * SUB + c] = k == 0.0f ? r.acc[j][p * SUB + c] : fmaf(k, (float)v[i][j][p * SUB + c], r.acc[j][p * SUB + c]);
+                            for (int c = 0; c < SUB; ++c) {
+                                // (what a head does not look at may be NaN)
+                                const float x = select && f.x == 0.0f ? 0.0f : (float)v[i][j][p * SUB + c];
+                                r.acc[j][p * SUB + c] = fmaf(k, x, r.acc[j][p * SUB + c]);
+                            }
                         }
                 }
                 w.load_row(v[i], w.value_row(base + g + e + R));
@@ -371,21 +406,17 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
     flush(w.e1 < P.n_edges && P.dst[w.e1] == cur);
 }
 
-// Rows that cross ranges: workgroup b looks at the border between ranges b and b + 1, and joins a row whose first crossing that is.  Each wave joins
-// every fourth record, then the four are joined in order.
-template <class T, int SUB, bool VEC, int NV> __global__ __launch_bounds__(256)
+// Rows that cross ranges.  A wave looks at one border between two ranges and takes a row whose first crossing that is: it joins up to 8 records by itself;
+// a longer row is joined by the whole workgroup, every wave a share of the records, then the waves' results in order.
+template <int NV> constexpr int merge_waves() { return 16 / NV; }
+template <class T, int SUB, bool VEC, int NV> __global__ __launch_bounds__(1024 / NV)
 void k_attn_merge(Args P, T* out, float* out32, double* norm, const void* records) {
-    constexpr int PARTS = 4 / SUB;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, H = P.heads, HD = H * P.d, qv = (HD + 3) >> 2;
-    const int64_t border = ((int64_t)blockIdx.x + 1) * P.range;
-    const int row = P.dst[border];
-    if (P.dst[border - 1] != row) return;
-    const int64_t begin = P.rowptr[row], w0 = blockIdx.x;
-    if (begin < w0 * P.range) return;                                   // an earlier border is its first
-    const int64_t w1 = ((int64_t)P.rowptr[row + 1] - 1) / P.range;
+    constexpr int PARTS = 4 / SUB, WAVES = merge_waves<NV>();
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), H = P.heads, HD = H * P.d, qv = (HD + 3) >> 2;
+    __shared__ Record<NV, PARTS> share[WAVES - 1][64];
+    __shared__ int long_row[WAVES], long_first[WAVES];
     const Record<NV, PARTS>* rec = (const Record<NV, PARTS>*)records + lane;
     Row<NV, PARTS> r;
-    r.clear();
     auto join = [&](const f4 (&acc)[NV], const double (&m)[NV][PARTS], const float (&sum)[NV][PARTS]) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
@@ -398,20 +429,45 @@ void k_attn_merge(Args P, T* out, float* out32, double* norm, const void* record
                 for (int i = 0; i < SUB; ++i) r.acc[j][p * SUB + i] = fmaf(acc[j][p * SUB + i], w_new, r.acc[j][p * SUB + i] * w_old);
             }
     };
-#pragma unroll 2
-    for (int64_t x = w0 + wave; x <= w1; x += kWaves) {
-        const Record<NV, PARTS> o = rec[(x * 2 + (x == w0 && begin > w0 * P.range ? 1 : 0)) * 64];
-        join(o.acc, o.m, o.sum);
-    }
-    __shared__ Record<NV, PARTS> share[kWaves - 1][64];
-    if (wave > 0) {
-        Record<NV, PARTS>& o = share[wave - 1][lane];
-        for (int j = 0; j < NV; ++j) { o.acc[j] = r.acc[j]; for (int p = 0; p < PARTS; ++p) { o.m[j][p] = r.m[j][p]; o.sum[j][p] = r.sum[j][p]; } }
+    // records first, first + step, .. <= last of a row that begins at edge `begin`, in range w0
+    auto join_records = [&](int64_t w0, int64_t begin, int64_t first, int64_t last, int step) {
+        r.clear();
+        constexpr int AHEAD = PARTS == 1 ? 4 : 1;
+#pragma unroll AHEAD
+        for (int64_t x = first; x <= last; x += step) {
+            const Record<NV, PARTS> o = rec[(x * 2 + (x == w0 && begin > w0 * P.range ? 1 : 0)) * 64];
+            join(o.acc, o.m, o.sum);
+        }
+    };
+    const int64_t mine = (int64_t)blockIdx.x * WAVES + wave, border = (mine + 1) * P.range;
+    if (lane == 0) long_row[wave] = -1;
+    if (border < P.n_edges) {
+        const int row = __builtin_amdgcn_readfirstlane(P.dst[border]);
+        if (P.dst[border - 1] == row) {
+            const int64_t begin = P.rowptr[row], last = ((int64_t)P.rowptr[row + 1] - 1) / P.range;
+            if (begin >= mine * P.range) {                              // (else an earlier border is its first)
+                if (last - mine < 8) { join_records(mine, begin, mine, last, 1); finish_row<T, SUB, VEC, NV>(P, row, r, lane, qv, HD, out, out32, norm); }
+                else if (lane == 0) { long_row[wave] = row; long_first[wave] = (int)mine; }
+            }
+        }
     }
     __syncthreads();
-    if (wave > 0) return;
-    for (int o = 0; o < kWaves - 1; ++o) join(share[o][lane].acc, share[o][lane].m, share[o][lane].sum);
-    finish_row<T, SUB, VEC, NV>(P, row, r, lane, qv, HD, out, out32, norm);
+    for (int i = 0; i < WAVES; ++i) {
+        const int row = long_row[i];
+        if (row < 0) continue;
+        const int64_t w0 = long_first[i], begin = P.rowptr[row], last = ((int64_t)P.rowptr[row + 1] - 1) / P.range;
+        join_records(w0, begin, w0 + wave, last, WAVES);
+        if (wave > 0) {
+            Record<NV, PARTS>& o = share[wave - 1][lane];
+            for (int j = 0; j < NV; ++j) { o.acc[j] = r.acc[j]; for (int p = 0; p < PARTS; ++p) { o.m[j][p] = r.m[j][p]; o.sum[j][p] = r.sum[j][p]; } }
+        }
+        __syncthreads();
+        if (wave == 0) {
+            for (int o = 0; o < WAVES - 1; ++o) join(share[o][lane].acc, share[o][lane].m, share[o][lane].sum);
+            finish_row<T, SUB, VEC, NV>(P, row, r, lane, qv, HD, out, out32, norm);
+        }
+        __syncthreads();
+    }
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------------------------------
@@ -447,6 +503,8 @@ void k_attn_backward(Args P, BackArgs B) {
     const size_t own = W::wave_bytes(P.heads) + (size_t)kBatch * P.heads * 4 + (size_t)((BH + 1) & ~1) * 4;
     W w(P, lds, (own + 15) & ~(size_t)15);
     const int lane = w.lane, H = w.H, HD = w.HD, HK = w.HK, qv = w.qv, subs = qv * PARTS, per_head = P.d / SUB;
+    float2* share = (float2*)w.keep;                    // [16][H] probability and dropout factor
+    float* weight = (float*)w.t;                        // [16][H] their product
     float* dt = (float*)(w.e_bucket + kBatch);          // [16][H]
     float* bins = dt + kBatch * H;                      // [buckets][H]
     for (int i = lane; i < BH; i += 64) bins[i] = 0.0f;
@@ -492,14 +550,14 @@ void k_attn_backward(Args P, BackArgs B) {
                     const int at = w.e_dst[g + (int)((min(lane, pairs - 1) * w.inv_h) >> 16)] * H + min(lane, pairs - 1) % H;
                     norm0 = *(const d2*)(B.norm + 2 * (int64_t)at);
                 }
-                w.logits(a, g);
-                wave_sync();
-                for (int idx = lane; idx < pairs; idx += 64) {          // t becomes p
+                w.partial_logits(a, g);
+                for (int idx = lane; idx < pairs; idx += 64) {
                     const int e = (int)((idx * w.inv_h) >> 16), h = idx - e * H, eb = g + e;
-                    const double x = w.t[eb * H + h];
+                    const double x = w.logit(g, e, h);
                     const d2 at = idx == lane ? norm0 : *(const d2*)(B.norm + 2 * ((int64_t)w.e_dst[eb] * H + h));
-                    w.t[eb * H + h] = x == -__builtin_inf() ? 0.0 : (double)(exp_d(x - at[0]) * (float)at[1]);
-                    w.keep[eb * H + h] = w.dropped(base + eb, h);
+                    const float p = x == -__builtin_inf() ? 0.0f : exp_d(x - at[0]) * (float)at[1], k = p == 0.0f ? 0.0f : w.dropped(base + eb, h);
+                    share[eb * H + h] = float2{p, k};
+                    weight[eb * H + h] = p * k;
                 }
                 wave_sync();
 #pragma unroll 1
@@ -514,15 +572,13 @@ void k_attn_backward(Args P, BackArgs B) {
                                 float dot[PARTS];
 #pragma unroll
                                 for (int p = 0; p < PARTS; ++p) {
-                                    const int at = (s + i) * H + head[j][p];
-                                    const float f = (float)w.t[at] * w.keep[at];
+                                    const float f = weight[(s + i) * H + head[j][p]];
                                     dot[p] = 0.0f;
 #pragma unroll
                                     for (int k = 0; k < SUB; ++k) {
                                         const int c = p * SUB + k;
-                                        const float u = (float)up[i][j][c];
-                                        o[c] = f == 0.0f ? 0.0f : f * u;
-                                        dot[p] = fmaf((float)v[i][j][c], u, dot[p]);
+                                        o[c] = f * (float)up[i][j][c];
+                                        dot[p] = fmaf((float)v[i][j][c], (float)up[i][j][c], dot[p]);
                                     }
                                 }
                                 if (q < qv) {
@@ -537,13 +593,28 @@ void k_attn_backward(Args P, BackArgs B) {
                         w.load_row(up[i], (const T*)B.grad + (int64_t)dst * HD);
                     }
                     wave_sync();
-                    const int last = min(s + R, w.n) - g;
-                    for (int idx = lane + (s - g) * H, k = lane; idx < last * H; idx += 64, k += 64) {
-                        const int i = (int)((k * w.inv_h) >> 16), h = k - i * H, eb = s + i;
+                    const int last = min(s + R, w.n) - s;          // edges of this part
+                    auto write_dt = [&](int i, int h, float dot) {
+                        const float2 f = share[(s + i) * H + h];
+                        // (a masked edge's value may be NaN)
+                        dt[(s + i) * H + h] = f.x == 0.0f ? 0.0f : f.x * ((f.y == 0.0f ? 0.0f : f.y * dot) - B.delta[(int64_t)w.e_dst[s + i] * H + h]);
+                    };
+                    if (H == 4) {          // 64 / (4 R) lanes share an edge and head's sum
+                        constexpr int L = 64 / (4 * R);
+                        const int k = lane / L, l = lane & (L - 1), i = k >> 2, h = k & 3;
                         float dot = 0.0f;
-                        for (int c = 0; c < per_head; ++c) dot += w.part[i * subs + h * per_head + c];
-                        const float p = (float)w.t[eb * H + h], kp = w.keep[eb * H + h];
-                        dt[eb * H + h] = p == 0.0f ? 0.0f : p * ((kp == 0.0f ? 0.0f : kp * dot) - B.delta[(int64_t)w.e_dst[eb] * H + h]);
+                        if (i < last) for (int c = l; c < per_head; c += L) dot += w.part[i * subs + h * per_head + c];
+                        dot += ror<0xB1>(dot);
+                        if (L > 2) dot += ror<0x4E>(dot);
+                        if (L > 4) dot += ror<0x141>(dot);
+                        if (i < last && l == 0) write_dt(i, h, dot);
+                    } else {
+                        for (int k = lane; k < last * H; k += 64) {
+                            const int i = (int)((k * w.inv_h) >> 16), h = k - i * H;
+                            float dot = 0.0f;
+                            for (int c = 0; c < per_head; ++c) dot += w.part[i * subs + h * per_head + c];
+                            write_dt(i, h, dot);
+                        }
                     }
                     wave_sync();
                 }

@@ -18,7 +18,7 @@ struct Forward {
         if (p.lds_forward > 65536 && hipFuncSetAttribute((const void*)k_attn_forward<T, SUB, VEC, NV>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds_forward) != hipSuccess) return DEDF_ERR_RUNTIME;
         const int empty_blocks = (p.a.n_dst + 64 * kWaves - 1) / (64 * kWaves);
         hipLaunchKernelGGL((k_attn_forward<T, SUB, VEC, NV>), dim3(p.blocks + empty_blocks), dim3(256), p.lds_forward, st, p.a, (T*)out, out32, norm, records, rng_used);
-        if (p.a.n_waves > 1) hipLaunchKernelGGL((k_attn_merge<T, SUB, VEC, NV>), dim3(p.a.n_waves - 1), dim3(256), 0, st, p.a, (T*)out, out32, norm, (const void*)records);
+        if (p.a.n_waves > 1) hipLaunchKernelGGL((k_attn_merge<T, SUB, VEC, NV>), dim3((p.a.n_waves - 1 + merge_waves<NV>() - 1) / merge_waves<NV>()), dim3(1024 / NV), 0, st, p.a, (T*)out, out32, norm, (const void*)records);
         return hipGetLastError() == hipSuccess ? DEDF_OK : DEDF_ERR_RUNTIME;
     }
 };

@@ -334,7 +334,7 @@ typedef struct dedf_edge_attn {
 int dedf_edge_segments(const int64_t* edge_dst, int64_t n_edges, int n_dst, int32_t* dst, int32_t* rowptr, int32_t* bad, void* stream);
 size_t dedf_edge_attention_scratch_bytes(const dedf_edge_attn* a, int backward);
 /* out (n_dst, heads, d) in `type`; for the backward call, or NULL: out_f the same in float32, norm (n_dst, heads, 2)
- * each row's largest logit and 1 / sum of exp(t - largest), rng_used (2) */
+ * a logit M near each row's largest and 1 / sum of exp(t - M), rng_used (2) */
 int dedf_edge_attention(const dedf_edge_attn* a, void* out, float* out_f, double* norm, int64_t* rng_used, void* scratch, size_t scratch_bytes, void* stream);
 /* a->rng: the forward call's rng_used.  Gradients may be NULL: d_alpha, d_value contiguous in `type`, the others float32. */
 int dedf_edge_attention_backward(const dedf_edge_attn* a, const double* norm, const float* out_f, const void* grad_out, void* d_alpha, void* d_value,
