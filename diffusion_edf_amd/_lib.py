@@ -153,6 +153,29 @@ def load() -> C.CDLL:
     return lib
 
 
+_TORCH_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc", "_dedf_torch.so")
+_ops = None
+
+
+def ops():
+    """The autograd module of the training operators (csrc/dedf_torch.cpp), with libdedf.so's entry points handed over.  Raises if it has not been built."""
+    global _ops
+    if _ops is None:
+        import importlib.machinery
+        import importlib.util
+        import torch  # noqa: F401  (the module needs torch's libraries)
+        if not os.path.exists(_TORCH_PATH):
+            raise RuntimeError(f"{_TORCH_PATH} not found: build it with `python -c 'import __graft_entry__ as g; g.build()'`")
+        loader = importlib.machinery.ExtensionFileLoader("_dedf_torch", _TORCH_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_dedf_torch", loader))
+        loader.exec_module(module)
+        lib = load()
+        module.init([C.cast(f, C.c_void_p).value for f in (lib.dedf_edge_attention, lib.dedf_edge_attention_backward, lib.dedf_edge_attention_scratch_bytes, lib.dedf_norm_gate_residual,
+                                                           lib.dedf_norm_gate_residual_backward, lib.dedf_norm_scratch_bytes, lib.dedf_channel_dropout)])
+        _ops = module
+    return _ops
+
+
 def make_config(cfg: HeadConfig, device: int, max_edges: int = 0) -> DedfConfig:
     if cfg.n_scales > MAX_SCALES:
         raise ValueError(f"{cfg.n_scales} scales: the library takes at most {MAX_SCALES} (dedf_config.radii)")

@@ -29,7 +29,7 @@ constexpr int kWaves = 4;                  // waves per workgroup
 // Waves a SIMD holds, by the registers of each instantiation; a launch has as many waves as are resident at once, each with one range of edges.  More
 // waves than that run in two rounds, of which the second is half empty: 1.97 M edges, float32, backward with 2 048 waves 0.95 ms, with 3 072 1.13 ms.
 constexpr int forward_waves(int nv, int sub, int bytes) { return nv == 1 ? (bytes == 2 && sub > 1 ? 4 : 3) : nv == 2 ? (sub == 4 ? 3 : sub) : (sub == 4 ? 2 : 1); }
-constexpr int kBackwardWaves = 2;
+constexpr int backward_waves(int nv, int bytes) { return bytes == 2 && nv <= 2 ? 3 : 2; }          // (499 979 edges, lmax 3, bfloat16: 0.46 ms with 3, 0.52 with 2)
 constexpr float kActNorm = 1.531320475574866f;
 constexpr double kLog2e = 1.4426950408889634;
 
@@ -494,7 +494,7 @@ struct BackArgs {
     float* param_rows;                      // (workgroups, H K + B H) sums of dw and dT, or null
 };
 
-template <class T, int SUB, bool VEC, int NV> __global__ __launch_bounds__(256, kBackwardWaves)
+template <class T, int SUB, bool VEC, int NV> __global__ __launch_bounds__(256, backward_waves(NV, sizeof(T)))
 void k_attn_backward(Args P, BackArgs B) {
     typedef Wave<T, SUB, VEC, NV> W;
     constexpr int NA = W::NA, PARTS = W::PARTS, GA = W::GA, R = W::R;

@@ -94,7 +94,7 @@ int make_plan(const dedf_edge_attn* x, bool backward, Plan& p, std::initializer_
     for (const void* t : tensors) whole = whole && whole_quads(t, 0, 0, x->type);
     p.sub = !whole ? 0 : x->d % 4 == 0 ? 4 : x->d % 2 == 0 ? 2 : 1;
     p.nv = a.heads * a.k > 64 || a.heads * a.d > 512 ? 4 : a.heads * a.d > 256 ? 2 : 1;
-    const int most = kSimds * (backward ? kBackwardWaves : forward_waves(p.nv, p.sub ? p.sub : 1, (int)element(x->type)));
+    const int most = kSimds * (backward ? backward_waves(p.nv, (int)element(x->type)) : forward_waves(p.nv, p.sub ? p.sub : 1, (int)element(x->type)));
     const int64_t even = (a.n_edges + most - 1) / most;
     a.range = (int)std::max<int64_t>(kBatch, (even + kBatch - 1) / kBatch * kBatch);
     a.n_waves = (int)((a.n_edges + a.range - 1) / a.range);

@@ -144,8 +144,7 @@ def test_c_entries_refuse_before_any_launch(built_lib):
     assert lib.dedf_edge_segments(None, 3, 2, V(16), V(16), V(16), None) == _lib.ERR_INVALID
 
     def norm(**kw):
-        shape = row_shape(LMAX2)
-        base = dict(type=0, n_rows=6, n_blocks=3, groups=1, mul=shape.mul, degree=shape.degree, x=16, y=16, scale=1.0, eps=1e-5)
+        base = dict(type=0, n_rows=6, n_blocks=3, groups=1, mul=(C.c_int * 4)(64, 32, 16, 0), degree=(C.c_int * 4)(0, 1, 2, 0), x=16, y=16, scale=1.0, eps=1e-5)
         a = _lib.DedfNorm()
         for k, v in {**base, **kw}.items():
             setattr(a, k, v)
@@ -164,10 +163,10 @@ def test_c_entries_refuse_before_any_launch(built_lib):
     assert lib.dedf_norm_gate_residual(C.byref(a), V(16), V(16), None, None) == _lib.ERR_INVALID          # z without next_weight
     assert lib.dedf_norm_gate_residual_backward(C.byref(a), None, None, V(16), None, None, None, None, None, None, V(16), 1 << 40, None) == _lib.ERR_INVALID
     assert lib.dedf_norm_gate_residual_backward(C.byref(a), V(16), None, V(16), None, None, None, None, None, None, V(16), 8, None) == _lib.ERR_INVALID
-    sh = row_shape(LMAX2)
-    assert lib.dedf_channel_dropout(0, 6, 3, sh.mul, sh.degree, V(16), 1.0, V(16), V(16), None, None) == _lib.ERR_INVALID
-    assert lib.dedf_channel_dropout(0, 6, 3, sh.mul, sh.degree, V(16), 0.5, None, V(16), None, None) == _lib.ERR_INVALID
-    assert lib.dedf_channel_dropout(9, 6, 3, sh.mul, sh.degree, V(16), 0.5, V(16), V(16), None, None) == _lib.ERR_UNSUPPORTED
+    mul, degree = three(64, 32, 16, 0), three(0, 1, 2, 0)
+    assert lib.dedf_channel_dropout(0, 6, 3, mul, degree, V(16), 1.0, V(16), V(16), None, None) == _lib.ERR_INVALID
+    assert lib.dedf_channel_dropout(0, 6, 3, mul, degree, V(16), 0.5, None, V(16), None, None) == _lib.ERR_INVALID
+    assert lib.dedf_channel_dropout(9, 6, 3, mul, degree, V(16), 0.5, V(16), V(16), None, None) == _lib.ERR_UNSUPPORTED
 
 
 def test_modules_are_the_identity_in_eval_and_carry_the_reference_names():
