@@ -117,14 +117,9 @@ template <class T, int SUB, bool VEC, int NV> struct Wave {
         qa = (HK + 3) >> 2; qv = (HD + 3) >> 2;
         sub_a = (K & 3) ? 1 : 4; n_sub_a = K / sub_a;
         inv_h = (65536 + H - 1) / H; inv_qa = (65536 + qa - 1) / qa;
-        float* s = (float*)lds;
+        float* s = (float*)lds;          // (filled by stage())
         const int hk4 = (HK + 3) & ~3, B = p.n_buckets;
-        for (int i = threadIdx.x; i < hk4; i += blockDim.x) s[i] = i < HK ? p.w[i] : 0.0f;
-        w = s; s += hk4;
-        for (int i = threadIdx.x; i < B - 1; i += blockDim.x) s[i] = p.bounds[i];
-        bounds = s; s += B;
-        for (int i = threadIdx.x; i < B * H; i += blockDim.x) s[i] = p.table[i];
-        table = s;
+        w = s; bounds = s + hk4; table = s + hk4 + B;
         char* mine = lds + shared_bytes(HK, H, B) + wave * own_bytes;
         t = (double*)mine; part = (float*)(mine + (size_t)kBatch * H * 8); keep = part + kPart;
         e_logit = keep + 2 * kBatch * H; e_dst = (int*)(e_logit + kBatch); e_bucket = e_dst + kBatch;
@@ -132,6 +127,14 @@ template <class T, int SUB, bool VEC, int NV> struct Wave {
         if (p.threshold) { seed = (uint64_t)p.rng[0]; offset = (uint64_t)p.rng[1]; }
         const int64_t id = (int64_t)blockIdx.x * kWaves + wave;
         e0 = min(id * p.range, p.n_edges); e1 = min(e0 + p.range, p.n_edges);
+    }
+    // the call's parameters into LDS: for every wave of the workgroup, behind its first loads of edges
+    __device__ void stage(char* lds) const {
+        float* s = (float*)lds;
+        const int hk4 = (HK + 3) & ~3, B = P.n_buckets;
+        for (int i = threadIdx.x; i < hk4; i += blockDim.x) s[i] = i < HK ? P.w[i] : 0.0f;
+        for (int i = threadIdx.x; i < B - 1; i += blockDim.x) s[hk4 + i] = P.bounds[i];
+        for (int i = threadIdx.x; i < B * H; i += blockDim.x) s[hk4 + B + i] = P.table[i];
         __syncthreads();
     }
     // per-edge values of the batch at b: requested early (into registers of the first 16 lanes), put into LDS when the batch begins
@@ -276,17 +279,26 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
         return;
     }
     W w(P, lds, W::wave_bytes(P.heads) + (size_t)kBatch * P.heads * 8);
-    if (w.e0 >= w.e1) return;
+    if (w.e0 >= w.e1) { w.stage(lds); return; }
     const int lane = w.lane, H = w.H, HD = w.HD, qv = w.qv;
     int head[NV][PARTS];
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) head[j][p] = min((4 * (j * 64 + lane) + p * SUB) / P.d, H - 1);
+    // R value rows are always in flight: a row's registers are loaded again, R edges ahead, as soon as it has been added
+    constexpr int R = W::R;
+    typename W::Edge edge = w.request(w.e0);
+    typename W::Raw a[W::NA], v[R][NV];
+    w.load_a(a, w.e0, (int)min((int64_t)kBatch, w.e1 - w.e0), 0);
+#pragma unroll
+    for (int i = 0; i < R; ++i) w.load_row(v[i], w.value_row(w.e0 + i));
+    const int before = P.dst[max(w.e0 - 1, (int64_t)0)], behind = P.dst[min(w.e1, P.n_edges - 1)];
+    w.stage(lds);
     Row<NV, PARTS> r;
     r.clear();
-    int cur = __builtin_amdgcn_readfirstlane(P.dst[w.e0]);
-    const bool open_front = w.e0 > 0 && P.dst[w.e0 - 1] == cur;
+    int cur = __builtin_amdgcn_readfirstlane(edge.dst);
+    const bool open_front = w.e0 > 0 && before == cur;
     bool first_row = true;
     Record<NV, PARTS>* rec = (Record<NV, PARTS>*)records + ((int64_t)blockIdx.x * kWaves + w.wave) * 2 * 64 + lane;
     auto flush = [&](bool open_back) {
@@ -298,13 +310,6 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
     };
     float2* share = (float2*)w.keep;                       // [16][H] share of the piece, and that share times the dropout factor
     double* top = (double*)(w.e_bucket + kBatch);          // [16][H] logit that the shares are relative to
-    typename W::Edge edge = w.request(w.e0);
-    // R value rows are always in flight: a row's registers are loaded again, R edges ahead, as soon as it has been added
-    constexpr int R = W::R;
-    typename W::Raw a[W::NA], v[R][NV];
-    w.load_a(a, w.e0, (int)min((int64_t)kBatch, w.e1 - w.e0), 0);
-#pragma unroll
-    for (int i = 0; i < R; ++i) w.load_row(v[i], w.value_row(w.e0 + i));
     for (int64_t base = w.e0; base < w.e1; base += kBatch) {
         w.begin(base, edge);
         edge = w.request(min(base + kBatch, w.e1 - 1));
@@ -403,7 +408,7 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
             wave_sync();
         }
     }
-    flush(w.e1 < P.n_edges && P.dst[w.e1] == cur);
+    flush(w.e1 < P.n_edges && behind == cur);
 }
 
 // Rows that cross ranges.  A wave looks at one border between two ranges and takes a row whose first crossing that is: it joins up to 8 records by itself;
@@ -523,7 +528,8 @@ void k_attn_backward(Args P, BackArgs B) {
         head_a[i] = min(4 * q / P.k, H - 1);
     }
 
-    if (w.e0 < w.e1) {
+    if (w.e0 >= w.e1) w.stage(lds);
+    else {
         // value rows and the upper gradient at their destinations, R edges ahead; a batch's per-edge values and features one batch ahead
         typename W::Edge edge = w.request(w.e0), next = edge;
         typename W::Raw a[NA], a_next[NA], v[R][NV], up[R][NV];
@@ -533,6 +539,7 @@ void k_attn_backward(Args P, BackArgs B) {
             w.load_row(v[i], w.value_row(w.e0 + i));
             w.load_row(up[i], (const T*)B.grad + (int64_t)__builtin_amdgcn_readlane(edge.dst, i) * HD);
         }
+        w.stage(lds);
         for (int64_t base = w.e0; base < w.e1; base += kBatch) {
             w.begin(base, edge);
             next = w.request(min(base + kBatch, w.e1 - 1));
