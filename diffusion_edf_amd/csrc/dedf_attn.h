@@ -28,7 +28,7 @@ constexpr int kBatch = 16;                 // edges per step of a wave
 constexpr int kWaves = 4;                  // waves per workgroup
 // Waves a SIMD holds, by the registers of each instantiation; a launch has as many waves as are resident at once, each with one range of edges.  More
 // waves than that run in two rounds, of which the second is half empty: 1.97 M edges, float32, backward with 2 048 waves 0.95 ms, with 3 072 1.13 ms.
-constexpr int forward_waves(int nv, int sub, int bytes) { return nv == 1 ? (bytes == 2 && sub > 1 ? 4 : 3) : nv == 2 ? (sub == 4 ? 3 : sub) : (sub == 4 ? 2 : 1); }
+constexpr int forward_waves(int nv, int sub, int bytes) { return nv == 1 ? (bytes == 2 && sub > 1 ? 4 : 3) : nv == 2 ? (sub == 4 ? 3 : bytes == 2 ? sub + 1 : sub) : (sub == 4 ? 2 : 1); }
 constexpr int backward_waves(int nv, int bytes) { return bytes == 2 && nv <= 2 ? 3 : 2; }          // (499 979 edges, lmax 3, bfloat16: 0.46 ms with 3, 0.52 with 2)
 constexpr float kActNorm = 1.531320475574866f;
 constexpr double kLog2e = 1.4426950408889634;
@@ -95,7 +95,7 @@ __device__ inline int bucket_of(const float* bounds, int n, float x) {
 //   NV: quads of a value row a lane holds: 1 (up to 256 channels) or 2 (512), with feature rows of up to 64, or 4 (1 024) with feature rows of up to 256
 template <class T, int SUB, bool VEC, int NV> struct Wave {
     static constexpr int NA = 4, GA = NV == 4 ? 4 : 16;                      // GA edges x feature quads fill NA loads of a wave
-    static constexpr int R = 8 / NV;                                         // value rows in flight
+    static constexpr int R = 8 / NV, RF = NV == 1 ? 8 : (sizeof(T) == 2 ? 16 : 8) / NV;    // value rows in flight: backward, forward
     static constexpr int PARTS = 4 / SUB;
     static constexpr int kPart = SUB == 1 ? 2048 : 1024;                     // floats of the partial-sum buffer
     const Args& P;
@@ -287,7 +287,7 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) head[j][p] = min((4 * (j * 64 + lane) + p * SUB) / P.d, H - 1);
     // R value rows are always in flight: a row's registers are loaded again, R edges ahead, as soon as it has been added
-    constexpr int R = W::R;
+    constexpr int R = W::RF;
     typename W::Edge edge = w.request(w.e0);
     typename W::Raw a[W::NA], v[R][NV];
     w.load_a(a, w.e0, (int)min((int64_t)kBatch, w.e1 - w.e0), 0);
