@@ -318,8 +318,8 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
             // the next features are on their way while this group is summed up
             if (g + GA < kBatch && g + GA < w.n) w.load_a(a, base, w.n, g + GA);
             else if (base + kBatch < w.e1) w.load_a(a, base + kBatch, (int)min((int64_t)kBatch, w.e1 - base - kBatch), 0);
-            // A "piece" is what one row has in this group.  Shares are relative to a logit that every lane of a head agrees on; any within e^60 of the piece's
-            // own largest keeps full precision.
+            // A "piece" is what one row has in this group.  Shares are relative to a logit that every lane of a head agrees on: the group's largest, if it is
+            // at most 24 above the smallest (shares of 4e-11 and more keep full precision for any values above 1e-27), else the piece's own largest.
             const uint32_t starts = (w.starts >> g) | 1u;
             const int live = min(GA, w.n - g);
             bool near = false;
@@ -335,7 +335,7 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
                 most = fmaxf(most, ror<0x128>(most)); least = fminf(least, ror<0x128>(least));
                 most = fmaxf(most, __shfl_xor(most, 16)); least = fminf(least, __shfl_xor(least, 16));
                 most = fmaxf(most, __shfl_xor(most, 32)); least = fminf(least, __shfl_xor(least, 32));
-                near = __ballot(most != -__builtin_inff() && !(most - least <= 60.0f && fabsf(most) <= 1e6f)) == 0;
+                near = __ballot(most != -__builtin_inff() && !(most - least <= 24.0f && fabsf(most) <= 1e6f)) == 0;
                 if (near) {
                     const float p = in ? exp_d(x - (double)most) : 0.0f;
                     share[(g + e) * 4 + h] = float2{p, in ? p * w.dropped(base + g + e, h) : 0.0f};
@@ -554,8 +554,8 @@ void k_attn_backward(Args P, BackArgs B) {
                 // the first 64 of the group's edges and heads (all of them for up to 4 heads): what their rows keep, on its way early
                 d2 norm0 = {0.0, 0.0};
                 {
-                    const int at = w.e_dst[g + (int)((min(lane, pairs - 1) * w.inv_h) >> 16)] * H + min(lane, pairs - 1) % H;
-                    norm0 = *(const d2*)(B.norm + 2 * (int64_t)at);
+                    const int k = min(lane, pairs - 1), e = (int)((k * w.inv_h) >> 16);
+                    norm0 = *(const d2*)(B.norm + 2 * ((int64_t)w.e_dst[g + e] * H + k - e * H));
                 }
                 w.partial_logits(a, g);
                 for (int idx = lane; idx < pairs; idx += 64) {

@@ -263,7 +263,7 @@ def _check(c, dtype=None):
     (1, 1, {}), (3, 2, {}), (40, 333, dict(buckets=8)), (7, 500, dict(drop=0.3, buckets=3)), (200, 201, dict(logits=False)), (1, 700, dict(drop=0.1)),
     (50, 400, dict(D=40)), (50, 400, dict(D=74, drop=0.2)), (9, 130, dict(H=1, K=1, D=1)), (9, 130, dict(H=3, K=5, D=7, buckets=2)), (9, 130, dict(H=2, K=3, D=6)),
     (9, 130, dict(H=8, K=31, D=51, drop=0.35)), (5, 90, dict(H=16, K=16, D=64, drop=0.5, buckets=1)), (5, 90, dict(H=4, K=64, D=256, buckets=16)), (4, 60, dict(H=1, K=2, D=1023)),
-    (4, 60, dict(H=3, K=21, D=85)), (4, 60, dict(H=1, K=256, D=2)), (6, 300, dict(buckets=512)),
+    (4, 60, dict(H=3, K=21, D=85)), (4, 60, dict(H=1, K=256, D=2)), (6, 300, dict(buckets=512)), (6, 300, dict(H=16, K=16, D=64, buckets=128)), (70, 1_000, dict(D=20, K=5)),
 ])
 def test_edge_attention(dtype, N, E, kw):
     _check(_case(dtype, N, E, **kw))
@@ -524,6 +524,34 @@ def test_norm_gate_residual(dtype, irreps):
 ])
 def test_norm_gate_residual_forms(R, kw, use):
     _norm_check(_norm_case(torch.float32, LMAX2, R, **kw), use)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,groups", [(30, 1), (30, 30), (30, 5), (9_000, 2), (9_000, 90)])
+def test_norm_gate_types(dtype, R, groups):
+    """a gate in the features' type and in float32, of one row, of groups cut into many and into few slices, one a node; small rows keep the oracle quick"""
+    for gate_type in (dtype, torch.float32):
+        c = _norm_case(dtype, "5x0e+3x1e+1x2e", R, groups=groups, drop=0.0, seed=groups)
+        c["gate"] = c["gate"].to(gate_type)
+        h, z, grads = _norm_gpu(c)
+        _, _, ref = _norm_reference(c)
+        assert grads["gate"].dtype == gate_type
+        # a sum of n = 5 R / groups products of values of a few units: float32 chains of at most 64 terms, 64 bits after, as in the test of many rows below
+        want = ref["gate"]
+        close(grads["gate"], want, 64 * 16 * U * float(want.abs().max()), "d_gate")
+
+
+@pytest.mark.gpu
+def test_edge_attention_far_logits_side_by_side():
+    """rows whose logits lie 100 and 10 000 apart next to each other, and float32 values of 1e-20: every row keeps its own precision"""
+    for gap in (20.0, 30.0, 100.0, 1e4):
+        c = _case(torch.float32, 40, 400, seed=int(gap))
+        c["logits"] = c["logits"] - gap * (c["dst"] % 3).float()
+        _check(c)
+        c["value"] *= 1e-20
+        c["grad"] *= 1e20
+        _check(c)
 
 
 @pytest.mark.gpu
