@@ -27,7 +27,8 @@ namespace attn {
 constexpr int kBatch = 16;                 // edges per step of a wave
 constexpr int kWaves = 4;                  // waves per workgroup
 // Waves a SIMD holds, by the registers of each instantiation; a launch has as many waves as are resident at once, each with one range of edges.  More
-// waves than that run in two rounds, of which the second is half empty: 1.97 M edges, float32, backward with 2 048 waves 0.95 ms, with 3 072 1.13 ms.
+// waves than that run in two rounds, of which the second is half empty: 1.97 M edges, float32, a training pass with 2 048 waves
+// in the backward kernel 1.65 ms, with 3 072 1.83 ms.
 constexpr int forward_waves(int nv, int sub, int bytes) { return nv == 1 ? (bytes == 2 && sub > 1 ? 4 : 3) : nv == 2 ? (sub == 4 ? 3 : bytes == 2 ? sub + 1 : sub) : (sub == 4 ? 2 : 1); }
 constexpr int backward_waves(int nv, int bytes) { return bytes == 2 && nv <= 2 ? 3 : 2; }          // (499 979 edges, lmax 3, bfloat16: 0.46 ms with 3, 0.52 with 2)
 constexpr float kActNorm = 1.531320475574866f;
@@ -258,6 +259,11 @@ finish_row(const Args& P, int row, const Row<NV, 4 / SUB>& r, int lane, int qv, 
     }
 }
 
+// Read of the per-edge rows once; bandwidth bounds it, in 16 bits nearly as much the 46 vector instructions of an edge.  1.97 M edges of 64 + 240 channels:
+// float32 0.57 ms (4.4 TB/s), float16 0.30 ms (4.2 TB/s), where a large copy reaches 4.8.  A logit's 16 products are summed per quad by the lanes that
+// loaded it and finished by one lane for each edge and head, which also draws the dropout word: the walk then needs one share per edge and lane.  (Running
+// maxima per edge and lane instead: 0.69 ms in float16.)  At lmax 3 (296 channels, 74 quads) a lane holds two quads, the second one mostly idle: 0.13 ms for
+// 499 979 edges, 2.7 TB/s, bound by instructions and by what 8 waves of a CU have in flight.
 template <class T, int SUB, bool VEC, int NV> __global__ __launch_bounds__(256, forward_waves(NV, SUB, sizeof(T)))
 void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, int64_t* rng_used) {
     typedef Wave<T, SUB, VEC, NV> W;
@@ -411,7 +417,7 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
     flush(w.e1 < P.n_edges && behind == cur);
 }
 
-// Rows that cross ranges.  A wave looks at one border between two ranges and takes a row whose first crossing that is: it joins up to 8 records by itself;
+// Rows that cross ranges.  Few bytes, all waiting: 3 000 ranges 7.5 us, 7 rows of 536 records each 29 us.  A wave looks at one border between two ranges and takes a row whose first crossing that is: it joins up to 8 records by itself;
 // a longer row is joined by the whole workgroup, every wave a share of the records, then the waves' results in order.
 template <int NV> constexpr int merge_waves() { return 16 / NV; }
 template <class T, int SUB, bool VEC, int NV> __global__ __launch_bounds__(1024 / NV)
@@ -477,7 +483,7 @@ void k_attn_merge(Args P, T* out, float* out32, double* norm, const void* record
 
 // ---- backward -------------------------------------------------------------------------------------------------------------------------------
 
-// delta[n,h] = sum_c dout out32: a wave per row
+// delta[n,h] = sum_c dout out32: a wave per row, two reads of (rows, H D); 103 000 rows of 240 float32 57 us, 3.5 TB/s
 template <class T> __global__ __launch_bounds__(256)
 void k_attn_delta(int64_t n_rows, int H, int D, const T* grad, const float* out32, float* delta) {
     const int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
@@ -499,6 +505,10 @@ struct BackArgs {
     float* param_rows;                      // (workgroups, H K + B H) sums of dw and dT, or null
 };
 
+// Reads the per-edge rows once and writes their gradients; the rows of dout come from the caches, read again for each edge rather than kept while a row
+// lasts, so nothing waits where rows are short.  1.97 M edges of 64 + 240 float32 channels: 1.02 ms, 4.8 TB/s, the rate of a large copy; 499 979 bfloat16 edges
+// of lmax 3 0.25 ms, 2.9 TB/s, bound by the latency that three waves a SIMD cover.  The dot of a value row with dout goes through LDS (a partial sum for each
+// quad part), since a head's quads are not a power of two of lanes.
 template <class T, int SUB, bool VEC, int NV> __global__ __launch_bounds__(256, backward_waves(NV, sizeof(T)))
 void k_attn_backward(Args P, BackArgs B) {
     typedef Wave<T, SUB, VEC, NV> W;
