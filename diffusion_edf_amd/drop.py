@@ -3,7 +3,9 @@
 No mask is ever stored.  An operator keeps an element where its Philox4x32-10 word -- key: the seed, counter: the element's place and the offset -- is at
 least ``floor(p * 2**32)``, and its backward pass draws the same words again (``include/dedf.h`` lists the counters).  ``rng = [seed, offset]`` is an int64
 tensor on the device: the kernels read it there, so a captured graph draws a new mask in each replay if the program changes the offset in between.  Two
-calls with one ``rng`` draw the same words: give each call of a step an offset of its own (``EquivariantDropout`` and ``EdgeAttention`` count theirs)."""
+calls with one ``rng`` draw the same words: give each call of a step an offset of its own (``EquivariantDropout``, ``EdgeAttention`` and ``NormGateResidual`` count theirs, from a seed that their state dicts do
+not hold; where a forward pass is run again for its activations, as in checkpointing, call the functions with an ``rng`` of your own, which such a run
+repeats)."""
 from __future__ import annotations
 
 import functools

@@ -63,7 +63,8 @@ def edge_attention(alpha: torch.Tensor, value: torch.Tensor, alpha_dot: torch.Te
 
 class EdgeAttention(torch.nn.Module):
     """``edge_attention`` with its parameters: ``alpha_dot`` ``(1, H, K)`` as in the reference's state dict (``graph_attention.py:139-214``) and, with
-    ``bias_boundaries``, ``bias_table`` (zero at the start).  Dropout in training only; ``rng`` holds the seed and counts the training calls."""
+    ``bias_boundaries``, ``bias_table`` (zero at the start); after ``half()`` they are used in float32 all the same.  Dropout in training only; ``rng`` holds the
+    seed and counts the training calls."""
 
     def __init__(self, num_heads: int, mul_alpha_head: int, alpha_drop: float = 0.0, bias_boundaries: Optional[Sequence[float]] = None, seed: int = 0):
         super().__init__()
@@ -77,8 +78,8 @@ class EdgeAttention(torch.nn.Module):
     def forward(self, alpha: torch.Tensor, value: torch.Tensor, segments: EdgeSegments, edge_logits: Optional[torch.Tensor] = None,
                 edge_length: Optional[torch.Tensor] = None) -> torch.Tensor:
         p = self.alpha_drop if self.training else 0.0
-        bias = {} if self.bias_table is None else {"edge_length": edge_length, "bias_boundaries": self.bias_boundaries, "bias_table": self.bias_table}
-        out = edge_attention(alpha, value, self.alpha_dot, segments, edge_logits, dropout=p, rng=self.rng, **bias)
+        bias = {} if self.bias_table is None else {"edge_length": edge_length, "bias_boundaries": self.bias_boundaries.float(), "bias_table": self.bias_table.float()}
+        out = edge_attention(alpha, value, self.alpha_dot.float(), segments, edge_logits, dropout=p, rng=self.rng, **bias)
         if p > 0.0:
             self.rng[1] += 1
         return out

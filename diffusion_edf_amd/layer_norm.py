@@ -42,7 +42,7 @@ class EquivariantLayerNormV2(torch.nn.Module):
         self.affine_bias = torch.nn.Parameter(torch.zeros(shape.scalars))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return equivariant_layer_norm(x, self.irreps, self.affine_weight, self.affine_bias if len(self.affine_bias) else None, self.eps)
+        return equivariant_layer_norm(x, self.irreps, self.affine_weight.float(), self.affine_bias.float(), self.eps)          # (float32 after half() too)
 
 
 class NormGateResidual(torch.nn.Module):
@@ -58,7 +58,7 @@ class NormGateResidual(torch.nn.Module):
 
     def forward(self, x: torch.Tensor, y: torch.Tensor, gate: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
         p = self.drop_prob if self.training else 0.0
-        affine = [None if n is None else t for n in (self.post_norm, self.next_norm) for t in ((None, None) if n is None else (n.affine_weight, n.affine_bias))]
+        affine = [None if n is None else t for n in (self.post_norm, self.next_norm) for t in ((None, None) if n is None else (n.affine_weight.float(), n.affine_bias.float()))]
         out = norm_gate_residual(x, y, self.irreps, self.scale, gate, affine[0], affine[1], p, self.rng, affine[2], affine[3], self.eps)
         if p > 0.0:
             self.rng[1] += 1

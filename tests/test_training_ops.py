@@ -778,6 +778,60 @@ def test_a_captured_training_step_draws_anew_and_matches_the_eager_one():
 
 
 @pytest.mark.gpu
+def test_a_captured_backward_accumulates_into_parameters():
+    """loss.backward() inside a capture, as training loops capture a step: the parameters' gradients after each replay are the eager ones (same masks; torch's own
+    index_add in between sums in no fixed order, as above)"""
+    torch.manual_seed(2)
+    block = _Block().cuda()
+    x, src, dst, logits, length = _block_inputs()
+    seg, x = EdgeSegments(dst, 150), x.cuda()
+    rngs = [block.attention.rng, block.drop.rng, block.residual.rng]
+
+    def step():
+        for p in block.parameters():
+            p.grad = None
+        h, z = block(x, src, seg, logits, length)
+        (h.square().sum() + (h * z).sum()).backward()
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    static = [p.grad for p in block.parameters()]
+    for i in range(3):
+        for r in rngs:
+            r[1] = 5 + i
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [g.clone() for g in static]
+        eager = _Block().cuda()
+        eager.load_state_dict(block.state_dict())
+        for r in (eager.attention.rng, eager.drop.rng, eager.residual.rng):
+            r[1] = 5 + i
+        h, z = eager(x, src, seg, logits, length)
+        (h.square().sum() + (h * z).sum()).backward()
+        for a, p in zip(got, eager.parameters()):
+            assert float((a - p.grad).abs().max()) <= 1e-4 * float(p.grad.abs().max()), i
+
+
+@pytest.mark.gpu
+def test_modules_in_half_precision():
+    """half() casts the parameters; the operators use them in float32 and return gradients in their type"""
+    block = _Block().cuda().half()
+    x, src, dst, logits, length = _block_inputs()
+    h, z = block(x.cuda().half(), src, EdgeSegments(dst, 150), logits, length)
+    assert h.dtype == z.dtype == torch.float16
+    (h.float().square().sum() + z.float().sum()).backward()
+    assert all(p.grad is not None and p.grad.dtype == torch.float16 and bool(p.grad.isfinite().all()) for p in block.parameters())
+
+
+@pytest.mark.gpu
 def test_two_captured_graphs_share_nothing():
     """two graphs of the operators alone, replayed in turn and out of order, against their eager results bit for bit: no workspace between them"""
     cases = [_case(torch.float32, 60, 900, buckets=4, drop=0.2, seed=s) for s in (1, 2)]
