@@ -26,11 +26,15 @@ namespace attn {
 
 constexpr int kBatch = 16;                 // edges per step of a wave
 constexpr int kWaves = 4;                  // waves per workgroup
+enum { kAny = 0, kHeads = 1, kAligned = 2 };          // how a row is cut into quads: see load_quad
 // Waves a SIMD holds, by the registers of each instantiation; a launch has as many waves as are resident at once, each with one range of edges.  More
 // waves than that run in two rounds, of which the second is half empty: 1.97 M edges, float32, a training pass with 2 048 waves
 // in the backward kernel 1.65 ms, with 3 072 1.83 ms.
-constexpr int forward_waves(int nv, int sub, int bytes) { return nv == 1 ? (bytes == 2 && sub > 1 ? 4 : 3) : nv == 2 ? (sub == 4 ? 3 : bytes == 2 ? sub + 1 : sub) : (sub == 4 ? 2 : 1); }
-constexpr int backward_waves(int nv, int bytes) { return bytes == 2 && nv <= 2 ? 3 : 2; }          // (499 979 edges, lmax 3, bfloat16: 0.46 ms with 3, 0.52 with 2)
+constexpr int forward_waves(int mode, int nv, int bytes) {
+    if (mode == kAny) return nv == 1 ? 3 : nv == 2 && bytes == 2 ? 2 : 1;
+    return nv == 4 ? 2 : nv == 1 && bytes == 2 ? 4 : 3;
+}
+constexpr int backward_waves(int mode, int nv, int bytes) { return bytes == 2 && nv <= 2 && mode != kAny ? 3 : 2; }          // (499 979 edges, lmax 3, bfloat16: 0.46 ms with 3, 0.52 with 2; parts by elements, which spill: 2)
 constexpr float kActNorm = 1.531320475574866f;
 constexpr double kLog2e = 1.4426950408889634;
 
@@ -56,19 +60,43 @@ struct Args {
     int range, n_waves;                    // edges per wave, waves
 };
 
-// quad of a row, as stored: one access where rows consist of whole, aligned quads (VEC), else its `left` elements
-template <class T, bool VEC> __device__ inline typename Quad<T>::type load_quad(const T* p, int left) {
-    if constexpr (VEC) return *(const typename Quad<T>::type*)p;
+// How a row is cut into quads (MODE):
+//   kAligned  head widths are multiples of 4 and every row begins at a whole quad: quads lie one behind the other, an aligned access each
+//   kHeads    any other head width from 4: each head has quads of its own, the last of which ends with the head and so begins inside the one before; an
+//             unaligned access each.  Elements that two quads hold are summed by the first of them.
+//   kAny      what has more quads than a wave holds that way, or narrower heads: quads one behind the other across the heads, by elements
+// 400 000 edges of 3 heads of 17 + 33 channels, a training pass: float32 0.24 ms (by elements 0.42), bfloat16 0.20 ms (0.64); 4 aligned heads of 16 + 60
+// 0.36 ms in float32, of 16 + 61 0.38 ms.
+template <class T, int MODE> __device__ inline typename Quad<T>::type load_quad(const T* p, int left) {
     typename Quad<T>::type r = {(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f};
+    if constexpr (MODE == kAligned) r = *(const typename Quad<T>::type*)p;
+    else if constexpr (MODE == kHeads) __builtin_memcpy(&r, p, sizeof(r));
+    else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) if (i < left) r[i] = p[i];
+        for (int i = 0; i < 4; ++i) if (i < left) r[i] = p[i];
+    }
     return r;
 }
-template <class T, bool VEC> __device__ inline void store_quad(T* p, f4 x, int left) {
-    if constexpr (VEC) { *(typename Quad<T>::type*)p = typename Quad<T>::type{(T)x[0], (T)x[1], (T)x[2], (T)x[3]}; return; }
+template <class T, int MODE> __device__ inline void store_quad(T* p, f4 x, int left) {
+    const typename Quad<T>::type r = {(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
+    if constexpr (MODE == kAligned) *(typename Quad<T>::type*)p = r;
+    else if constexpr (MODE == kHeads) __builtin_memcpy(p, &r, sizeof(r));
+    else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) if (i < left) p[i] = (T)x[i];
+        for (int i = 0; i < 4; ++i) if (i < left) p[i] = r[i];
+    }
 }
+// quads of a row of H heads of `width` elements, as the kernels and their launches see it
+__host__ __device__ constexpr int row_quads(int mode, int H, int width) { return mode == kAny ? (H * width + 3) >> 2 : H * ((width + 3) >> 2); }
+// first element of quad q and the head that it lies in (kAny: that its first element lies in)
+template <int MODE> __device__ inline int quad_start(int q, int H, int width, int& head) {
+    if constexpr (MODE == kAny) { head = min(4 * q / width, H - 1); return 4 * q; }
+    const int n = (width + 3) >> 2;
+    head = min(q / n, H - 1);
+    return head * width + min(4 * (q - head * n), width - 4);
+}
+// elements of it that the quad before holds too
+template <int MODE> __device__ inline int quad_shared(int start, int head, int width) { return MODE == kHeads ? -(start - head * width) & 3 : 0; }
 
 // LDS of one wave is written and read by its own lanes only: LDS operations of a wave complete in order, the compiler must keep that order
 __device__ inline void wave_sync() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
@@ -91,17 +119,19 @@ __device__ inline int bucket_of(const float* bounds, int n, float x) {
 }
 
 // what both directions share: the wave's place, its LDS, the batch's per-edge values, the logits
-//   SUB: a quad is cut into 4 / SUB parts that each lie inside one head (4: head widths divisible by 4; 2: even; 1: any)
-//   VEC: rows consist of whole, aligned quads
-//   NV: quads of a value row a lane holds: 1 (up to 256 channels) or 2 (512), with feature rows of up to 64, or 4 (1 024) with feature rows of up to 256
-template <class T, int SUB, bool VEC, int NV> struct Wave {
-    static constexpr int NA = 4, GA = NV == 4 ? 4 : 16;                      // GA edges x feature quads fill NA loads of a wave
-    static constexpr int R = 8 / NV, RF = NV == 1 ? 8 : (sizeof(T) == 2 ? 16 : 8) / NV;    // value rows in flight: backward, forward
-    static constexpr int PARTS = 4 / SUB;
-    static constexpr int kPart = SUB == 1 ? 2048 : 1024;                     // floats of the partial-sum buffer
+//   MODE: see load_quad; a quad is cut into PARTS parts of SUB elements that each lie inside one head
+//   NV: quads of a value row a lane holds: 1, 2 or 4 (up to 64, 128, 256 quads)
+//   GA: edges whose features are loaded at once: 16 (feature rows of up to 16 quads), 8 (32) or 4 (64)
+template <class T, int MODE, int NV, int GA> struct Wave {
+    static constexpr int NA = 4;                                             // GA edges x feature quads fill NA loads of a wave
+    static constexpr int rows(int quads) { return quads / NV < GA ? quads / NV : GA; }
+    static constexpr int R = rows(8), RF = rows(NV > 1 && sizeof(T) == 2 ? 16 : 8);        // value rows in flight: backward, forward
+    static constexpr int SUB = MODE == kAny ? 1 : 4, PARTS = 4 / SUB;
+    static constexpr int kPart = MODE == kAny ? 2048 : 1024;       // floats of the partial-sum buffer
     const Args& P;
     int lane, wave, H, K, D, HK, HD, qa, qv, sub_a, n_sub_a;
-    uint32_t inv_h, inv_qa;
+    int begin_v[NV], head_v[NV];                                             // of the lane's value quads (the last one where it has none): first element, its head
+    uint32_t inv_h, inv_qa, inv_head;
     int64_t e0, e1;
     float* part; double* t; float* keep; const float* w; const float* bounds; const float* table;
     uint64_t seed, offset;
@@ -110,18 +140,20 @@ template <class T, int SUB, bool VEC, int NV> struct Wave {
     int* e_dst; int* e_bucket; float* e_logit;                               // its edges' destination, length bucket, edge logit
 
     static __host__ __device__ size_t wave_bytes(int H) { return (size_t)kPart * 4 + (size_t)kBatch * (H * 16 + 12); }
-    static __host__ __device__ size_t shared_bytes(int HK, int H, int B) { return (((size_t)((HK + 3) & ~3) + (B ? B + (size_t)B * H : 0)) * 4 + 15) & ~(size_t)15; }
+    static __host__ __device__ size_t shared_bytes(int qa, int H, int B) { return ((4 * (size_t)qa + (B ? B + (size_t)B * H : 0)) * 4 + 15) & ~(size_t)15; }
 
     __device__ Wave(const Args& p, char* lds, size_t own_bytes) : P(p) {
         lane = threadIdx.x & 63; wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);          // (known to be uniform: row addresses stay scalar)
         H = p.heads; K = p.k; D = p.d; HK = H * K; HD = H * D;
-        qa = (HK + 3) >> 2; qv = (HD + 3) >> 2;
-        sub_a = (K & 3) ? 1 : 4; n_sub_a = K / sub_a;
-        inv_h = (65536 + H - 1) / H; inv_qa = (65536 + qa - 1) / qa;
+        qa = row_quads(MODE, H, K); qv = row_quads(MODE, H, D);
+        sub_a = MODE == kAny && (K & 3) ? 1 : 4; n_sub_a = sub_a == 1 ? K : (K + 3) >> 2;
+        inv_h = (65536 + H - 1) / H; inv_qa = (65536 + qa - 1) / qa; inv_head = (65536 + n_sub_a - 1) / n_sub_a;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) begin_v[j] = quad_start<MODE>(min(j * 64 + lane, qv - 1), H, D, head_v[j]);
         float* s = (float*)lds;          // (filled by stage())
-        const int hk4 = (HK + 3) & ~3, B = p.n_buckets;
+        const int hk4 = 4 * qa, B = p.n_buckets;
         w = s; bounds = s + hk4; table = s + hk4 + B;
-        char* mine = lds + shared_bytes(HK, H, B) + wave * own_bytes;
+        char* mine = lds + shared_bytes(qa, H, B) + wave * own_bytes;
         t = (double*)mine; part = (float*)(mine + (size_t)kBatch * H * 8); keep = part + kPart;
         e_logit = keep + 2 * kBatch * H; e_dst = (int*)(e_logit + kBatch); e_bucket = e_dst + kBatch;
         seed = offset = 0;
@@ -132,8 +164,8 @@ template <class T, int SUB, bool VEC, int NV> struct Wave {
     // the call's parameters into LDS: for every wave of the workgroup, behind its first loads of edges
     __device__ void stage(char* lds) const {
         float* s = (float*)lds;
-        const int hk4 = (HK + 3) & ~3, B = P.n_buckets;
-        for (int i = threadIdx.x; i < hk4; i += blockDim.x) s[i] = i < HK ? P.w[i] : 0.0f;
+        const int hk4 = 4 * qa, B = P.n_buckets;
+        for (int i = threadIdx.x; i < hk4; i += blockDim.x) { int h; const int c = begin_a(i >> 2, h) + (i & 3); s[i] = c < HK ? P.w[c] : 0.0f; }
         for (int i = threadIdx.x; i < B - 1; i += blockDim.x) s[hk4 + i] = P.bounds[i];
         for (int i = threadIdx.x; i < B * H; i += blockDim.x) s[hk4 + B + i] = P.table[i];
         __syncthreads();
@@ -154,6 +186,12 @@ template <class T, int SUB, bool VEC, int NV> struct Wave {
         const int before = __shfl_up(x.dst, 1);
         starts = (uint32_t)__ballot(lane < n && (lane == 0 || x.dst != before));
     }
+    // first element of feature quad q and its head
+    __device__ int begin_a(int q, int& h) const {
+        if (MODE == kAny || MODE == kAligned) { h = MODE == kAny ? 0 : (int)((q * inv_head) >> 16); return 4 * q; }
+        h = (int)((q * inv_head) >> 16);
+        return h * K + min(4 * (q - h * n_sub_a), K - 4);
+    }
     // feature quad i of the edges e_first .. e_first + GA - 1: its edge (relative to e_first) and quad; false if there is none
     __device__ bool a_place(int i, int e_first, int& e, int& q) const {
         const int idx = i * 64 + lane;
@@ -166,16 +204,16 @@ template <class T, int SUB, bool VEC, int NV> struct Wave {
     __device__ void load_a(Raw (&a)[NA], int64_t base, int n, int e_first) const {
 #pragma unroll
         for (int i = 0; i < NA; ++i) {
-            const int idx = i * 64 + lane, e = (int)((idx * inv_qa) >> 16), q = idx - e * qa;
-            a[i] = load_quad<T, VEC>((const T*)P.a + (base + min(e_first + e, n - 1)) * P.a_stride + 4 * q, HK - 4 * q);
+            int h;
+            const int idx = i * 64 + lane, e = (int)((idx * inv_qa) >> 16), q = idx - e * qa, c = begin_a(q, h);
+            a[i] = load_quad<T, MODE>((const T*)P.a + (base + min(e_first + e, n - 1)) * P.a_stride + c, HK - c);
         }
     }
     // the lane's quads of a row of H D elements
     __device__ void load_row(Raw (&v)[NV], const T* row) const {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int q = min(j * 64 + lane, qv - 1);
-            v[j] = load_quad<T, VEC>(row + 4 * q, HD - 4 * q);
+            v[j] = load_quad<T, MODE>(row + begin_v[j], HD - begin_v[j]);
         }
     }
     __device__ const T* value_row(int64_t e) const { return (const T*)P.v + min(e, e1 - 1) * P.v_stride; }
@@ -195,8 +233,10 @@ template <class T, int SUB, bool VEC, int NV> struct Wave {
             if (!a_place(i, e_first, e, q)) continue;
             const f4 wq = *(const f4*)(w + 4 * q);
             f4 x;
+            int h;
+            const int c = begin_a(q, h), shared = quad_shared<MODE>(c, h, K);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = act((float)a[i][j]);          // (0 where the row has no such element)
+            for (int j = 0; j < 4; ++j) x[j] = j < shared ? 0.0f : act((float)a[i][j]);          // (0 where the row has no such element)
             if (sub_a == 4) part[e * subs + q] = fmaf(x[3], wq[3], fmaf(x[2], wq[2], fmaf(x[1], wq[1], x[0] * wq[0])));
             else *(f4*)(part + e * subs + 4 * q) = x * wq;
         }
@@ -238,36 +278,43 @@ template <int NV, int PARTS> struct Row {
 // first row, slot 1 its last one.
 template <int NV, int PARTS> struct Record { f4 acc[NV]; double m[NV][PARTS]; float sum[NV][PARTS]; };
 
-template <class T, int SUB, bool VEC, int NV> __device__ inline void
-finish_row(const Args& P, int row, const Row<NV, 4 / SUB>& r, int lane, int qv, int HD, T* out, float* out32, double* norm) {
-    constexpr int PARTS = 4 / SUB;
+// begin_v, head: first element of each of the lane's quads, head of each of their parts
+template <class T, int MODE, int NV, int PARTS> __device__ inline void
+finish_row(const Args& P, int row, const Row<NV, PARTS>& r, int lane, int qv, const int (&begin_v)[NV], const int (&head)[NV][PARTS], T* out, float* out32, double* norm) {
+    constexpr int SUB = 4 / PARTS;
+    const int HD = P.heads * P.d;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int q = j * 64 + lane;
-        if (q >= qv) continue;
+        if (j * 64 + lane >= qv) continue;
         f4 o;
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
             const float inv = r.sum[j][p] == 0.0f ? 0.0f : 1.0f / r.sum[j][p];          // (no edge takes part: 0)
 #pragma unroll
             for (int i = 0; i < SUB; ++i) o[p * SUB + i] = r.acc[j][p * SUB + i] * inv;
-            const int c = 4 * q + p * SUB;
-            if (norm && c < HD && c % P.d == 0) *(d2*)(norm + 2 * ((int64_t)row * P.heads + c / P.d)) = d2{r.m[j][p], (double)inv};
+            if (norm && begin_v[j] + p * SUB == head[j][p] * P.d) *(d2*)(norm + 2 * ((int64_t)row * P.heads + head[j][p])) = d2{r.m[j][p], (double)inv};
         }
-        store_quad<T, VEC>(out + (int64_t)row * HD + 4 * q, o, HD - 4 * q);
-        if (out32) store_quad<float, VEC>(out32 + (int64_t)row * HD + 4 * q, o, HD - 4 * q);
+        store_quad<T, MODE>(out + (int64_t)row * HD + begin_v[j], o, HD - begin_v[j]);
+        if (out32) store_quad<float, MODE>(out32 + (int64_t)row * HD + begin_v[j], o, HD - begin_v[j]);
     }
+}
+// head of each part of the lane's quads
+template <int NV, int PARTS> __device__ inline void part_heads(const Args& P, const int (&begin_v)[NV], const int (&head_v)[NV], int (&head)[NV][PARTS]) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) head[j][p] = PARTS == 1 ? head_v[j] : min((begin_v[j] + p) / P.d, P.heads - 1);
 }
 
 // Read of the per-edge rows once; bandwidth bounds it, in 16 bits nearly as much the 46 vector instructions of an edge.  1.97 M edges of 64 + 240 channels:
 // float32 0.57 ms (4.4 TB/s), float16 0.30 ms (4.2 TB/s), where a large copy reaches 4.8.  A logit's 16 products are summed per quad by the lanes that
 // loaded it and finished by one lane for each edge and head, which also draws the dropout word: the walk then needs one share per edge and lane.  (Running
-// maxima per edge and lane instead: 0.69 ms in float16.)  At lmax 3 (296 channels, 74 quads) a lane holds two quads, the second one mostly idle: 0.13 ms for
+// maxima per edge and lane instead: 0.69 ms in float16.)  At lmax 3 (296 channels, 76 quads) a lane holds two quads, the second one mostly idle: 0.13 ms for
 // 499 979 edges, 2.7 TB/s, bound by instructions and by what 8 waves of a CU have in flight.
-template <class T, int SUB, bool VEC, int NV> __global__ __launch_bounds__(256, forward_waves(NV, SUB, sizeof(T)))
+template <class T, int MODE, int NV, int GA> __global__ __launch_bounds__(256, forward_waves(MODE, NV, sizeof(T)))
 void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, int64_t* rng_used) {
-    typedef Wave<T, SUB, VEC, NV> W;
-    constexpr int PARTS = W::PARTS, GA = W::GA;
+    typedef Wave<T, MODE, NV, GA> W;
+    constexpr int PARTS = W::PARTS, SUB = W::SUB;
     extern __shared__ __align__(16) char lds[];
     if (rng_used && P.threshold && blockIdx.x == 0 && threadIdx.x < 2) rng_used[threadIdx.x] = P.rng[threadIdx.x];
     const int edge_blocks = (P.n_waves + kWaves - 1) / kWaves;
@@ -286,12 +333,9 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
     }
     W w(P, lds, W::wave_bytes(P.heads) + (size_t)kBatch * P.heads * 8);
     if (w.e0 >= w.e1) { w.stage(lds); return; }
-    const int lane = w.lane, H = w.H, HD = w.HD, qv = w.qv;
+    const int lane = w.lane, H = w.H, qv = w.qv;
     int head[NV][PARTS];
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) head[j][p] = min((4 * (j * 64 + lane) + p * SUB) / P.d, H - 1);
+    part_heads(P, w.begin_v, w.head_v, head);
     // R value rows are always in flight: a row's registers are loaded again, R edges ahead, as soon as it has been added
     constexpr int R = W::RF;
     typename W::Edge edge = w.request(w.e0);
@@ -312,7 +356,7 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
             Record<NV, PARTS> x;
             for (int j = 0; j < NV; ++j) { x.acc[j] = r.acc[j]; for (int p = 0; p < PARTS; ++p) { x.m[j][p] = r.m[j][p]; x.sum[j][p] = r.sum[j][p]; } }
             rec[first_row ? 0 : 64] = x;
-        } else finish_row<T, SUB, VEC, NV>(P, cur, r, lane, qv, HD, out, out32, norm);
+        } else finish_row<T, MODE>(P, cur, r, lane, qv, w.begin_v, head, out, out32, norm);
     };
     float2* share = (float2*)w.keep;                       // [16][H] share of the piece, and that share times the dropout factor
     double* top = (double*)(w.e_bucket + kBatch);          // [16][H] logit that the shares are relative to
@@ -331,10 +375,11 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
             bool near = false;
             uint64_t some = ~(uint64_t)0;          // bit 4 e: edge e takes part somewhere
             bool select = true;                    // an edge may take part in one head and not in another
-            if (GA == 16 && H == 4) {
+            if (GA == 16 && H <= 4) {
                 // one edge and head a lane: the largest and smallest logits of the group, through the wave
                 const int e = lane >> 2, h = lane & 3;
-                const double x = w.logit(g, e, h);
+                const bool there = h < H;
+                const double x = there ? w.logit(g, e, h) : -__builtin_inf();
                 const bool in = e < live && x != -__builtin_inf();
                 float most = in ? (float)x : -__builtin_inff(), least = in ? (float)x : __builtin_inff();
                 most = fmaxf(most, ror<0x124>(most)); least = fminf(least, ror<0x124>(least));
@@ -344,12 +389,14 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
                 near = __ballot(most != -__builtin_inff() && !(most - least <= 24.0f && fabsf(most) <= 1e6f)) == 0;
                 if (near) {
                     const float p = in ? exp_d(x - (double)most) : 0.0f;
-                    share[(g + e) * 4 + h] = float2{p, in ? p * w.dropped(base + g + e, h) : 0.0f};
-                    top[(g + e) * 4 + h] = (double)most;
-                    const uint64_t b = __ballot(in), heads = 0x1111111111111111ull;
+                    if (there) {
+                        share[(g + e) * H + h] = float2{p, in ? p * w.dropped(base + g + e, h) : 0.0f};
+                        top[(g + e) * H + h] = (double)most;
+                    }
+                    const uint64_t b = __ballot(in), all = __ballot(in || !there), heads = 0x1111111111111111ull;
                     some = b | b >> 1 | b >> 2 | b >> 3;
-                    select = ((some ^ (b & b >> 1 & b >> 2 & b >> 3)) & heads) != 0;
-                } else w.t[(g + e) * 4 + h] = x;
+                    select = ((some ^ (all & all >> 1 & all >> 2 & all >> 3)) & heads) != 0;
+                } else if (there) w.t[(g + e) * H + h] = x;
             } else {
                 for (int idx = lane; idx < GA * H; idx += 64) {
                     const int e = (int)((idx * w.inv_h) >> 16), h = idx - e * H;
@@ -420,10 +467,14 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
 // Rows that cross ranges.  Few bytes, all waiting: 3 000 ranges 7.5 us, 7 rows of 536 records each 29 us.  A wave looks at one border between two ranges and takes a row whose first crossing that is: it joins up to 8 records by itself;
 // a longer row is joined by the whole workgroup, every wave a share of the records, then the waves' results in order.
 template <int NV> constexpr int merge_waves() { return 16 / NV; }
-template <class T, int SUB, bool VEC, int NV> __global__ __launch_bounds__(1024 / NV)
+template <class T, int MODE, int NV> __global__ __launch_bounds__(1024 / NV)
 void k_attn_merge(Args P, T* out, float* out32, double* norm, const void* records) {
-    constexpr int PARTS = 4 / SUB, WAVES = merge_waves<NV>();
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), H = P.heads, HD = H * P.d, qv = (HD + 3) >> 2;
+    constexpr int SUB = MODE == kAny ? 1 : 4, PARTS = 4 / SUB, WAVES = merge_waves<NV>();
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), qv = row_quads(MODE, P.heads, P.d);
+    int begin_v[NV], head_v[NV], head[NV][PARTS];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) begin_v[j] = quad_start<MODE>(min(j * 64 + lane, qv - 1), P.heads, P.d, head_v[j]);
+    part_heads(P, begin_v, head_v, head);
     __shared__ Record<NV, PARTS> share[WAVES - 1][64];
     __shared__ int long_row[WAVES], long_first[WAVES];
     const Record<NV, PARTS>* rec = (const Record<NV, PARTS>*)records + lane;
@@ -457,7 +508,7 @@ void k_attn_merge(Args P, T* out, float* out32, double* norm, const void* record
         if (P.dst[border - 1] == row) {
             const int64_t begin = P.rowptr[row], last = ((int64_t)P.rowptr[row + 1] - 1) / P.range;
             if (begin >= mine * P.range) {                              // (else an earlier border is its first)
-                if (last - mine < 8) { join_records(mine, begin, mine, last, 1); finish_row<T, SUB, VEC, NV>(P, row, r, lane, qv, HD, out, out32, norm); }
+                if (last - mine < 8) { join_records(mine, begin, mine, last, 1); finish_row<T, MODE>(P, row, r, lane, qv, begin_v, head, out, out32, norm); }
                 else if (lane == 0) { long_row[wave] = row; long_first[wave] = (int)mine; }
             }
         }
@@ -475,7 +526,7 @@ void k_attn_merge(Args P, T* out, float* out32, double* norm, const void* record
         __syncthreads();
         if (wave == 0) {
             for (int o = 0; o < WAVES - 1; ++o) join(share[o][lane].acc, share[o][lane].m, share[o][lane].sum);
-            finish_row<T, SUB, VEC, NV>(P, row, r, lane, qv, HD, out, out32, norm);
+            finish_row<T, MODE>(P, row, r, lane, qv, begin_v, head, out, out32, norm);
         }
         __syncthreads();
     }
@@ -509,25 +560,27 @@ struct BackArgs {
 // lasts, so nothing waits where rows are short.  1.97 M edges of 64 + 240 float32 channels: 1.02 ms, 4.8 TB/s, the rate of a large copy; 499 979 bfloat16 edges
 // of lmax 3 0.25 ms, 2.9 TB/s, bound by the latency that three waves a SIMD cover.  The dot of a value row with dout goes through LDS (a partial sum for each
 // quad part), since a head's quads are not a power of two of lanes.
-template <class T, int SUB, bool VEC, int NV> __global__ __launch_bounds__(256, backward_waves(NV, sizeof(T)))
+template <class T, int MODE, int NV, int GA> __global__ __launch_bounds__(256, backward_waves(MODE, NV, sizeof(T)))
 void k_attn_backward(Args P, BackArgs B) {
-    typedef Wave<T, SUB, VEC, NV> W;
-    constexpr int NA = W::NA, PARTS = W::PARTS, GA = W::GA, R = W::R;
+    typedef Wave<T, MODE, NV, GA> W;
+    constexpr int NA = W::NA, PARTS = W::PARTS, SUB = W::SUB, R = W::R;
     extern __shared__ __align__(16) char lds[];
     const int BH = P.n_buckets * P.heads;
     const size_t own = W::wave_bytes(P.heads) + (size_t)kBatch * P.heads * 4 + (size_t)((BH + 1) & ~1) * 4;
     W w(P, lds, (own + 15) & ~(size_t)15);
-    const int lane = w.lane, H = w.H, HD = w.HD, HK = w.HK, qv = w.qv, subs = qv * PARTS, per_head = P.d / SUB;
+    const int lane = w.lane, H = w.H, HD = w.HD, HK = w.HK, qv = w.qv, subs = qv * PARTS, per_head = MODE == kAny ? P.d : (P.d + 3) >> 2;
     float2* share = (float2*)w.keep;                    // [16][H] probability and dropout factor
     float* weight = (float*)w.t;                        // [16][H] their product
     float* dt = (float*)(w.e_bucket + kBatch);          // [16][H]
     float* bins = dt + kBatch * H;                      // [buckets][H]
     for (int i = lane; i < BH; i += 64) bins[i] = 0.0f;
     int head[NV][PARTS];
+    part_heads(P, w.begin_v, w.head_v, head);
+    int shared_v[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) head[j][p] = min((4 * (j * 64 + lane) + p * SUB) / P.d, H - 1);
+    for (int j = 0; j < NV; ++j) shared_v[j] = quad_shared<MODE>(w.begin_v[j], w.head_v[j], P.d);
+    int lanes = 0;          // 2^lanes lanes sum the dot of an edge and head
+    while (lanes < 3 && (2 * R * H << lanes) <= 64) ++lanes;
     f4 dw[NA];
     int head_a[NA];          // of the lane's feature quads, where a quad lies inside one head
 #pragma unroll
@@ -535,7 +588,7 @@ void k_attn_backward(Args P, BackArgs B) {
         int e, q;
         w.a_place(i, 0, e, q);
         dw[i] = f4{0, 0, 0, 0};
-        head_a[i] = min(4 * q / P.k, H - 1);
+        head_a[i] = min(MODE == kAny ? 4 * q / P.k : (int)((q * w.inv_head) >> 16), H - 1);
     }
 
     if (w.e0 >= w.e1) w.stage(lds);
@@ -596,12 +649,13 @@ void k_attn_backward(Args P, BackArgs B) {
                                         const int c = p * SUB + k;
                                         o[c] = f * (float)up[i][j][c];
                                         dot[p] = fmaf((float)v[i][j][c], (float)up[i][j][c], dot[p]);
+                                        if (MODE == kHeads && c < 3) dot[p] = c < shared_v[j] ? 0.0f : dot[p];
                                     }
                                 }
                                 if (q < qv) {
 #pragma unroll
                                     for (int p = 0; p < PARTS; ++p) w.part[i * subs + q * PARTS + p] = dot[p];
-                                    if (B.dv) store_quad<T, VEC>((T*)B.dv + (base + s + i) * HD + 4 * q, o, HD - 4 * q);
+                                    if (B.dv) store_quad<T, MODE>((T*)B.dv + (base + s + i) * HD + w.begin_v[j], o, HD - w.begin_v[j]);
                                 }
                             }
                         }
@@ -616,22 +670,14 @@ void k_attn_backward(Args P, BackArgs B) {
                         // (a masked edge's value may be NaN)
                         dt[(s + i) * H + h] = f.x == 0.0f ? 0.0f : f.x * ((f.y == 0.0f ? 0.0f : f.y * dot) - B.delta[(int64_t)w.e_dst[s + i] * H + h]);
                     };
-                    if (H == 4) {          // 64 / (4 R) lanes share an edge and head's sum
-                        constexpr int L = 64 / (4 * R);
-                        const int k = lane / L, l = lane & (L - 1), i = k >> 2, h = k & 3;
+                    for (int k = lane >> lanes; k < last * H; k += 64 >> lanes) {
+                        const int i = (int)((k * w.inv_h) >> 16), h = k - i * H, l = lane & ((1 << lanes) - 1);
                         float dot = 0.0f;
-                        if (i < last) for (int c = l; c < per_head; c += L) dot += w.part[i * subs + h * per_head + c];
-                        dot += ror<0xB1>(dot);
-                        if (L > 2) dot += ror<0x4E>(dot);
-                        if (L > 4) dot += ror<0x141>(dot);
-                        if (i < last && l == 0) write_dt(i, h, dot);
-                    } else {
-                        for (int k = lane; k < last * H; k += 64) {
-                            const int i = (int)((k * w.inv_h) >> 16), h = k - i * H;
-                            float dot = 0.0f;
-                            for (int c = 0; c < per_head; ++c) dot += w.part[i * subs + h * per_head + c];
-                            write_dt(i, h, dot);
-                        }
+                        for (int c = l; c < per_head; c += 1 << lanes) dot += w.part[i * subs + h * per_head + c];
+                        if (lanes > 0) dot += ror<0xB1>(dot);
+                        if (lanes > 1) dot += ror<0x4E>(dot);
+                        if (lanes > 2) dot += ror<0x141>(dot);
+                        if (l == 0) write_dt(i, h, dot);
                     }
                     wave_sync();
                 }
@@ -654,7 +700,9 @@ void k_attn_backward(Args P, BackArgs B) {
                         o[j] = f == 0.0f ? 0.0f : f * wq[j] * slope;
                         dw[i][j] = f == 0.0f ? dw[i][j] : fmaf(f, kActNorm * x * fmaf(0.8f, sg, 0.2f), dw[i][j]);
                     }
-                    if (B.da) store_quad<T, VEC>((T*)B.da + (base + g + e) * HK + 4 * q, o, HK - 4 * q);
+                    int h;
+                    const int c = w.begin_a(q, h);
+                    if (B.da) store_quad<T, MODE>((T*)B.da + (base + g + e) * HK + c, o, HK - c);
                 }
                 if (BH && B.param_rows && lane < H)          // in the edges' order: lane h alone adds to the sums of its head
                     for (int e = 0; e < GA && g + e < w.n; ++e) bins[w.e_bucket[g + e] * H + lane] += dt[(g + e) * H + lane];
@@ -671,10 +719,12 @@ void k_attn_backward(Args P, BackArgs B) {
     __syncthreads();
     const size_t stride = (own + 15) & ~(size_t)15;
     for (int c = threadIdx.x; c < HK; c += 256) {
+        int at = c;          // its place among the feature quads' elements
+        if (MODE == kHeads) { const int h = c / P.k, x = c - h * P.k; at = 4 * (h * w.n_sub_a + (x >> 2)) + x - min(x & ~3, P.k - 4); }
         float s = 0.0f;
         for (int x = 0; x < kWaves; ++x) {
             const float* part = (const float*)((const char*)w.part + ((ptrdiff_t)x - w.wave) * (ptrdiff_t)stride);
-            for (int i = c >> 2; i < GA * w.qa; i += w.qa) s += part[4 * i + (c & 3)];
+            for (int i = at >> 2; i < GA * w.qa; i += w.qa) s += part[4 * i + (at & 3)];
         }
         B.param_rows[(size_t)blockIdx.x * (HK + BH) + c] = s;
     }

@@ -10,25 +10,25 @@ using namespace dedf::attn;
 namespace dedf {
 namespace attn {
 
-struct Plan { Args a; int nv, sub; size_t record, lds_forward, lds_backward; int blocks; };
+struct Plan { Args a; int mode, nv, ga; size_t record, lds_forward, lds_backward; int blocks; };
 
 struct Forward {
     const Plan& p; void* out; float* out32; double* norm; int64_t* rng_used; void* records; hipStream_t st;
-    template <class T, int SUB, bool VEC, int NV> int run() {
-        if (p.lds_forward > 65536 && hipFuncSetAttribute((const void*)k_attn_forward<T, SUB, VEC, NV>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds_forward) != hipSuccess) return DEDF_ERR_RUNTIME;
+    template <class T, int MODE, int NV, int GA> int run() {
+        if (p.lds_forward > 65536 && hipFuncSetAttribute((const void*)k_attn_forward<T, MODE, NV, GA>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds_forward) != hipSuccess) return DEDF_ERR_RUNTIME;
         const int empty_blocks = (p.a.n_dst + 64 * kWaves - 1) / (64 * kWaves);
-        hipLaunchKernelGGL((k_attn_forward<T, SUB, VEC, NV>), dim3(p.blocks + empty_blocks), dim3(256), p.lds_forward, st, p.a, (T*)out, out32, norm, records, rng_used);
-        if (p.a.n_waves > 1) hipLaunchKernelGGL((k_attn_merge<T, SUB, VEC, NV>), dim3((p.a.n_waves - 1 + merge_waves<NV>() - 1) / merge_waves<NV>()), dim3(1024 / NV), 0, st, p.a, (T*)out, out32, norm, (const void*)records);
+        hipLaunchKernelGGL((k_attn_forward<T, MODE, NV, GA>), dim3(p.blocks + empty_blocks), dim3(256), p.lds_forward, st, p.a, (T*)out, out32, norm, records, rng_used);
+        if (p.a.n_waves > 1) hipLaunchKernelGGL((k_attn_merge<T, MODE, NV>), dim3((p.a.n_waves - 1 + merge_waves<NV>() - 1) / merge_waves<NV>()), dim3(1024 / NV), 0, st, p.a, (T*)out, out32, norm, (const void*)records);
         return hipGetLastError() == hipSuccess ? DEDF_OK : DEDF_ERR_RUNTIME;
     }
 };
 struct Backward {
     const Plan& p; BackArgs b; const float* out32; float* delta; float* d_alpha_dot; float* d_table; hipStream_t st;
-    template <class T, int SUB, bool VEC, int NV> int run() {
-        if (p.lds_backward > 65536 && hipFuncSetAttribute((const void*)k_attn_backward<T, SUB, VEC, NV>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds_backward) != hipSuccess) return DEDF_ERR_RUNTIME;
+    template <class T, int MODE, int NV, int GA> int run() {
+        if (p.lds_backward > 65536 && hipFuncSetAttribute((const void*)k_attn_backward<T, MODE, NV, GA>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds_backward) != hipSuccess) return DEDF_ERR_RUNTIME;
         const Args& a = p.a;
         hipLaunchKernelGGL((k_attn_delta<T>), dim3((a.n_dst + kWaves - 1) / kWaves), dim3(256), 0, st, (int64_t)a.n_dst, a.heads, a.d, (const T*)b.grad, out32, delta);
-        hipLaunchKernelGGL((k_attn_backward<T, SUB, VEC, NV>), dim3(p.blocks), dim3(256), p.lds_backward, st, a, b);
+        hipLaunchKernelGGL((k_attn_backward<T, MODE, NV, GA>), dim3(p.blocks), dim3(256), p.lds_backward, st, a, b);
         if (b.param_rows) {
             const int n_w = a.heads * a.k, columns = n_w + a.heads * a.n_buckets;
             hipLaunchKernelGGL(k_column_sums, dim3((columns + 15) / 16), dim3(1024), 0, st, (const float*)b.param_rows, p.blocks, columns, d_alpha_dot, n_w, d_table);
@@ -37,14 +37,16 @@ struct Backward {
     }
 };
 
-template <class T, int SUB, bool VEC, class F> int by_width(int nv, F& f) {
-    return nv == 1 ? f.template run<T, SUB, VEC, 1>() : nv == 2 ? f.template run<T, SUB, VEC, 2>() : f.template run<T, SUB, VEC, 4>();
+template <class T, int MODE, class F> int by_width(int nv, int ga, F& f) {
+    if (nv == 4) return f.template run<T, MODE, 4, 4>();
+    if (nv == 2) return ga == 16 ? f.template run<T, MODE, 2, 16>() : ga == 8 ? f.template run<T, MODE, 2, 8>() : f.template run<T, MODE, 2, 4>();
+    return ga == 16 ? f.template run<T, MODE, 1, 16>() : f.template run<T, MODE, 1, 8>();
 }
-template <class T, class F> int launch(int sub, int nv, F f) {          // sub 0: rows that do not consist of whole, aligned quads
-    return sub == 4 ? by_width<T, 4, true>(nv, f) : sub == 2 ? by_width<T, 2, true>(nv, f) : sub == 1 ? by_width<T, 1, true>(nv, f) : by_width<T, 1, false>(nv, f);
+template <class T, class F> int launch(int mode, int nv, int ga, F f) {
+    return mode == kAligned ? by_width<T, kAligned>(nv, ga, f) : mode == kHeads ? by_width<T, kHeads>(nv, ga, f) : by_width<T, kAny>(nv, ga, f);
 }
 
-#define DEDF_LAUNCHES(T, PREFIX) PREFIX template int launch<T, Forward>(int, int, Forward); PREFIX template int launch<T, Backward>(int, int, Backward);
+#define DEDF_LAUNCHES(T, PREFIX) PREFIX template int launch<T, Forward>(int, int, int, Forward); PREFIX template int launch<T, Backward>(int, int, int, Backward);
 #ifndef DEDF_ELEMENT
 DEDF_LAUNCHES(float, extern) DEDF_LAUNCHES(_Float16, extern) DEDF_LAUNCHES(__bf16, extern)
 #elif DEDF_ELEMENT == 0
@@ -65,9 +67,9 @@ constexpr int kSimds = 1024;          // 256 CUs of 4
 constexpr size_t kMostLds = 160 * 1024;
 
 size_t element(int type) { return type == DEDF_F32 ? 4 : 2; }
-bool whole_quads(const void* p, int64_t stride, int width, int type) {
+bool whole_quads(const void* p, int64_t stride, int type) {
     const size_t quad = 4 * element(type);
-    return (reinterpret_cast<uintptr_t>(p) % quad) == 0 && stride % 4 == 0 && width % 4 == 0;
+    return (reinterpret_cast<uintptr_t>(p) % quad) == 0 && stride % 4 == 0;
 }
 
 // `tensors`: the call's other tensors of (edges or rows, heads, k or d) in the element type
@@ -90,21 +92,23 @@ int make_plan(const dedf_edge_attn* x, bool backward, Plan& p, std::initializer_
     a.n_buckets = x->n_buckets;
     a.threshold = (uint32_t)std::floor(x->dropout * 4294967296.0);
     a.keep_scale = (float)(1.0 / (1.0 - x->dropout)); a.rng = x->rng;
-    bool whole = whole_quads(a.a, a.a_stride, a.heads * a.k, x->type) && whole_quads(a.v, a.v_stride, a.heads * a.d, x->type);
-    for (const void* t : tensors) whole = whole && whole_quads(t, 0, 0, x->type);
-    p.sub = !whole ? 0 : x->d % 4 == 0 ? 4 : x->d % 2 == 0 ? 2 : 1;
-    p.nv = a.heads * a.k > 64 || a.heads * a.d > 512 ? 4 : a.heads * a.d > 256 ? 2 : 1;
-    const int most = kSimds * (backward ? backward_waves(p.nv, (int)element(x->type)) : forward_waves(p.nv, p.sub ? p.sub : 1, (int)element(x->type)));
+    bool whole = a.k % 4 == 0 && a.d % 4 == 0 && whole_quads(a.a, a.a_stride, x->type) && whole_quads(a.v, a.v_stride, x->type);
+    for (const void* t : tensors) whole = whole && whole_quads(t, 0, x->type);
+    p.mode = whole ? kAligned : a.k >= 4 && a.d >= 4 && row_quads(kHeads, a.heads, a.k) <= 64 && row_quads(kHeads, a.heads, a.d) <= 256 ? kHeads : kAny;
+    const int qa = row_quads(p.mode, a.heads, a.k), qv = row_quads(p.mode, a.heads, a.d);
+    p.ga = qv > 128 || qa > 32 ? 4 : qa > 16 ? 8 : 16;
+    p.nv = qv > 128 ? 4 : qv > 64 || p.ga == 4 ? 2 : 1;
+    const int bytes = (int)element(x->type), most = kSimds * (backward ? backward_waves(p.mode, p.nv, bytes) : forward_waves(p.mode, p.nv, bytes));
     const int64_t even = (a.n_edges + most - 1) / most;
     a.range = (int)std::max<int64_t>(kBatch, (even + kBatch - 1) / kBatch * kBatch);
     a.n_waves = (int)((a.n_edges + a.range - 1) / a.range);
     p.blocks = (a.n_waves + kWaves - 1) / kWaves;
-    const int parts = p.sub == 4 ? 1 : p.sub == 2 ? 2 : 4;          // (as the kernels' Record<nv, parts>)
+    const int parts = p.mode == kAny ? 4 : 1;          // (as the kernels' Record<nv, parts>)
     p.record = (size_t)(p.nv * 16 + p.nv * parts * 12 + 15) / 16 * 16 * 64 * 2;
-    static_assert(sizeof(Record<1, 1>) == 32 && sizeof(Record<1, 4>) == 64 && sizeof(Record<2, 2>) == 80 && sizeof(Record<4, 4>) == 256, "records are as large as computed here");
-    const size_t own = p.sub <= 1 ? Wave<float, 1, true, 1>::wave_bytes(a.heads) : Wave<float, 4, true, 1>::wave_bytes(a.heads);          // (whatever the type and width)
+    static_assert(sizeof(Record<1, 1>) == 32 && sizeof(Record<1, 4>) == 64 && sizeof(Record<2, 1>) == 64 && sizeof(Record<4, 1>) == 112 && sizeof(Record<2, 4>) == 128 && sizeof(Record<4, 4>) == 256, "records are as large as computed here");
+    const size_t own = p.mode == kAny ? Wave<float, kAny, 1, 16>::wave_bytes(a.heads) : Wave<float, kAligned, 1, 16>::wave_bytes(a.heads);          // (whatever the type and width)
     const int BH = a.n_buckets * a.heads;
-    const size_t shared = Wave<float, 4, true, 1>::shared_bytes(a.heads * a.k, a.heads, a.n_buckets);
+    const size_t shared = Wave<float, kAligned, 1, 16>::shared_bytes(qa, a.heads, a.n_buckets);
     p.lds_forward = shared + kWaves * (own + (size_t)kBatch * a.heads * 8);
     p.lds_backward = shared + kWaves * ((own + (size_t)kBatch * a.heads * 4 + (size_t)((BH + 1) & ~1) * 4 + 15) & ~(size_t)15);
     if (p.lds_forward > kMostLds || p.lds_backward > kMostLds) return DEDF_ERR_UNSUPPORTED;
@@ -112,8 +116,8 @@ int make_plan(const dedf_edge_attn* x, bool backward, Plan& p, std::initializer_
 }
 size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 size_t forward_bytes(const Plan& p) { return (size_t)p.blocks * kWaves * p.record; }
-template <class F> int by_shape(int type, int sub, int nv, F f) {
-    return type == DEDF_F32 ? launch<float>(sub, nv, f) : type == DEDF_F16 ? launch<_Float16>(sub, nv, f) : launch<__bf16>(sub, nv, f);
+template <class F> int by_shape(int type, const Plan& p, F f) {
+    return type == DEDF_F32 ? launch<float>(p.mode, p.nv, p.ga, f) : type == DEDF_F16 ? launch<_Float16>(p.mode, p.nv, p.ga, f) : launch<__bf16>(p.mode, p.nv, p.ga, f);
 }
 size_t backward_bytes(const Plan& p) {
     return up16((size_t)p.a.n_dst * p.a.heads * 4) + (size_t)p.blocks * (p.a.heads * (p.a.k + p.a.n_buckets)) * 4;
@@ -147,7 +151,7 @@ int dedf_edge_attention(const dedf_edge_attn* x, void* out, float* out_f, double
     if (p.a.n_dst == 0) return DEDF_OK;
     if (!out || scratch_bytes < forward_bytes(p) || (forward_bytes(p) > 0 && !scratch) || (reinterpret_cast<uintptr_t>(scratch) & 15)) return DEDF_ERR_INVALID;
     Forward f{p, out, out_f, norm, rng_used, scratch, static_cast<hipStream_t>(stream)};
-    return by_shape(x->type, p.sub, p.nv, f);
+    return by_shape(x->type, p, f);
 }
 
 int dedf_edge_attention_backward(const dedf_edge_attn* x, const double* norm, const float* out_f, const void* grad_out, void* d_alpha, void* d_value,
@@ -166,7 +170,7 @@ int dedf_edge_attention_backward(const dedf_edge_attn* x, const double* norm, co
     BackArgs b{norm, (const float*)scratch, grad_out, d_alpha, d_value, d_edge_logits,
                d_alpha_dot || d_bias_table ? (float*)((char*)scratch + up16((size_t)p.a.n_dst * p.a.heads * 4)) : nullptr};
     Backward f{p, b, out_f, (float*)scratch, d_alpha_dot, d_bias_table, st};
-    return by_shape(x->type, p.sub, p.nv, f);
+    return by_shape(x->type, p, f);
 }
 
 }  // extern "C"

@@ -270,6 +270,41 @@ def test_edge_attention(dtype, N, E, kw):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,K,D", [
+    (8, 16, 30), (8, 17, 31), (8, 9, 65), (8, 16, 64), (16, 13, 13), (16, 4, 5), (16, 9, 64), (2, 128, 6), (1, 129, 130), (1, 61, 62), (1, 255, 1021), (3, 23, 341), (2, 7, 509),
+    (5, 51, 9), (13, 17, 4), (4, 4, 4), (5, 5, 5), (7, 6, 6), (1, 4, 7), (6, 3, 9), (6, 9, 3), (16, 2, 64), (8, 1, 20), (7, 3, 10), (2, 2, 12), (5, 1, 60), (16, 3, 4),
+])
+def test_edge_attention_heads_of_any_width(dtype, H, K, D):
+    """head widths that are no multiples of 4 (each remainder, in features and values), widths below 4, feature rows of up to 16, 32 and 64 quads, value rows of
+    up to 64, 128 and 256, and rows that have more quads than that if each head has its own"""
+    _check(_case(dtype, 11, 150, H=H, K=K, D=D, buckets=3, drop=0.15, seed=H * K))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,K,D", [(3, 5, 7), (8, 17, 31), (3, 23, 341), (6, 3, 9), (1, 7, 13)])
+def test_edge_attention_heads_of_any_width_across_ranges(H, K, D):
+    g = torch.Generator().manual_seed(D)
+    _check(_case(torch.float32, 3, 9_001, H=H, K=K, D=D, buckets=5, drop=0.0, dst=torch.randint(0, 3, (9_001,), generator=g).sort().values))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,K,D", [(8, 17, 31), (3, 5, 7), (6, 3, 9)])
+def test_edge_attention_columns_at_an_odd_element(H, K, D):
+    """value as columns of a wider tensor with NaN around them, at an odd element: the same bits, and a gradient of those columns alone"""
+    c = _case(torch.float32, 5, 70, H=H, K=K, D=D, seed=2, drop=0.0)
+    want, ref = _gpu(c)
+    a, v, seg = c["alpha"].cuda(), c["value"].cuda(), EdgeSegments(c["dst"].cuda(), 5)
+    wide = torch.full((70, 3 + H * D + 2), float("nan"), device="cuda")
+    wide[:, 3:3 + H * D] = v.reshape(70, H * D)
+    wide.requires_grad_(True)
+    out = edge_attention(a, wide[:, 3:3 + H * D].view(70, H, D), c["dot"].cuda(), seg, edge_logits=c["logits"].cuda())
+    assert torch.equal(out, want)
+    g, = torch.autograd.grad(out, wide, c["grad"].cuda())
+    assert torch.equal(g[:, 3:3 + H * D].reshape(70, H, D), ref["value"]) and not g[:, :3].any() and not g[:, 3 + H * D:].any()
+
+
+@pytest.mark.gpu
 def test_edge_attention_without_edges_or_rows():
     for N, E in ((0, 0), (5, 0)):
         out, grads = _check(_case(torch.float32, N, E, buckets=4, drop=0.1))
