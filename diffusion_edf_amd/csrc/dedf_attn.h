@@ -26,15 +26,12 @@ namespace attn {
 
 constexpr int kBatch = 16;                 // edges per step of a wave
 constexpr int kWaves = 4;                  // waves per workgroup
-enum { kAny = 0, kHeads = 1, kAligned = 2 };          // how a row is cut into quads: see load_quad
+enum { kElements = 0, kHeads = 1, kAligned = 2 };          // how a row is cut into quads: see load_quad
 // Waves a SIMD holds, by the registers of each instantiation; a launch has as many waves as are resident at once, each with one range of edges.  More
 // waves than that run in two rounds, of which the second is half empty: 1.97 M edges, float32, a training pass with 2 048 waves
 // in the backward kernel 1.65 ms, with 3 072 1.83 ms.
-constexpr int forward_waves(int mode, int nv, int bytes) {
-    if (mode == kAny) return nv == 1 ? 3 : nv == 2 && bytes == 2 ? 2 : 1;
-    return nv == 4 ? 2 : nv == 1 && bytes == 2 ? 4 : 3;
-}
-constexpr int backward_waves(int mode, int nv, int bytes) { return bytes == 2 && nv <= 2 && mode != kAny ? 3 : 2; }          // (499 979 edges, lmax 3, bfloat16: 0.46 ms with 3, 0.52 with 2; parts by elements, which spill: 2)
+constexpr int forward_waves(int nv, int bytes) { return nv == 4 ? 2 : nv == 1 && bytes == 2 ? 4 : 3; }
+constexpr int backward_waves(int nv, int bytes) { return bytes == 2 && nv <= 2 ? 3 : 2; }          // (499 979 edges, lmax 3, bfloat16: 0.46 ms with 3, 0.52 with 2)
 constexpr float kActNorm = 1.531320475574866f;
 constexpr double kLog2e = 1.4426950408889634;
 
@@ -60,43 +57,37 @@ struct Args {
     int range, n_waves;                    // edges per wave, waves
 };
 
-// How a row is cut into quads (MODE):
-//   kAligned  head widths are multiples of 4 and every row begins at a whole quad: quads lie one behind the other, an aligned access each
-//   kHeads    any other head width from 4: each head has quads of its own, the last of which ends with the head and so begins inside the one before; an
-//             unaligned access each.  Elements that two quads hold are summed by the first of them.
-//   kAny      what has more quads than a wave holds that way, or narrower heads: quads one behind the other across the heads, by elements
-// 400 000 edges of 3 heads of 17 + 33 channels, a training pass: float32 0.24 ms (by elements 0.42), bfloat16 0.20 ms (0.64); 4 aligned heads of 16 + 60
-// 0.36 ms in float32, of 16 + 61 0.38 ms.
-template <class T, int MODE> __device__ inline typename Quad<T>::type load_quad(const T* p, int left) {
+// How a row of H heads is cut into quads (MODE).  A quad lies inside one head.
+//   kAligned   head widths are multiples of 4 and every row begins at a whole quad: an aligned access each
+//   kHeads     any other head width from 4: the head's last quad ends with the head and so begins inside the one before; an unaligned access each.  What two
+//              quads hold is summed by the first of them.
+//   kElements  heads narrower than a quad: element by element, the others zero
+// 400 000 edges of 3 heads of 17 + 33 channels, a training pass: float32 0.24 ms (quads across the heads, by elements: 0.42), bfloat16 0.20 ms (0.64); 4 aligned
+// heads of 16 + 60 0.36 ms in float32, of 16 + 61 0.38 ms.
+template <class T, int MODE> __device__ inline typename Quad<T>::type load_quad(const T* p, int width) {
     typename Quad<T>::type r = {(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f};
     if constexpr (MODE == kAligned) r = *(const typename Quad<T>::type*)p;
     else if constexpr (MODE == kHeads) __builtin_memcpy(&r, p, sizeof(r));
     else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) if (i < left) r[i] = p[i];
+        for (int i = 0; i < 3; ++i) if (i < width) r[i] = p[i];
     }
     return r;
 }
-template <class T, int MODE> __device__ inline void store_quad(T* p, f4 x, int left) {
+template <class T, int MODE> __device__ inline void store_quad(T* p, f4 x, int width) {
     const typename Quad<T>::type r = {(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
     if constexpr (MODE == kAligned) *(typename Quad<T>::type*)p = r;
     else if constexpr (MODE == kHeads) __builtin_memcpy(p, &r, sizeof(r));
     else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) if (i < left) p[i] = r[i];
+        for (int i = 0; i < 3; ++i) if (i < width) p[i] = r[i];
     }
 }
-// quads of a row of H heads of `width` elements, as the kernels and their launches see it
-__host__ __device__ constexpr int row_quads(int mode, int H, int width) { return mode == kAny ? (H * width + 3) >> 2 : H * ((width + 3) >> 2); }
-// first element of quad q and the head that it lies in (kAny: that its first element lies in)
-template <int MODE> __device__ inline int quad_start(int q, int H, int width, int& head) {
-    if constexpr (MODE == kAny) { head = min(4 * q / width, H - 1); return 4 * q; }
-    const int n = (width + 3) >> 2;
-    head = min(q / n, H - 1);
-    return head * width + min(4 * (q - head * n), width - 4);
-}
-// elements of it that the quad before holds too
-template <int MODE> __device__ inline int quad_shared(int start, int head, int width) { return MODE == kHeads ? -(start - head * width) & 3 : 0; }
+// quads of a row of H heads
+__host__ __device__ constexpr int row_quads(int H, int width) { return H * ((width + 3) >> 2); }
+// first element of the head's quad i, relative to the head, and how many of its elements the quad before holds too
+__device__ inline int quad_begin(int i, int width) { return width < 4 ? 0 : min(4 * i, width - 4); }
+__device__ inline int quad_shared(int begin) { return -begin & 3; }
 
 // LDS of one wave is written and read by its own lanes only: LDS operations of a wave complete in order, the compiler must keep that order
 __device__ inline void wave_sync() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
@@ -118,20 +109,30 @@ __device__ inline int bucket_of(const float* bounds, int n, float x) {
     return lo;
 }
 
+// first element of each of the lane's value quads (the last one where it has none) and its head
+template <int NV> __device__ inline void value_places(const Args& P, int lane, int (&begin)[NV], int (&head)[NV]) {
+    const int per = (P.d + 3) >> 2;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int q = min(j * 64 + lane, P.heads * per - 1);
+        head[j] = q / per;
+        begin[j] = head[j] * P.d + quad_begin(q - head[j] * per, P.d);
+    }
+}
+
 // what both directions share: the wave's place, its LDS, the batch's per-edge values, the logits
-//   MODE: see load_quad; a quad is cut into PARTS parts of SUB elements that each lie inside one head
+//   MODE: how value rows are cut (see load_quad); feature rows are cut that way too, with kHeads and kElements by the width of their own heads
 //   NV: quads of a value row a lane holds: 1, 2 or 4 (up to 64, 128, 256 quads)
-//   GA: edges whose features are loaded at once: 16 (feature rows of up to 16 quads), 8 (32) or 4 (64)
+//   GA: edges whose features are loaded at once: 16 (feature rows of up to 16 quads), 8 (32), 4 (64) or 2 (128)
 template <class T, int MODE, int NV, int GA> struct Wave {
     static constexpr int NA = 4;                                             // GA edges x feature quads fill NA loads of a wave
     static constexpr int rows(int quads) { return quads / NV < GA ? quads / NV : GA; }
     static constexpr int R = rows(8), RF = rows(NV > 1 && sizeof(T) == 2 ? 16 : 8);        // value rows in flight: backward, forward
-    static constexpr int SUB = MODE == kAny ? 1 : 4, PARTS = 4 / SUB;
-    static constexpr int kPart = MODE == kAny ? 2048 : 1024;       // floats of the partial-sum buffer
+    static constexpr int kPart = 256 * NA;                                   // floats of the partial-sum buffer
     const Args& P;
-    int lane, wave, H, K, D, HK, HD, qa, qv, sub_a, n_sub_a;
+    int lane, wave, H, K, D, HK, HD, per_a, qa, qv;                          // (per_a: feature quads of a head)
     int begin_v[NV], head_v[NV];                                             // of the lane's value quads (the last one where it has none): first element, its head
-    uint32_t inv_h, inv_qa, inv_head;
+    uint32_t inv_h, inv_qa, inv_per_a;
     int64_t e0, e1;
     float* part; double* t; float* keep; const float* w; const float* bounds; const float* table;
     uint64_t seed, offset;
@@ -145,11 +146,9 @@ template <class T, int MODE, int NV, int GA> struct Wave {
     __device__ Wave(const Args& p, char* lds, size_t own_bytes) : P(p) {
         lane = threadIdx.x & 63; wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);          // (known to be uniform: row addresses stay scalar)
         H = p.heads; K = p.k; D = p.d; HK = H * K; HD = H * D;
-        qa = row_quads(MODE, H, K); qv = row_quads(MODE, H, D);
-        sub_a = MODE == kAny && (K & 3) ? 1 : 4; n_sub_a = sub_a == 1 ? K : (K + 3) >> 2;
-        inv_h = (65536 + H - 1) / H; inv_qa = (65536 + qa - 1) / qa; inv_head = (65536 + n_sub_a - 1) / n_sub_a;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) begin_v[j] = quad_start<MODE>(min(j * 64 + lane, qv - 1), H, D, head_v[j]);
+        per_a = (K + 3) >> 2; qa = row_quads(H, K); qv = row_quads(H, D);
+        inv_h = (65536 + H - 1) / H; inv_qa = (65536 + qa - 1) / qa; inv_per_a = (65536 + per_a - 1) / per_a;
+        value_places(P, lane, begin_v, head_v);
         float* s = (float*)lds;          // (filled by stage())
         const int hk4 = 4 * qa, B = p.n_buckets;
         w = s; bounds = s + hk4; table = s + hk4 + B;
@@ -165,7 +164,7 @@ template <class T, int MODE, int NV, int GA> struct Wave {
     __device__ void stage(char* lds) const {
         float* s = (float*)lds;
         const int hk4 = 4 * qa, B = P.n_buckets;
-        for (int i = threadIdx.x; i < hk4; i += blockDim.x) { int h; const int c = begin_a(i >> 2, h) + (i & 3); s[i] = c < HK ? P.w[c] : 0.0f; }
+        for (int i = threadIdx.x; i < hk4; i += blockDim.x) { int h; const int c = begin_a(i >> 2, h) + (i & 3); s[i] = (i & 3) < K ? P.w[c] : 0.0f; }
         for (int i = threadIdx.x; i < B - 1; i += blockDim.x) s[hk4 + i] = P.bounds[i];
         for (int i = threadIdx.x; i < B * H; i += blockDim.x) s[hk4 + B + i] = P.table[i];
         __syncthreads();
@@ -188,9 +187,8 @@ template <class T, int MODE, int NV, int GA> struct Wave {
     }
     // first element of feature quad q and its head
     __device__ int begin_a(int q, int& h) const {
-        if (MODE == kAny || MODE == kAligned) { h = MODE == kAny ? 0 : (int)((q * inv_head) >> 16); return 4 * q; }
-        h = (int)((q * inv_head) >> 16);
-        return h * K + min(4 * (q - h * n_sub_a), K - 4);
+        h = (int)((q * inv_per_a) >> 16);
+        return MODE == kAligned ? 4 * q : h * K + quad_begin(q - h * per_a, K);
     }
     // feature quad i of the edges e_first .. e_first + GA - 1: its edge (relative to e_first) and quad; false if there is none
     __device__ bool a_place(int i, int e_first, int& e, int& q) const {
@@ -206,14 +204,16 @@ template <class T, int MODE, int NV, int GA> struct Wave {
         for (int i = 0; i < NA; ++i) {
             int h;
             const int idx = i * 64 + lane, e = (int)((idx * inv_qa) >> 16), q = idx - e * qa, c = begin_a(q, h);
-            a[i] = load_quad<T, MODE>((const T*)P.a + (base + min(e_first + e, n - 1)) * P.a_stride + c, HK - c);
+            const T* p = (const T*)P.a + (base + min(e_first + e, n - 1)) * P.a_stride + c;
+            if (MODE == kAligned) a[i] = load_quad<T, kAligned>(p, 4);
+            else a[i] = K < 4 ? load_quad<T, kElements>(p, K) : load_quad<T, kHeads>(p, 4);
         }
     }
     // the lane's quads of a row of H D elements
     __device__ void load_row(Raw (&v)[NV], const T* row) const {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            v[j] = load_quad<T, MODE>(row + begin_v[j], HD - begin_v[j]);
+            v[j] = load_quad<T, MODE>(row + begin_v[j], D);
         }
     }
     __device__ const T* value_row(int64_t e) const { return (const T*)P.v + min(e, e1 - 1) * P.v_stride; }
@@ -223,30 +223,27 @@ template <class T, int MODE, int NV, int GA> struct Wave {
         const uint32_t lo = h & 1 ? x.w[1] : x.w[0], hi = h & 1 ? x.w[3] : x.w[2];
         return (h & 2 ? hi : lo) >= P.threshold ? P.keep_scale : 0.0f;
     }
-    // sums over a quad (or single products) of act(a) w for the edges e_first .. e_first + GA - 1, into LDS
+    // sums over a quad of act(a) w for the edges e_first .. e_first + GA - 1, into LDS
     __device__ void partial_logits(const Raw (&a)[NA], int e_first) {
-        const int subs = sub_a == 4 ? qa : 4 * qa;
         wave_sync();
 #pragma unroll
         for (int i = 0; i < NA; ++i) {
-            int e, q;
+            int e, q, h;
             if (!a_place(i, e_first, e, q)) continue;
             const f4 wq = *(const f4*)(w + 4 * q);
             f4 x;
-            int h;
-            const int c = begin_a(q, h), shared = quad_shared<MODE>(c, h, K);
+            const int begin = begin_a(q, h), shared = MODE == kAligned ? 0 : quad_shared(begin - h * K);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = j < shared ? 0.0f : act((float)a[i][j]);          // (0 where the row has no such element)
-            if (sub_a == 4) part[e * subs + q] = fmaf(x[3], wq[3], fmaf(x[2], wq[2], fmaf(x[1], wq[1], x[0] * wq[0])));
-            else *(f4*)(part + e * subs + 4 * q) = x * wq;
+            for (int j = 0; j < 4; ++j) x[j] = j < shared ? 0.0f : act((float)a[i][j]);          // (0 where the head has no such element)
+            part[e * qa + q] = fmaf(x[3], wq[3], fmaf(x[2], wq[2], fmaf(x[1], wq[1], x[0] * wq[0])));
         }
         wave_sync();
     }
     // t of edge e_first + e and head h
     __device__ double logit(int e_first, int e, int h) const {
-        const int subs = sub_a == 4 ? qa : 4 * qa, eb = e_first + e;
+        const int eb = e_first + e;
         float s = 0.0f;
-        for (int i = 0; i < n_sub_a; ++i) s += part[e * subs + h * n_sub_a + i];
+        for (int i = 0; i < per_a; ++i) s += part[e * qa + h * per_a + i];
         const float l = e_logit[eb];
         double x = (double)s + (double)l;
         if (P.n_buckets) { const float b = table[e_bucket[eb] * H + h]; x = b == -__builtin_inff() ? (double)b : x + (double)b; }
@@ -260,11 +257,11 @@ template <int CTRL> __device__ inline float ror(float x) { return __builtin_bit_
 
 // ---- forward --------------------------------------------------------------------------------------------------------------------------------
 
-// running softmax of one row in a lane: its quads' weighted sums, and a maximum and sum for each head that the quads touch
-template <int NV, int PARTS> struct Row {
-    f4 acc[NV]; double m[NV][PARTS]; float sum[NV][PARTS];
+// running softmax of one row in a lane: its quads' weighted sums, and a maximum and sum for the head of each
+template <int NV> struct Row {
+    f4 acc[NV]; double m[NV]; float sum[NV];
     __device__ void clear() {
-        for (int j = 0; j < NV; ++j) { acc[j] = f4{0, 0, 0, 0}; for (int p = 0; p < PARTS; ++p) { m[j][p] = -__builtin_inf(); sum[j][p] = 0.0f; } }
+        for (int j = 0; j < NV; ++j) { acc[j] = f4{0, 0, 0, 0}; m[j] = -__builtin_inf(); sum[j] = 0.0f; }
     }
     // a sum relative to x comes in (x = -inf: an empty one): factors of the old sum and of the new one
     __device__ static void weights(double& m, double x, float& w_old, float& w_new) {
@@ -274,36 +271,22 @@ template <int NV, int PARTS> struct Row {
     }
 };
 
-// Record of a row that crosses ranges, for each lane of the walk: [NV] quads, then per part a 64-bit maximum and a sum.  Slot 0 of a wave holds its
-// first row, slot 1 its last one.
-template <int NV, int PARTS> struct Record { f4 acc[NV]; double m[NV][PARTS]; float sum[NV][PARTS]; };
+// Record of a row that crosses ranges, for each lane of the walk: [NV] quads, a 64-bit maximum and a sum for each.  Slot 0 of a wave holds its first row, slot 1
+// its last one.
+template <int NV> struct Record { f4 acc[NV]; double m[NV]; float sum[NV]; };
 
-// begin_v, head: first element of each of the lane's quads, head of each of their parts
-template <class T, int MODE, int NV, int PARTS> __device__ inline void
-finish_row(const Args& P, int row, const Row<NV, PARTS>& r, int lane, int qv, const int (&begin_v)[NV], const int (&head)[NV][PARTS], T* out, float* out32, double* norm) {
-    constexpr int SUB = 4 / PARTS;
+template <class T, int MODE, int NV> __device__ inline void
+finish_row(const Args& P, int row, const Row<NV>& r, int lane, int qv, const int (&begin_v)[NV], const int (&head_v)[NV], T* out, float* out32, double* norm) {
     const int HD = P.heads * P.d;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         if (j * 64 + lane >= qv) continue;
-        f4 o;
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
-            const float inv = r.sum[j][p] == 0.0f ? 0.0f : 1.0f / r.sum[j][p];          // (no edge takes part: 0)
-#pragma unroll
-            for (int i = 0; i < SUB; ++i) o[p * SUB + i] = r.acc[j][p * SUB + i] * inv;
-            if (norm && begin_v[j] + p * SUB == head[j][p] * P.d) *(d2*)(norm + 2 * ((int64_t)row * P.heads + head[j][p])) = d2{r.m[j][p], (double)inv};
-        }
-        store_quad<T, MODE>(out + (int64_t)row * HD + begin_v[j], o, HD - begin_v[j]);
-        if (out32) store_quad<float, MODE>(out32 + (int64_t)row * HD + begin_v[j], o, HD - begin_v[j]);
+        const float inv = r.sum[j] == 0.0f ? 0.0f : 1.0f / r.sum[j];          // (no edge takes part: 0)
+        const f4 o = {r.acc[j][0] * inv, r.acc[j][1] * inv, r.acc[j][2] * inv, r.acc[j][3] * inv};
+        if (norm && begin_v[j] == head_v[j] * P.d) *(d2*)(norm + 2 * ((int64_t)row * P.heads + head_v[j])) = d2{r.m[j], (double)inv};
+        store_quad<T, MODE>(out + (int64_t)row * HD + begin_v[j], o, P.d);
+        if (out32) store_quad<float, MODE>(out32 + (int64_t)row * HD + begin_v[j], o, P.d);
     }
-}
-// head of each part of the lane's quads
-template <int NV, int PARTS> __device__ inline void part_heads(const Args& P, const int (&begin_v)[NV], const int (&head_v)[NV], int (&head)[NV][PARTS]) {
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) head[j][p] = PARTS == 1 ? head_v[j] : min((begin_v[j] + p) / P.d, P.heads - 1);
 }
 
 // Read of the per-edge rows once; bandwidth bounds it, in 16 bits nearly as much the 46 vector instructions of an edge.  1.97 M edges of 64 + 240 channels:
@@ -311,10 +294,9 @@ template <int NV, int PARTS> __device__ inline void part_heads(const Args& P, co
 // loaded it and finished by one lane for each edge and head, which also draws the dropout word: the walk then needs one share per edge and lane.  (Running
 // maxima per edge and lane instead: 0.69 ms in float16.)  At lmax 3 (296 channels, 76 quads) a lane holds two quads, the second one mostly idle: 0.13 ms for
 // 499 979 edges, 2.7 TB/s, bound by instructions and by what 8 waves of a CU have in flight.
-template <class T, int MODE, int NV, int GA> __global__ __launch_bounds__(256, forward_waves(MODE, NV, sizeof(T)))
+template <class T, int MODE, int NV, int GA> __global__ __launch_bounds__(256, forward_waves(NV, sizeof(T)))
 void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, int64_t* rng_used) {
     typedef Wave<T, MODE, NV, GA> W;
-    constexpr int PARTS = W::PARTS, SUB = W::SUB;
     extern __shared__ __align__(16) char lds[];
     if (rng_used && P.threshold && blockIdx.x == 0 && threadIdx.x < 2) rng_used[threadIdx.x] = P.rng[threadIdx.x];
     const int edge_blocks = (P.n_waves + kWaves - 1) / kWaves;
@@ -334,8 +316,6 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
     W w(P, lds, W::wave_bytes(P.heads) + (size_t)kBatch * P.heads * 8);
     if (w.e0 >= w.e1) { w.stage(lds); return; }
     const int lane = w.lane, H = w.H, qv = w.qv;
-    int head[NV][PARTS];
-    part_heads(P, w.begin_v, w.head_v, head);
     // R value rows are always in flight: a row's registers are loaded again, R edges ahead, as soon as it has been added
     constexpr int R = W::RF;
     typename W::Edge edge = w.request(w.e0);
@@ -345,18 +325,18 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
     for (int i = 0; i < R; ++i) w.load_row(v[i], w.value_row(w.e0 + i));
     const int before = P.dst[max(w.e0 - 1, (int64_t)0)], behind = P.dst[min(w.e1, P.n_edges - 1)];
     w.stage(lds);
-    Row<NV, PARTS> r;
+    Row<NV> r;
     r.clear();
     int cur = __builtin_amdgcn_readfirstlane(edge.dst);
     const bool open_front = w.e0 > 0 && before == cur;
     bool first_row = true;
-    Record<NV, PARTS>* rec = (Record<NV, PARTS>*)records + ((int64_t)blockIdx.x * kWaves + w.wave) * 2 * 64 + lane;
+    Record<NV>* rec = (Record<NV>*)records + ((int64_t)blockIdx.x * kWaves + w.wave) * 2 * 64 + lane;
     auto flush = [&](bool open_back) {
         if ((first_row && open_front) || open_back) {
-            Record<NV, PARTS> x;
-            for (int j = 0; j < NV; ++j) { x.acc[j] = r.acc[j]; for (int p = 0; p < PARTS; ++p) { x.m[j][p] = r.m[j][p]; x.sum[j][p] = r.sum[j][p]; } }
+            Record<NV> x;
+            for (int j = 0; j < NV; ++j) { x.acc[j] = r.acc[j]; x.m[j] = r.m[j]; x.sum[j] = r.sum[j]; }
             rec[first_row ? 0 : 64] = x;
-        } else finish_row<T, MODE>(P, cur, r, lane, qv, w.begin_v, head, out, out32, norm);
+        } else finish_row<T, MODE>(P, cur, r, lane, qv, w.begin_v, w.head_v, out, out32, norm);
     };
     float2* share = (float2*)w.keep;                       // [16][H] share of the piece, and that share times the dropout factor
     double* top = (double*)(w.e_bucket + kBatch);          // [16][H] logit that the shares are relative to
@@ -419,7 +399,7 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
                 }
                 wave_sync();
             }
-            float scale[NV][PARTS];
+            float scale[NV];
 #pragma unroll 1
             for (int s = 0; s < GA; s += R)
 #pragma unroll
@@ -430,31 +410,27 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
                         const int d = __builtin_amdgcn_readfirstlane(w.e_dst[g + e]);
                         if (d != cur) { flush(false); cur = d; first_row = false; r.clear(); }
 #pragma unroll
-                        for (int j = 0; j < NV; ++j)
+                        for (int j = 0; j < NV; ++j) {
+                            float w_old;
+                            Row<NV>::weights(r.m[j], top[(g + e) * H + w.head_v[j]], w_old, scale[j]);
+                            r.sum[j] *= w_old;
 #pragma unroll
-                            for (int p = 0; p < PARTS; ++p) {
-                                float w_old;
-                                Row<NV, PARTS>::weights(r.m[j][p], top[(g + e) * H + head[j][p]], w_old, scale[j][p]);
-                                r.sum[j][p] *= w_old;
-#pragma unroll
-                                for (int c = 0; c < SUB; ++c) r.acc[j][p * SUB + c] *= w_old;
-                            }
+                            for (int c = 0; c < 4; ++c) r.acc[j][c] *= w_old;
+                        }
                     }
                     if (GA != 16 || (some >> ((4 * e) & 63)) & 1)
 #pragma unroll
-                    for (int j = 0; j < NV; ++j)
+                    for (int j = 0; j < NV; ++j) {
+                        const float2 f = share[(g + e) * H + w.head_v[j]];
+                        const float k = f.y * scale[j];
+                        r.sum[j] = fmaf(f.x, scale[j], r.sum[j]);
 #pragma unroll
-                        for (int p = 0; p < PARTS; ++p) {
-                            const float2 f = share[(g + e) * H + head[j][p]];
-                            const float k = f.y * scale[j][p];
-                            r.sum[j][p] = fmaf(f.x, scale[j][p], r.sum[j][p]);
-#pragma unroll
-                            for (int c = 0; c < SUB; ++c) {
-                                // (what a head does not look at may be NaN)
-                                const float x = select && f.x == 0.0f ? 0.0f : (float)v[i][j][p * SUB + c];
-                                r.acc[j][p * SUB + c] = fmaf(k, x, r.acc[j][p * SUB + c]);
-                            }
+                        for (int c = 0; c < 4; ++c) {
+                            // (what a head does not look at may be NaN)
+                            const float x = select && f.x == 0.0f ? 0.0f : (float)v[i][j][c];
+                            r.acc[j][c] = fmaf(k, x, r.acc[j][c]);
                         }
+                    }
                 }
                 w.load_row(v[i], w.value_row(base + g + e + R));
             }
@@ -469,35 +445,30 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
 template <int NV> constexpr int merge_waves() { return 16 / NV; }
 template <class T, int MODE, int NV> __global__ __launch_bounds__(1024 / NV)
 void k_attn_merge(Args P, T* out, float* out32, double* norm, const void* records) {
-    constexpr int SUB = MODE == kAny ? 1 : 4, PARTS = 4 / SUB, WAVES = merge_waves<NV>();
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), qv = row_quads(MODE, P.heads, P.d);
-    int begin_v[NV], head_v[NV], head[NV][PARTS];
-#pragma unroll
-    for (int j = 0; j < NV; ++j) begin_v[j] = quad_start<MODE>(min(j * 64 + lane, qv - 1), P.heads, P.d, head_v[j]);
-    part_heads(P, begin_v, head_v, head);
-    __shared__ Record<NV, PARTS> share[WAVES - 1][64];
+    constexpr int WAVES = merge_waves<NV>();
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), qv = row_quads(P.heads, P.d);
+    int begin_v[NV], head_v[NV];
+    value_places(P, lane, begin_v, head_v);
+    __shared__ Record<NV> share[WAVES - 1][64];
     __shared__ int long_row[WAVES], long_first[WAVES];
-    const Record<NV, PARTS>* rec = (const Record<NV, PARTS>*)records + lane;
-    Row<NV, PARTS> r;
-    auto join = [&](const f4 (&acc)[NV], const double (&m)[NV][PARTS], const float (&sum)[NV][PARTS]) {
+    const Record<NV>* rec = (const Record<NV>*)records + lane;
+    Row<NV> r;
+    auto join = [&](const f4 (&acc)[NV], const double (&m)[NV], const float (&sum)[NV]) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j) {
+            float w_old, w_new;
+            Row<NV>::weights(r.m[j], m[j], w_old, w_new);
+            r.sum[j] = fmaf(sum[j], w_new, r.sum[j] * w_old);
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p) {
-                float w_old, w_new;
-                Row<NV, PARTS>::weights(r.m[j][p], m[j][p], w_old, w_new);
-                r.sum[j][p] = fmaf(sum[j][p], w_new, r.sum[j][p] * w_old);
-#pragma unroll
-                for (int i = 0; i < SUB; ++i) r.acc[j][p * SUB + i] = fmaf(acc[j][p * SUB + i], w_new, r.acc[j][p * SUB + i] * w_old);
-            }
+            for (int i = 0; i < 4; ++i) r.acc[j][i] = fmaf(acc[j][i], w_new, r.acc[j][i] * w_old);
+        }
     };
     // records first, first + step, .. <= last of a row that begins at edge `begin`, in range w0
     auto join_records = [&](int64_t w0, int64_t begin, int64_t first, int64_t last, int step) {
         r.clear();
-        constexpr int AHEAD = PARTS == 1 ? 4 : 1;
-#pragma unroll AHEAD
+#pragma unroll 4
         for (int64_t x = first; x <= last; x += step) {
-            const Record<NV, PARTS> o = rec[(x * 2 + (x == w0 && begin > w0 * P.range ? 1 : 0)) * 64];
+            const Record<NV> o = rec[(x * 2 + (x == w0 && begin > w0 * P.range ? 1 : 0)) * 64];
             join(o.acc, o.m, o.sum);
         }
     };
@@ -508,7 +479,7 @@ void k_attn_merge(Args P, T* out, float* out32, double* norm, const void* record
         if (P.dst[border - 1] == row) {
             const int64_t begin = P.rowptr[row], last = ((int64_t)P.rowptr[row + 1] - 1) / P.range;
             if (begin >= mine * P.range) {                              // (else an earlier border is its first)
-                if (last - mine < 8) { join_records(mine, begin, mine, last, 1); finish_row<T, MODE>(P, row, r, lane, qv, begin_v, head, out, out32, norm); }
+                if (last - mine < 8) { join_records(mine, begin, mine, last, 1); finish_row<T, MODE>(P, row, r, lane, qv, begin_v, head_v, out, out32, norm); }
                 else if (lane == 0) { long_row[wave] = row; long_first[wave] = (int)mine; }
             }
         }
@@ -520,13 +491,13 @@ void k_attn_merge(Args P, T* out, float* out32, double* norm, const void* record
         const int64_t w0 = long_first[i], begin = P.rowptr[row], last = ((int64_t)P.rowptr[row + 1] - 1) / P.range;
         join_records(w0, begin, w0 + wave, last, WAVES);
         if (wave > 0) {
-            Record<NV, PARTS>& o = share[wave - 1][lane];
-            for (int j = 0; j < NV; ++j) { o.acc[j] = r.acc[j]; for (int p = 0; p < PARTS; ++p) { o.m[j][p] = r.m[j][p]; o.sum[j][p] = r.sum[j][p]; } }
+            Record<NV>& o = share[wave - 1][lane];
+            for (int j = 0; j < NV; ++j) { o.acc[j] = r.acc[j]; o.m[j] = r.m[j]; o.sum[j] = r.sum[j]; }
         }
         __syncthreads();
         if (wave == 0) {
             for (int o = 0; o < WAVES - 1; ++o) join(share[o][lane].acc, share[o][lane].m, share[o][lane].sum);
-            finish_row<T, MODE>(P, row, r, lane, qv, begin_v, head, out, out32, norm);
+            finish_row<T, MODE>(P, row, r, lane, qv, begin_v, head_v, out, out32, norm);
         }
         __syncthreads();
     }
@@ -560,35 +531,33 @@ struct BackArgs {
 // lasts, so nothing waits where rows are short.  1.97 M edges of 64 + 240 float32 channels: 1.02 ms, 4.8 TB/s, the rate of a large copy; 499 979 bfloat16 edges
 // of lmax 3 0.25 ms, 2.9 TB/s, bound by the latency that three waves a SIMD cover.  The dot of a value row with dout goes through LDS (a partial sum for each
 // quad part), since a head's quads are not a power of two of lanes.
-template <class T, int MODE, int NV, int GA> __global__ __launch_bounds__(256, backward_waves(MODE, NV, sizeof(T)))
+template <class T, int MODE, int NV, int GA> __global__ __launch_bounds__(256, backward_waves(NV, sizeof(T)))
 void k_attn_backward(Args P, BackArgs B) {
     typedef Wave<T, MODE, NV, GA> W;
-    constexpr int NA = W::NA, PARTS = W::PARTS, SUB = W::SUB, R = W::R;
+    constexpr int NA = W::NA, R = W::R;
     extern __shared__ __align__(16) char lds[];
     const int BH = P.n_buckets * P.heads;
     const size_t own = W::wave_bytes(P.heads) + (size_t)kBatch * P.heads * 4 + (size_t)((BH + 1) & ~1) * 4;
     W w(P, lds, (own + 15) & ~(size_t)15);
-    const int lane = w.lane, H = w.H, HD = w.HD, HK = w.HK, qv = w.qv, subs = qv * PARTS, per_head = MODE == kAny ? P.d : (P.d + 3) >> 2;
+    const int lane = w.lane, H = w.H, HD = w.HD, HK = w.HK, qv = w.qv, per_head = (P.d + 3) >> 2;
     float2* share = (float2*)w.keep;                    // [16][H] probability and dropout factor
     float* weight = (float*)w.t;                        // [16][H] their product
     float* dt = (float*)(w.e_bucket + kBatch);          // [16][H]
     float* bins = dt + kBatch * H;                      // [buckets][H]
     for (int i = lane; i < BH; i += 64) bins[i] = 0.0f;
-    int head[NV][PARTS];
-    part_heads(P, w.begin_v, w.head_v, head);
     int shared_v[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) shared_v[j] = quad_shared<MODE>(w.begin_v[j], w.head_v[j], P.d);
+    for (int j = 0; j < NV; ++j) shared_v[j] = quad_shared(w.begin_v[j] - w.head_v[j] * P.d);
     int lanes = 0;          // 2^lanes lanes sum the dot of an edge and head
     while (lanes < 3 && (2 * R * H << lanes) <= 64) ++lanes;
     f4 dw[NA];
-    int head_a[NA];          // of the lane's feature quads, where a quad lies inside one head
+    int head_a[NA];          // of the lane's feature quads
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
         int e, q;
         w.a_place(i, 0, e, q);
         dw[i] = f4{0, 0, 0, 0};
-        head_a[i] = min(MODE == kAny ? 4 * q / P.k : (int)((q * w.inv_head) >> 16), H - 1);
+        w.begin_a(q, head_a[i]);
     }
 
     if (w.e0 >= w.e1) w.stage(lds);
@@ -638,24 +607,18 @@ void k_attn_backward(Args P, BackArgs B) {
 #pragma unroll
                             for (int j = 0; j < NV; ++j) {
                                 const int q = j * 64 + lane;
+                                const float f = weight[(s + i) * H + w.head_v[j]];
                                 f4 o;
-                                float dot[PARTS];
+                                float dot = 0.0f;
 #pragma unroll
-                                for (int p = 0; p < PARTS; ++p) {
-                                    const float f = weight[(s + i) * H + head[j][p]];
-                                    dot[p] = 0.0f;
-#pragma unroll
-                                    for (int k = 0; k < SUB; ++k) {
-                                        const int c = p * SUB + k;
-                                        o[c] = f * (float)up[i][j][c];
-                                        dot[p] = fmaf((float)v[i][j][c], (float)up[i][j][c], dot[p]);
-                                        if (MODE == kHeads && c < 3) dot[p] = c < shared_v[j] ? 0.0f : dot[p];
-                                    }
+                                for (int c = 0; c < 4; ++c) {
+                                    o[c] = f * (float)up[i][j][c];
+                                    dot = fmaf((float)v[i][j][c], (float)up[i][j][c], dot);
+                                    if (MODE == kHeads && c < 3) dot = c < shared_v[j] ? 0.0f : dot;
                                 }
                                 if (q < qv) {
-#pragma unroll
-                                    for (int p = 0; p < PARTS; ++p) w.part[i * subs + q * PARTS + p] = dot[p];
-                                    if (B.dv) store_quad<T, MODE>((T*)B.dv + (base + s + i) * HD + w.begin_v[j], o, HD - w.begin_v[j]);
+                                    w.part[i * qv + q] = dot;
+                                    if (B.dv) store_quad<T, MODE>((T*)B.dv + (base + s + i) * HD + w.begin_v[j], o, P.d);
                                 }
                             }
                         }
@@ -673,7 +636,7 @@ void k_attn_backward(Args P, BackArgs B) {
                     for (int k = lane >> lanes; k < last * H; k += 64 >> lanes) {
                         const int i = (int)((k * w.inv_h) >> 16), h = k - i * H, l = lane & ((1 << lanes) - 1);
                         float dot = 0.0f;
-                        for (int c = l; c < per_head; c += 1 << lanes) dot += w.part[i * subs + h * per_head + c];
+                        for (int c = l; c < per_head; c += 1 << lanes) dot += w.part[i * qv + h * per_head + c];
                         if (lanes > 0) dot += ror<0xB1>(dot);
                         if (lanes > 1) dot += ror<0x4E>(dot);
                         if (lanes > 2) dot += ror<0x141>(dot);
@@ -691,18 +654,23 @@ void k_attn_backward(Args P, BackArgs B) {
                     int e, q;
                     if (!w.a_place(i, g, e, q)) continue;
                     const f4 wq = *(const f4*)(w.w + 4 * q);
+                    const float f = dt[(g + e) * H + head_a[i]];
                     f4 o;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const int h = w.sub_a == 4 ? head_a[i] : min((4 * q + j) / P.k, H - 1);
-                        const float f = dt[(g + e) * H + h], x = (float)a[i][j], sg = sigmoid(x);
+                        const float x = (float)a[i][j], sg = sigmoid(x);
                         const float slope = kActNorm * fmaf(0.8f * sg, fmaf(x, 1.0f - sg, 1.0f), 0.2f);
                         o[j] = f == 0.0f ? 0.0f : f * wq[j] * slope;
                         dw[i][j] = f == 0.0f ? dw[i][j] : fmaf(f, kActNorm * x * fmaf(0.8f, sg, 0.2f), dw[i][j]);
                     }
                     int h;
                     const int c = w.begin_a(q, h);
-                    if (B.da) store_quad<T, MODE>((T*)B.da + (base + g + e) * HK + c, o, HK - c);
+                    if (B.da) {
+                        T* p = (T*)B.da + (base + g + e) * HK + c;
+                        if (MODE == kAligned) store_quad<T, kAligned>(p, o, 4);
+                        else if (P.k < 4) store_quad<T, kElements>(p, o, P.k);
+                        else store_quad<T, kHeads>(p, o, 4);
+                    }
                 }
                 if (BH && B.param_rows && lane < H)          // in the edges' order: lane h alone adds to the sums of its head
                     for (int e = 0; e < GA && g + e < w.n; ++e) bins[w.e_bucket[g + e] * H + lane] += dt[(g + e) * H + lane];
@@ -720,7 +688,7 @@ void k_attn_backward(Args P, BackArgs B) {
     const size_t stride = (own + 15) & ~(size_t)15;
     for (int c = threadIdx.x; c < HK; c += 256) {
         int at = c;          // its place among the feature quads' elements
-        if (MODE == kHeads) { const int h = c / P.k, x = c - h * P.k; at = 4 * (h * w.n_sub_a + (x >> 2)) + x - min(x & ~3, P.k - 4); }
+        if (MODE != kAligned) { const int h = c / P.k, x = c - h * P.k; at = 4 * (h * w.per_a + (x >> 2)) + x - quad_begin(x >> 2, P.k); }
         float s = 0.0f;
         for (int x = 0; x < kWaves; ++x) {
             const float* part = (const float*)((const char*)w.part + ((ptrdiff_t)x - w.wave) * (ptrdiff_t)stride);

@@ -38,12 +38,15 @@ struct Backward {
 };
 
 template <class T, int MODE, class F> int by_width(int nv, int ga, F& f) {
+    if constexpr (MODE == kHeads) if (ga == 2) return f.template run<T, MODE, 4, 2>();          // (aligned features have at most 64 quads)
     if (nv == 4) return f.template run<T, MODE, 4, 4>();
     if (nv == 2) return ga == 16 ? f.template run<T, MODE, 2, 16>() : ga == 8 ? f.template run<T, MODE, 2, 8>() : f.template run<T, MODE, 2, 4>();
     return ga == 16 ? f.template run<T, MODE, 1, 16>() : f.template run<T, MODE, 1, 8>();
 }
 template <class T, class F> int launch(int mode, int nv, int ga, F f) {
-    return mode == kAligned ? by_width<T, kAligned>(nv, ga, f) : mode == kHeads ? by_width<T, kHeads>(nv, ga, f) : by_width<T, kAny>(nv, ga, f);
+    if (mode != kElements) return mode == kAligned ? by_width<T, kAligned>(nv, ga, f) : by_width<T, kHeads>(nv, ga, f);
+    if (ga == 2) return f.template run<T, kElements, 4, 2>();          // (at most 16 value quads)
+    return ga == 16 ? f.template run<T, kElements, 1, 16>() : ga == 8 ? f.template run<T, kElements, 1, 8>() : f.template run<T, kElements, 2, 4>();
 }
 
 #define DEDF_LAUNCHES(T, PREFIX) PREFIX template int launch<T, Forward>(int, int, int, Forward); PREFIX template int launch<T, Backward>(int, int, int, Backward);
@@ -76,7 +79,7 @@ bool whole_quads(const void* p, int64_t stride, int type) {
 int make_plan(const dedf_edge_attn* x, bool backward, Plan& p, std::initializer_list<const void*> tensors) {
     if (!x || x->n_edges < 0 || x->n_dst < 0 || x->heads < 1 || x->k < 1 || x->d < 1 || x->n_buckets < 0) return DEDF_ERR_INVALID;
     if (x->type != DEDF_F32 && x->type != DEDF_F16 && x->type != DEDF_BF16) return DEDF_ERR_UNSUPPORTED;
-    if (x->n_edges >= (int64_t)1 << 31 || x->heads > 16 || x->k > 256 || x->d > 1024 || x->heads * x->k > 256 || x->heads * x->d > 1024) return DEDF_ERR_UNSUPPORTED;
+    if (x->n_edges >= (int64_t)1 << 31 || x->heads > 16 || x->k > 256 || x->d > 1024 || x->heads * x->k > 256 || row_quads(x->heads, x->d) > 256) return DEDF_ERR_UNSUPPORTED;
     if (x->n_buckets > 1024 || x->n_buckets * x->heads > 2048) return DEDF_ERR_UNSUPPORTED;
     if (x->n_edges > 0 && (!x->alpha || !x->value || !x->alpha_dot || !x->dst)) return DEDF_ERR_INVALID;
     if (x->n_dst > 0 && !x->rowptr) return DEDF_ERR_INVALID;
@@ -94,19 +97,18 @@ int make_plan(const dedf_edge_attn* x, bool backward, Plan& p, std::initializer_
     a.keep_scale = (float)(1.0 / (1.0 - x->dropout)); a.rng = x->rng;
     bool whole = a.k % 4 == 0 && a.d % 4 == 0 && whole_quads(a.a, a.a_stride, x->type) && whole_quads(a.v, a.v_stride, x->type);
     for (const void* t : tensors) whole = whole && whole_quads(t, 0, x->type);
-    p.mode = whole ? kAligned : a.k >= 4 && a.d >= 4 && row_quads(kHeads, a.heads, a.k) <= 64 && row_quads(kHeads, a.heads, a.d) <= 256 ? kHeads : kAny;
-    const int qa = row_quads(p.mode, a.heads, a.k), qv = row_quads(p.mode, a.heads, a.d);
-    p.ga = qv > 128 || qa > 32 ? 4 : qa > 16 ? 8 : 16;
-    p.nv = qv > 128 ? 4 : qv > 64 || p.ga == 4 ? 2 : 1;
-    const int bytes = (int)element(x->type), most = kSimds * (backward ? backward_waves(p.mode, p.nv, bytes) : forward_waves(p.mode, p.nv, bytes));
+    p.mode = whole ? kAligned : a.d >= 4 ? kHeads : kElements;
+    const int qa = row_quads(a.heads, a.k), qv = row_quads(a.heads, a.d);          // (qa <= 76: 16 heads, 256 channels)
+    p.ga = qa > 64 ? 2 : qv > 128 || qa > 32 ? 4 : qa > 16 ? 8 : 16;
+    p.nv = qv > 128 || p.ga == 2 ? 4 : qv > 64 || p.ga == 4 ? 2 : 1;
+    const int bytes = (int)element(x->type), most = kSimds * (backward ? backward_waves(p.nv, bytes) : forward_waves(p.nv, bytes));
     const int64_t even = (a.n_edges + most - 1) / most;
     a.range = (int)std::max<int64_t>(kBatch, (even + kBatch - 1) / kBatch * kBatch);
     a.n_waves = (int)((a.n_edges + a.range - 1) / a.range);
     p.blocks = (a.n_waves + kWaves - 1) / kWaves;
-    const int parts = p.mode == kAny ? 4 : 1;          // (as the kernels' Record<nv, parts>)
-    p.record = (size_t)(p.nv * 16 + p.nv * parts * 12 + 15) / 16 * 16 * 64 * 2;
-    static_assert(sizeof(Record<1, 1>) == 32 && sizeof(Record<1, 4>) == 64 && sizeof(Record<2, 1>) == 64 && sizeof(Record<4, 1>) == 112 && sizeof(Record<2, 4>) == 128 && sizeof(Record<4, 4>) == 256, "records are as large as computed here");
-    const size_t own = p.mode == kAny ? Wave<float, kAny, 1, 16>::wave_bytes(a.heads) : Wave<float, kAligned, 1, 16>::wave_bytes(a.heads);          // (whatever the type and width)
+    p.record = (size_t)(p.nv * 28 + 15) / 16 * 16 * 64 * 2;
+    static_assert(sizeof(Record<1>) == 32 && sizeof(Record<2>) == 64 && sizeof(Record<4>) == 112, "records are as large as computed here");
+    const size_t own = Wave<float, kAligned, 1, 16>::wave_bytes(a.heads);          // (whatever the type, mode and width)
     const int BH = a.n_buckets * a.heads;
     const size_t shared = Wave<float, kAligned, 1, 16>::shared_bytes(qa, a.heads, a.n_buckets);
     p.lds_forward = shared + kWaves * (own + (size_t)kBatch * a.heads * 8);
@@ -139,9 +141,7 @@ size_t dedf_edge_attention_scratch_bytes(const dedf_edge_attn* x, int backward) 
     Plan p;
     if (make_plan(x, backward != 0, p, {}) != DEDF_OK) return 0;
     if (backward) return backward_bytes(p);
-    // (outputs that are not aligned to whole quads choose another instantiation: room for either)
-    const size_t aligned = forward_bytes(p);
-    return make_plan(x, false, p, {reinterpret_cast<const void*>(1)}) == DEDF_OK ? std::max(aligned, forward_bytes(p)) : aligned;
+    return forward_bytes(p);
 }
 
 int dedf_edge_attention(const dedf_edge_attn* x, void* out, float* out_f, double* norm, int64_t* rng_used, void* scratch, size_t scratch_bytes, void* stream) {

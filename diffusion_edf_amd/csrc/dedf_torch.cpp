@@ -177,8 +177,8 @@ Tensor edge_attention(const Tensor& alpha, const Tensor& value, const Tensor& do
         TORCH_CHECK_VALUE(B == 1 || (bounds.defined() && has_shape(bounds, {B - 1}) && is_float(bounds)), "bias_boundaries: float32 (", B - 1, ",)");
         if (B == 1) bounds = Tensor();
     }
-    TORCH_CHECK_NOT_IMPLEMENTED(H <= 16 && H * K <= 256 && H * D <= 1024 && (!table.defined() || (table.size(0) <= 1024 && table.numel() <= 2048)),
-                                "at most 16 heads, 256 attention features and 1024 value channels an edge, 1024 buckets, 2048 bias entries");
+    TORCH_CHECK_NOT_IMPLEMENTED(H <= 16 && H * K <= 256 && H * ((D + 3) / 4) <= 256 && (!table.defined() || (table.size(0) <= 1024 && table.numel() <= 2048)),
+                                "at most 16 heads, 256 attention features and 1024 value channels an edge (head widths rounded up to multiples of 4), 1024 buckets, 2048 bias entries");
     check_dropout(p, rng, value);
     check_gpu("edge_attention", value, {alpha, dot, logits, length, bounds, table});
     TORCH_CHECK_VALUE(dst.device() == value.device(), "segments on ", dst.device(), ", the features on ", value.device());

@@ -310,7 +310,7 @@ int dedf_radius(const float* x_src, int n_src, const float* x_dst, int n_dst, fl
  *   t[e,h] = sum_k act(alpha[e,h,k]) alpha_dot[h,k] + edge_logits[e] + bias_table[b(edge_length[e]), h],   b(x) = number of boundaries <= x
  *   out[n,h,:] = sum over the edges of n of softmax(t)[e,h] keep[e,h] value[e,h,:]
  * An edge and head whose t is -inf, by its edge logit or its bucket's bias, takes no part, whatever alpha and value hold there; a row in which none does
- * is zero.  Limits: n_edges < 2^31, heads <= 16, heads k <= 256, heads d <= 1024, n_buckets <= 1024, heads n_buckets <= 2048. */
+ * is zero.  Limits: n_edges < 2^31, heads <= 16, heads k <= 256, heads ceil(d / 4) <= 256 (1024 channels, each head a whole number of quads), n_buckets <= 1024, heads n_buckets <= 2048. */
 typedef struct dedf_edge_attn {
     int64_t n_edges;
     int n_dst, heads, k, d, type;

@@ -91,6 +91,18 @@ def test_edge_attention_refusals():
             EdgeSegments(*args)
 
 
+def test_edge_attention_counts_value_channels_in_whole_quads(built_lib):
+    """3 heads of 341 are 258 quads, of 340 255"""
+    import ctypes as C
+    seg, lib = _segments_without_gpu(6, 3), built_lib
+    for D, fits in ((340, True), (341, False)):
+        with pytest.raises(RuntimeError if fits else NotImplementedError) as e:          # (that fits: only the device is wrong)
+            edge_attention(torch.zeros(6, 3, 8), torch.zeros(6, 3, D), torch.zeros(3, 8), seg)
+        assert fits == (not isinstance(e.value, NotImplementedError))
+        a = _lib.DedfEdgeAttn(type=0, n_edges=6, n_dst=3, heads=3, k=8, d=D, alpha=16, value=16, alpha_dot=16, dst=16, rowptr=16, alpha_stride=24, value_stride=3 * D)
+        assert (lib.dedf_edge_attention_scratch_bytes(C.byref(a), 0) > 0) == fits
+
+
 def test_row_operators_refusals():
     x, y = torch.randn(6, 240), torch.randn(6, 240)
     w, b = torch.ones(112), torch.zeros(64)
@@ -272,17 +284,17 @@ def test_edge_attention(dtype, N, E, kw):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("H,K,D", [
-    (8, 16, 30), (8, 17, 31), (8, 9, 65), (8, 16, 64), (16, 13, 13), (16, 4, 5), (16, 9, 64), (2, 128, 6), (1, 129, 130), (1, 61, 62), (1, 255, 1021), (3, 23, 341), (2, 7, 509),
-    (5, 51, 9), (13, 17, 4), (4, 4, 4), (5, 5, 5), (7, 6, 6), (1, 4, 7), (6, 3, 9), (6, 9, 3), (16, 2, 64), (8, 1, 20), (7, 3, 10), (2, 2, 12), (5, 1, 60), (16, 3, 4),
+    (8, 16, 30), (8, 17, 31), (8, 9, 65), (8, 16, 64), (16, 13, 13), (16, 4, 5), (16, 9, 64), (2, 128, 6), (1, 129, 130), (1, 61, 62), (1, 255, 1021), (3, 23, 340), (2, 7, 509),
+    (5, 51, 9), (13, 17, 4), (4, 4, 4), (5, 5, 5), (7, 6, 6), (1, 4, 7), (6, 3, 9), (6, 9, 3), (16, 2, 64), (15, 17, 65), (15, 17, 3), (9, 12, 1), (16, 16, 2), (8, 1, 20), (7, 3, 10), (2, 2, 12), (5, 1, 60), (16, 3, 4),
 ])
 def test_edge_attention_heads_of_any_width(dtype, H, K, D):
-    """head widths that are no multiples of 4 (each remainder, in features and values), widths below 4, feature rows of up to 16, 32 and 64 quads, value rows of
-    up to 64, 128 and 256, and rows that have more quads than that if each head has its own"""
+    """head widths that are no multiples of 4 (each remainder, in features and values), widths below 4, feature rows of up to 16, 32 and 75 quads, value rows of
+    up to 64, 128 and 256"""
     _check(_case(dtype, 11, 150, H=H, K=K, D=D, buckets=3, drop=0.15, seed=H * K))
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("H,K,D", [(3, 5, 7), (8, 17, 31), (3, 23, 341), (6, 3, 9), (1, 7, 13)])
+@pytest.mark.parametrize("H,K,D", [(3, 5, 7), (8, 17, 31), (3, 23, 337), (6, 3, 9), (5, 3, 2), (1, 7, 13)])
 def test_edge_attention_heads_of_any_width_across_ranges(H, K, D):
     g = torch.Generator().manual_seed(D)
     _check(_case(torch.float32, 3, 9_001, H=H, K=K, D=D, buckets=5, drop=0.0, dst=torch.randint(0, 3, (9_001,), generator=g).sort().values))
