@@ -252,7 +252,7 @@ template <class T, int MODE, int NV, int GA> struct Wave {
     }
 };
 
-// a value of another lane of the row of 16: rotations by 4 (0x124) and 8, the neighbour (0xB1), the other pair (0x4E), the mirrored half (0x141)
+// a value of another lane of the row of 16: rotations by 4 (0x124) and 8, the neighbour (0xB1), the other pair (0x4E), the mirrored half (0x141), the mirrored row (0x140)
 template <int CTRL> __device__ inline float ror(float x) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true)); }
 
 // ---- forward --------------------------------------------------------------------------------------------------------------------------------
@@ -269,11 +269,27 @@ template <int NV> struct Row {
         else if (x > m) { w_old = m == -__builtin_inf() ? 0.0f : exp_d(m - x); w_new = 1.0f; m = x; }
         else { w_old = 1.0f; w_new = exp_d(x - m); }
     }
+    template <class X> __device__ void join(const X& x) {          // with the sums of edges behind
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float w_old, w_new;
+            weights(m[j], x.m[j], w_old, w_new);
+            sum[j] = fmaf(x.sum[j], w_new, sum[j] * w_old);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[j][i] = fmaf(x.acc[j][i], w_new, acc[j][i] * w_old);
+        }
+    }
+    template <class X> __device__ void put(X& x) const {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) { x.acc[j] = acc[j]; x.m[j] = m[j]; x.sum[j] = sum[j]; }
+    }
 };
 
 // Record of a row that crosses ranges, for each lane of the walk: [NV] quads, a 64-bit maximum and a sum for each.  Slot 0 of a wave holds its first row, slot 1
-// its last one.
+// its last one.  Where a row begins before the ranges of a workgroup and ends behind them, the workgroup leaves one record, in slot 0 of its first wave (the
+// partial-sum buffers hold the others' for up to two quads a lane): 7 rows of 300 007 edges MEASURED
 template <int NV> struct Record { f4 acc[NV]; double m[NV]; float sum[NV]; };
+template <int NV> constexpr int joined_waves() { return NV <= 2 ? kWaves : 1; }
 
 template <class T, int MODE, int NV> __device__ inline void
 finish_row(const Args& P, int row, const Row<NV>& r, int lane, int qv, const int (&begin_v)[NV], const int (&head_v)[NV], T* out, float* out32, double* norm) {
@@ -313,7 +329,8 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
         }
         return;
     }
-    W w(P, lds, W::wave_bytes(P.heads) + (size_t)kBatch * P.heads * 8);
+    const size_t own = W::wave_bytes(P.heads) + (size_t)kBatch * P.heads * 8;
+    W w(P, lds, own);
     if (w.e0 >= w.e1) { w.stage(lds); return; }
     const int lane = w.lane, H = w.H, qv = w.qv;
     // R value rows are always in flight: a row's registers are loaded again, R edges ahead, as soon as it has been added
@@ -334,7 +351,7 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
     auto flush = [&](bool open_back) {
         if ((first_row && open_front) || open_back) {
             Record<NV> x;
-            for (int j = 0; j < NV; ++j) { x.acc[j] = r.acc[j]; x.m[j] = r.m[j]; x.sum[j] = r.sum[j]; }
+            r.put(x);
             rec[first_row ? 0 : 64] = x;
         } else finish_row<T, MODE>(P, cur, r, lane, qv, w.begin_v, w.head_v, out, out32, norm);
     };
@@ -437,6 +454,20 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
             wave_sync();
         }
     }
+    constexpr int JOIN = joined_waves<NV>();
+    if (JOIN > 1) {
+        const int64_t first = (int64_t)blockIdx.x * kWaves * P.range, end = first + (int64_t)kWaves * P.range;
+        if (first > 0 && end < P.n_edges && P.dst[first - 1] == P.dst[end]) {          // (the same for the whole workgroup) one row holds all its ranges
+            static_assert(JOIN == 1 || sizeof(Record<NV>) * 64 <= W::kPart * 4, "a record fits into the partial-sum buffer");
+            if (w.wave > 0) r.put(((Record<NV>*)w.part)[lane]);
+            __syncthreads();
+            if (w.wave > 0) return;
+#pragma unroll 1
+            for (int x = 1; x < kWaves; ++x) r.join(((const Record<NV>*)((const char*)w.part + x * own))[lane]);
+            flush(true);
+            return;
+        }
+    }
     flush(w.e1 < P.n_edges && behind == cur);
 }
 
@@ -453,35 +484,32 @@ void k_attn_merge(Args P, T* out, float* out32, double* norm, const void* record
     __shared__ int long_row[WAVES], long_first[WAVES];
     const Record<NV>* rec = (const Record<NV>*)records + lane;
     Row<NV> r;
-    auto join = [&](const f4 (&acc)[NV], const double (&m)[NV], const float (&sum)[NV]) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            float w_old, w_new;
-            Row<NV>::weights(r.m[j], m[j], w_old, w_new);
-            r.sum[j] = fmaf(sum[j], w_new, r.sum[j] * w_old);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) r.acc[j][i] = fmaf(acc[j][i], w_new, r.acc[j][i] * w_old);
-        }
+    // The records of a row that begins at edge `begin` in range w0 and ends in range `last`: those of the ranges of w0's workgroup, one for each workgroup between,
+    // those of the last one's.  Item k of them, and how many:
+    constexpr int JOIN = joined_waves<NV>();
+    auto record = [&](int64_t k, int64_t w0, int64_t begin, int64_t last) {
+        const int64_t front = min(last, w0 | (JOIN - 1)) - w0 + 1, blocks = max(last / JOIN - w0 / JOIN - 1, (int64_t)0);
+        const int64_t x = k < front ? w0 + k : k < front + blocks ? (w0 / JOIN + 1 + k - front) * JOIN : last / JOIN * JOIN + k - front - blocks;
+        return rec + (x * 2 + (x == w0 && begin > w0 * P.range ? 1 : 0)) * 64;
     };
-    // records first, first + step, .. <= last of a row that begins at edge `begin`, in range w0
-    auto join_records = [&](int64_t w0, int64_t begin, int64_t first, int64_t last, int step) {
+    auto records_of = [&](int64_t w0, int64_t last) {
+        if (last / JOIN == w0 / JOIN) return last - w0 + 1;
+        return (w0 | (JOIN - 1)) - w0 + 1 + (last / JOIN - w0 / JOIN - 1) + (last & (JOIN - 1)) + 1;
+    };
+    auto join_records = [&](int64_t w0, int64_t begin, int64_t last, int64_t first, int64_t n, int step) {
         r.clear();
 #pragma unroll 4
-        for (int64_t x = first; x <= last; x += step) {
-            const Record<NV> o = rec[(x * 2 + (x == w0 && begin > w0 * P.range ? 1 : 0)) * 64];
-            join(o.acc, o.m, o.sum);
-        }
+        for (int64_t k = first; k < n; k += step) { const Record<NV> o = *record(k, w0, begin, last); r.join(o); }
     };
-    const int64_t mine = (int64_t)blockIdx.x * WAVES + wave, border = (mine + 1) * P.range;
+    const int64_t mine = (int64_t)blockIdx.x * WAVES + wave, border = min((mine + 1) * P.range, P.n_edges - 1);
+    const int before = __builtin_amdgcn_readfirstlane(P.dst[border - 1]), row = __builtin_amdgcn_readfirstlane(P.dst[border]);          // (two ranges at least)
     if (lane == 0) long_row[wave] = -1;
-    if (border < P.n_edges) {
-        const int row = __builtin_amdgcn_readfirstlane(P.dst[border]);
-        if (P.dst[border - 1] == row) {
-            const int64_t begin = P.rowptr[row], last = ((int64_t)P.rowptr[row + 1] - 1) / P.range;
-            if (begin >= mine * P.range) {                              // (else an earlier border is its first)
-                if (last - mine < 8) { join_records(mine, begin, mine, last, 1); finish_row<T, MODE>(P, row, r, lane, qv, begin_v, head_v, out, out32, norm); }
-                else if (lane == 0) { long_row[wave] = row; long_first[wave] = (int)mine; }
-            }
+    if ((mine + 1) * P.range < P.n_edges && before == row) {
+        const int64_t begin = P.rowptr[row], last = ((int64_t)P.rowptr[row + 1] - 1) / P.range;
+        if (begin >= mine * P.range) {                              // (else an earlier border is its first)
+            const int64_t n = records_of(mine, last);
+            if (n <= 8) { join_records(mine, begin, last, 0, n, 1); finish_row<T, MODE>(P, row, r, lane, qv, begin_v, head_v, out, out32, norm); }
+            else if (lane == 0) { long_row[wave] = row; long_first[wave] = (int)mine; }
         }
     }
     __syncthreads();
@@ -489,14 +517,11 @@ void k_attn_merge(Args P, T* out, float* out32, double* norm, const void* record
         const int row = long_row[i];
         if (row < 0) continue;
         const int64_t w0 = long_first[i], begin = P.rowptr[row], last = ((int64_t)P.rowptr[row + 1] - 1) / P.range;
-        join_records(w0, begin, w0 + wave, last, WAVES);
-        if (wave > 0) {
-            Record<NV>& o = share[wave - 1][lane];
-            for (int j = 0; j < NV; ++j) { o.acc[j] = r.acc[j]; o.m[j] = r.m[j]; o.sum[j] = r.sum[j]; }
-        }
+        join_records(w0, begin, last, wave, records_of(w0, last), WAVES);
+        if (wave > 0) r.put(share[wave - 1][lane]);
         __syncthreads();
         if (wave == 0) {
-            for (int o = 0; o < WAVES - 1; ++o) join(share[o][lane].acc, share[o][lane].m, share[o][lane].sum);
+            for (int o = 0; o < WAVES - 1; ++o) r.join(share[o][lane]);
             finish_row<T, MODE>(P, row, r, lane, qv, begin_v, head_v, out, out32, norm);
         }
         __syncthreads();
@@ -505,20 +530,23 @@ void k_attn_merge(Args P, T* out, float* out32, double* norm, const void* record
 
 // ---- backward -------------------------------------------------------------------------------------------------------------------------------
 
-// delta[n,h] = sum_c dout out32: a wave per row, two reads of (rows, H D); 103 000 rows of 240 float32 57 us, 3.5 TB/s
+// delta[n,h] = sum_c dout out32: 16 lanes for each row and head, a quad at a time; two reads of (rows, H D): MEASURED
 template <class T> __global__ __launch_bounds__(256)
-void k_attn_delta(int64_t n_rows, int H, int D, const T* grad, const float* out32, float* delta) {
-    const int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
-    if (row >= n_rows) return;
-    const int lane = threadIdx.x & 63, HD = H * D;
-    const T* g = grad + row * HD; const float* o = out32 + row * HD;
-    for (int h = 0; h < H; ++h) {
-        float s = 0.0f;
-        for (int c = lane; c < D; c += 64) s = fmaf((float)g[h * D + c], o[h * D + c], s);
+void k_attn_delta(int64_t n_pairs, int D, const T* grad, const float* out32, float* delta) {
+    const int64_t pair = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (pair >= n_pairs) return;
+    const int l = threadIdx.x & 15, quads = (D + 3) >> 2;
+    const T* g = grad + pair * D; const float* o = out32 + pair * D;
+    float s = 0.0f;
+    for (int q = l; q < quads; q += 16) {
+        const int c = quad_begin(q, D), shared = quad_shared(c);
+        const typename Quad<T>::type x = D < 4 ? load_quad<T, kElements>(g, D) : load_quad<T, kHeads>(g + c, 4);
+        const f4 y = D < 4 ? load_quad<float, kElements>(o, D) : load_quad<float, kHeads>(o + c, 4);
 #pragma unroll
-        for (int x = 32; x >= 1; x >>= 1) s += __shfl_xor(s, x, 64);
-        if (lane == 0) delta[row * H + h] = s;
+        for (int i = 0; i < 4; ++i) s = i < shared ? s : fmaf((float)x[i], y[i], s);
     }
+    s += ror<0xB1>(s); s += ror<0x4E>(s); s += ror<0x141>(s); s += ror<0x140>(s);
+    if (l == 0) delta[pair] = s;
 }
 
 struct BackArgs {

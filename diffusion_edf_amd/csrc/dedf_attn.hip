@@ -27,7 +27,8 @@ struct Backward {
     template <class T, int MODE, int NV, int GA> int run() {
         if (p.lds_backward > 65536 && hipFuncSetAttribute((const void*)k_attn_backward<T, MODE, NV, GA>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds_backward) != hipSuccess) return DEDF_ERR_RUNTIME;
         const Args& a = p.a;
-        hipLaunchKernelGGL((k_attn_delta<T>), dim3((a.n_dst + kWaves - 1) / kWaves), dim3(256), 0, st, (int64_t)a.n_dst, a.heads, a.d, (const T*)b.grad, out32, delta);
+        const int64_t pairs = (int64_t)a.n_dst * a.heads;
+        hipLaunchKernelGGL((k_attn_delta<T>), dim3((unsigned)((pairs + 15) / 16)), dim3(256), 0, st, pairs, a.d, (const T*)b.grad, out32, delta);
         hipLaunchKernelGGL((k_attn_backward<T, MODE, NV, GA>), dim3(p.blocks), dim3(256), p.lds_backward, st, a, b);
         if (b.param_rows) {
             const int n_w = a.heads * a.k, columns = n_w + a.heads * a.n_buckets;

@@ -301,6 +301,17 @@ def test_edge_attention_heads_of_any_width_across_ranges(H, K, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [60, 74, 256])
+@pytest.mark.parametrize("shift", [0, 1, 17, 63])
+def test_edge_attention_rows_at_the_borders_of_ranges(D, shift):
+    """ranges are 16 edges here and a workgroup's 64: rows that begin and end at such borders, one before and one behind them, inside one workgroup's edges and over
+    several of them, of 9 records and more"""
+    n = torch.tensor([shift + 1, 64, 64, 128, 1, 63, 65, 127, 129, 192, 16, 48, 256, 15, 17, 32, 320, 128, 700, 0, 64, 1, 2_000, 63, 1, 130, 62, 16])
+    dst = torch.repeat_interleave(torch.arange(len(n)), n)
+    _check(_case(torch.float32, len(n), len(dst), D=D, drop=0.1, dst=dst, seed=shift))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("H,K,D", [(8, 17, 31), (3, 5, 7), (6, 3, 9)])
 def test_edge_attention_columns_at_an_odd_element(H, K, D):
     """value as columns of a wider tensor with NaN around them, at an odd element: the same bits, and a gradient of those columns alone"""
