@@ -571,6 +571,7 @@ void k_attn_backward(Args P, BackArgs B) {
     const int lane = w.lane, H = w.H, HD = w.HD, HK = w.HK, qv = w.qv, per_head = (P.d + 3) >> 2;
     float2* share = (float2*)w.keep;                    // [16][H] probability and dropout factor
     float* weight = (float*)w.t;                        // [16][H] their product
+    float* delta = weight + kBatch * H;                 // [16][H] the row's delta
     float* dt = (float*)(w.e_bucket + kBatch);          // [16][H]
     float* bins = dt + kBatch * H;                      // [buckets][H]
     for (int i = lane; i < BH; i += 64) bins[i] = 0.0f;
@@ -595,6 +596,17 @@ void k_attn_backward(Args P, BackArgs B) {
         typename W::Edge edge = w.request(w.e0), next = edge;
         typename W::Raw a[NA], a_next[NA], v[R][NV], up[R][NV];
         w.load_a(a_next, w.e0, (int)min((int64_t)kBatch, w.e1 - w.e0), 0);
+        // What the rows of the next group's first 64 edges and heads keep (of all of them for up to 4 heads), on its way before the last value rows of this one:
+        // loads return in order, so a load issued where it is used would wait for every row in flight.  499 979 bfloat16 edges of lmax 3 0.216 ms
+        // (loads where they are used 0.253)
+        struct Kept { d2 norm; float delta; } kept;
+        auto request_kept = [&](const typename W::Edge& x, int first, int n) {          // of a batch of x, its edges first .. first + n - 1
+            const int k = min(lane, n * H - 1), e = (int)((k * w.inv_h) >> 16);
+            const int64_t at = (int64_t)__shfl(x.dst, first + e) * H + k - e * H;
+            kept.norm = *(const d2*)(B.norm + 2 * at);
+            kept.delta = B.delta[at];
+        };
+        request_kept(edge, 0, (int)min((int64_t)GA, w.e1 - w.e0));
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             w.load_row(v[i], w.value_row(w.e0 + i));
@@ -612,24 +624,24 @@ void k_attn_backward(Args P, BackArgs B) {
                 if (g + GA < kBatch && g + GA < w.n) w.load_a(a_next, base, w.n, g + GA);
                 else if (base + kBatch < w.e1) w.load_a(a_next, base + kBatch, (int)min((int64_t)kBatch, w.e1 - base - kBatch), 0);
                 const int pairs = min(GA, w.n - g) * H;
-                // the first 64 of the group's edges and heads (all of them for up to 4 heads): what their rows keep, on its way early
-                d2 norm0 = {0.0, 0.0};
-                {
-                    const int k = min(lane, pairs - 1), e = (int)((k * w.inv_h) >> 16);
-                    norm0 = *(const d2*)(B.norm + 2 * ((int64_t)w.e_dst[g + e] * H + k - e * H));
-                }
                 w.partial_logits(a, g);
                 for (int idx = lane; idx < pairs; idx += 64) {
                     const int e = (int)((idx * w.inv_h) >> 16), h = idx - e * H, eb = g + e;
                     const double x = w.logit(g, e, h);
-                    const d2 at = idx == lane ? norm0 : *(const d2*)(B.norm + 2 * ((int64_t)w.e_dst[eb] * H + h));
+                    const int64_t row = (int64_t)w.e_dst[eb] * H + h;
+                    const d2 at = idx == lane ? kept.norm : *(const d2*)(B.norm + 2 * row);
                     const float p = x == -__builtin_inf() ? 0.0f : exp_d(x - at[0]) * (float)at[1], k = p == 0.0f ? 0.0f : w.dropped(base + eb, h);
                     share[eb * H + h] = float2{p, k};
                     weight[eb * H + h] = p * k;
+                    delta[eb * H + h] = idx == lane ? kept.delta : B.delta[row];
                 }
                 wave_sync();
 #pragma unroll 1
                 for (int s = g; s < g + GA && s < w.n; s += R) {
+                    if (s + R >= g + GA || s + R >= w.n) {
+                        if (g + GA < kBatch && g + GA < w.n) request_kept(edge, g + GA, min(GA, w.n - g - GA));
+                        else if (base + kBatch < w.e1) request_kept(next, 0, (int)min((int64_t)GA, w.e1 - base - kBatch));
+                    }
 #pragma unroll
                     for (int i = 0; i < R; ++i) {
                         if (s + i < w.n) {
@@ -660,7 +672,7 @@ void k_attn_backward(Args P, BackArgs B) {
                     auto write_dt = [&](int i, int h, float dot) {
                         const float2 f = share[(s + i) * H + h];
                         // (a masked edge's value may be NaN)
-                        dt[(s + i) * H + h] = f.x == 0.0f ? 0.0f : f.x * ((f.y == 0.0f ? 0.0f : f.y * dot) - B.delta[(int64_t)w.e_dst[s + i] * H + h]);
+                        dt[(s + i) * H + h] = f.x == 0.0f ? 0.0f : f.x * ((f.y == 0.0f ? 0.0f : f.y * dot) - delta[(s + i) * H + h]);
                     };
                     for (int k = lane >> lanes; k < last * H; k += 64 >> lanes) {
                         const int i = (int)((k * w.inv_h) >> 16), h = k - i * H, l = lane & ((1 << lanes) - 1);
