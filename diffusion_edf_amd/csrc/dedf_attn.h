@@ -593,29 +593,36 @@ void k_attn_backward(Args P, BackArgs B) {
     if (w.e0 >= w.e1) w.stage(lds);
     else {
         // value rows and the upper gradient at their destinations, R edges ahead; a batch's per-edge values and features one batch ahead
-        typename W::Edge edge = w.request(w.e0), next = edge;
+        // (destinations two batches ahead, so that they are there when this one asks for the next one's rows)
+        auto request_dst = [&](int64_t b) { return P.dst[min(b + (lane & (kBatch - 1)), w.e1 - 1)]; };
+        typename W::Edge edge = w.request(w.e0);
+        int dst_next = request_dst(w.e0 + kBatch);
         typename W::Raw a[NA], a_next[NA], v[R][NV], up[R][NV];
         w.load_a(a_next, w.e0, (int)min((int64_t)kBatch, w.e1 - w.e0), 0);
         // What the rows of the next group's first 64 edges and heads keep (of all of them for up to 4 heads), on its way before the last value rows of this one:
         // loads return in order, so a load issued where it is used would wait for every row in flight.  499 979 bfloat16 edges of lmax 3 0.216 ms
         // (loads where they are used 0.253)
         struct Kept { d2 norm; float delta; } kept;
-        auto request_kept = [&](const typename W::Edge& x, int first, int n) {          // of a batch of x, its edges first .. first + n - 1
+        auto request_kept = [&](int dst, int first, int n) {          // of a batch of these destinations, its edges first .. first + n - 1
             const int k = min(lane, n * H - 1), e = (int)((k * w.inv_h) >> 16);
-            const int64_t at = (int64_t)__shfl(x.dst, first + e) * H + k - e * H;
+            const int64_t at = (int64_t)__shfl(dst, first + e) * H + k - e * H;
             kept.norm = *(const d2*)(B.norm + 2 * at);
             kept.delta = B.delta[at];
         };
-        request_kept(edge, 0, (int)min((int64_t)GA, w.e1 - w.e0));
+        // waits for it: left to the head of a loop, the wait would be for the fewest loads that any way there has issued since, which is everything in flight
+        auto arrived = [](Kept& x) { double m = x.norm[0], z = x.norm[1]; asm volatile("" : "+v"(m), "+v"(z), "+v"(x.delta)); x.norm = d2{m, z}; };
+        request_kept(edge.dst, 0, (int)min((int64_t)GA, w.e1 - w.e0));
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             w.load_row(v[i], w.value_row(w.e0 + i));
             w.load_row(up[i], (const T*)B.grad + (int64_t)__builtin_amdgcn_readlane(edge.dst, i) * HD);
         }
         w.stage(lds);
+        arrived(kept);
         for (int64_t base = w.e0; base < w.e1; base += kBatch) {
             w.begin(base, edge);
-            next = w.request(min(base + kBatch, w.e1 - 1));
+            const typename W::Edge next = w.request(min(base + kBatch, w.e1 - 1));
+            const int dst_after = request_dst(base + 2 * kBatch);
             wave_sync();
 #pragma unroll 1
             for (int g = 0; g < kBatch && g < w.n; g += GA) {
@@ -625,22 +632,28 @@ void k_attn_backward(Args P, BackArgs B) {
                 else if (base + kBatch < w.e1) w.load_a(a_next, base + kBatch, (int)min((int64_t)kBatch, w.e1 - base - kBatch), 0);
                 const int pairs = min(GA, w.n - g) * H;
                 w.partial_logits(a, g);
+                arrived(kept);
+#pragma unroll 1
                 for (int idx = lane; idx < pairs; idx += 64) {
                     const int e = (int)((idx * w.inv_h) >> 16), h = idx - e * H, eb = g + e;
                     const double x = w.logit(g, e, h);
-                    const int64_t row = (int64_t)w.e_dst[eb] * H + h;
-                    const d2 at = idx == lane ? kept.norm : *(const d2*)(B.norm + 2 * row);
-                    const float p = x == -__builtin_inf() ? 0.0f : exp_d(x - at[0]) * (float)at[1], k = p == 0.0f ? 0.0f : w.dropped(base + eb, h);
+                    const float p = x == -__builtin_inf() ? 0.0f : exp_d(x - kept.norm[0]) * (float)kept.norm[1], k = p == 0.0f ? 0.0f : w.dropped(base + eb, h);
                     share[eb * H + h] = float2{p, k};
                     weight[eb * H + h] = p * k;
-                    delta[eb * H + h] = idx == lane ? kept.delta : B.delta[row];
+                    delta[eb * H + h] = kept.delta;
+                    if (idx + 64 < pairs) {
+                        const int e = (int)(((idx + 64) * w.inv_h) >> 16);
+                        const int64_t row = (int64_t)w.e_dst[g + e] * H + idx + 64 - e * H;
+                        kept = Kept{*(const d2*)(B.norm + 2 * row), B.delta[row]};
+                        arrived(kept);
+                    }
                 }
                 wave_sync();
 #pragma unroll 1
                 for (int s = g; s < g + GA && s < w.n; s += R) {
                     if (s + R >= g + GA || s + R >= w.n) {
-                        if (g + GA < kBatch && g + GA < w.n) request_kept(edge, g + GA, min(GA, w.n - g - GA));
-                        else if (base + kBatch < w.e1) request_kept(next, 0, (int)min((int64_t)GA, w.e1 - base - kBatch));
+                        if (g + GA < kBatch && g + GA < w.n) request_kept(edge.dst, g + GA, min(GA, w.n - g - GA));
+                        else if (base + kBatch < w.e1) request_kept(dst_next, 0, (int)min((int64_t)GA, w.e1 - base - kBatch));
                     }
 #pragma unroll
                     for (int i = 0; i < R; ++i) {
@@ -663,7 +676,7 @@ void k_attn_backward(Args P, BackArgs B) {
                                 }
                             }
                         }
-                        const int ahead = s + i + R, dst = ahead < kBatch ? __builtin_amdgcn_readlane(edge.dst, ahead) : __builtin_amdgcn_readlane(next.dst, ahead - kBatch);
+                        const int ahead = s + i + R, dst = ahead < kBatch ? __builtin_amdgcn_readlane(edge.dst, ahead) : __builtin_amdgcn_readlane(dst_next, ahead - kBatch);
                         w.load_row(v[i], w.value_row(base + ahead));
                         w.load_row(up[i], (const T*)B.grad + (int64_t)dst * HD);
                     }
@@ -717,7 +730,8 @@ void k_attn_backward(Args P, BackArgs B) {
                     for (int e = 0; e < GA && g + e < w.n; ++e) bins[w.e_bucket[g + e] * H + lane] += dt[(g + e) * H + lane];
                 wave_sync();
             }
-            edge = next;
+            edge = typename W::Edge{dst_next, next.logit, next.length};
+            dst_next = dst_after;
         }
     }
     if (!B.param_rows) return;
