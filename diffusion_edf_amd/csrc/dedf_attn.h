@@ -360,7 +360,8 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
     for (int64_t base = w.e0; base < w.e1; base += kBatch) {
         w.begin(base, edge);
         edge = w.request(min(base + kBatch, w.e1 - 1));
-        for (int g = 0; g < kBatch && g < w.n; g += GA) {
+        int g = 0;
+        do {          // (at least once: a load from before the loop has its later ones to count, and no wait for everything in flight)
             w.partial_logits(a, g);
             // the next features are on their way while this group is summed up
             if (g + GA < kBatch && g + GA < w.n) w.load_a(a, base, w.n, g + GA);
@@ -452,7 +453,7 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
                 w.load_row(v[i], w.value_row(base + g + e + R));
             }
             wave_sync();
-        }
+        } while ((g += GA) < kBatch && g < w.n);
     }
     constexpr int JOIN = joined_waves<NV>();
     if (JOIN > 1) {
@@ -624,8 +625,9 @@ void k_attn_backward(Args P, BackArgs B) {
             const typename W::Edge next = w.request(min(base + kBatch, w.e1 - 1));
             const int dst_after = request_dst(base + 2 * kBatch);
             wave_sync();
+            int g = 0;
 #pragma unroll 1
-            for (int g = 0; g < kBatch && g < w.n; g += GA) {
+            do {
 #pragma unroll
                 for (int i = 0; i < NA; ++i) a[i] = a_next[i];
                 if (g + GA < kBatch && g + GA < w.n) w.load_a(a_next, base, w.n, g + GA);
@@ -649,8 +651,9 @@ void k_attn_backward(Args P, BackArgs B) {
                     }
                 }
                 wave_sync();
+                int s = g;
 #pragma unroll 1
-                for (int s = g; s < g + GA && s < w.n; s += R) {
+                do {
                     if (s + R >= g + GA || s + R >= w.n) {
                         if (g + GA < kBatch && g + GA < w.n) request_kept(edge.dst, g + GA, min(GA, w.n - g - GA));
                         else if (base + kBatch < w.e1) request_kept(dst_next, 0, (int)min((int64_t)GA, w.e1 - base - kBatch));
@@ -697,7 +700,7 @@ void k_attn_backward(Args P, BackArgs B) {
                         if (l == 0) write_dt(i, h, dot);
                     }
                     wave_sync();
-                }
+                } while ((s += R) < g + GA && s < w.n);
                 if (B.dl && lane < GA && g + lane < w.n) {
                     float s = 0.0f;
                     for (int h = 0; h < H; ++h) s += dt[(g + lane) * H + h];
@@ -729,7 +732,7 @@ void k_attn_backward(Args P, BackArgs B) {
                 if (BH && B.param_rows && lane < H)          // in the edges' order: lane h alone adds to the sums of its head
                     for (int e = 0; e < GA && g + e < w.n; ++e) bins[w.e_bucket[g + e] * H + lane] += dt[(g + e) * H + lane];
                 wave_sync();
-            }
+            } while ((g += GA) < kBatch && g < w.n);
             edge = typename W::Edge{dst_next, next.logit, next.length};
             dst_next = dst_after;
         }
