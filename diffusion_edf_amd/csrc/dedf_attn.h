@@ -11,9 +11,9 @@
 //
 // Both directions stream the per-edge rows once, so memory bandwidth bounds them.  A wave owns a contiguous RANGE of edges whatever the rows are:
 // the load is even for any degree distribution, from one edge per row to one row with every edge.  It walks its range in batches of 16 edges; a lane
-// holds 4 consecutive channels (a "quad") of every row, 16 rows in flight.  Rows that lie inside a range are finished by its wave; a row that
-// crosses ranges leaves one record per range (running maximum, sum, weighted sum), which k_attn_merge joins in order: no atomics, and the result
-// depends on the sizes alone.  Logits and maxima are held in 64 bits (with masks of a type's lowest value in edge_logits, t loses s in 32), and M and Z
+// holds 4 consecutive channels of one head (a "quad") of every row, 8 rows in flight.  Rows that lie inside a range are finished by its wave; a row
+// that crosses ranges leaves one record per range, or per workgroup of ranges (running maximum, sum, weighted sum), which k_attn_merge joins in order: no
+// atomics, and the result depends on the sizes alone.  Logits and maxima are held in 64 bits (with masks of a type's lowest value in edge_logits, t loses s in 32), and M and Z
 // apart: beside such a mask log Z would be lost in 64.
 #pragma once
 #include "dedf_philox.h"
@@ -308,8 +308,8 @@ finish_row(const Args& P, int row, const Row<NV>& r, int lane, int qv, const int
 // Read of the per-edge rows once; bandwidth bounds it, in 16 bits nearly as much the 46 vector instructions of an edge.  1.97 M edges of 64 + 240 channels:
 // float32 0.57 ms (4.4 TB/s), float16 0.30 ms (4.2 TB/s), where a large copy reaches 4.8.  A logit's 16 products are summed per quad by the lanes that
 // loaded it and finished by one lane for each edge and head, which also draws the dropout word: the walk then needs one share per edge and lane.  (Running
-// maxima per edge and lane instead: 0.69 ms in float16.)  At lmax 3 (296 channels, 76 quads) a lane holds two quads, the second one mostly idle: 0.13 ms for
-// 499 979 edges, 2.7 TB/s, bound by instructions and by what 8 waves of a CU have in flight.
+// maxima per edge and lane instead: 0.69 ms in float16.)  At lmax 3 (296 channels, 76 quads) a lane holds two quads, the second one mostly idle: 0.124 ms for
+// 499 979 bfloat16 edges, 2.9 TB/s, vector instructions in half of all cycles (a fourth wave a SIMD and half the rows in flight: 0.127).
 template <class T, int MODE, int NV, int GA> __global__ __launch_bounds__(256, forward_waves(NV, sizeof(T)))
 void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, int64_t* rng_used) {
     typedef Wave<T, MODE, NV, GA> W;
@@ -558,8 +558,8 @@ struct BackArgs {
 };
 
 // Reads the per-edge rows once and writes their gradients; the rows of dout come from the caches, read again for each edge rather than kept while a row
-// lasts, so nothing waits where rows are short.  1.97 M edges of 64 + 240 float32 channels: 1.02 ms, 4.8 TB/s, the rate of a large copy; 499 979 bfloat16 edges
-// of lmax 3 0.25 ms, 2.9 TB/s, bound by the latency that three waves a SIMD cover.  The dot of a value row with dout goes through LDS (a partial sum for each
+// lasts, so nothing waits where rows are short.  1.97 M edges of 64 + 240 float32 channels: 1.01 ms, 4.8 TB/s, the rate of a large copy; 499 979 bfloat16 edges
+// of lmax 3 0.213 ms, 3.4 TB/s, bound by 135 vector instructions an edge (53 % of all cycles; with a fourth wave a SIMD, which spills, 0.25).  The dot of a value row with dout goes through LDS (a partial sum for each
 // quad part), since a head's quads are not a power of two of lanes.
 template <class T, int MODE, int NV, int GA> __global__ __launch_bounds__(256, backward_waves(NV, sizeof(T)))
 void k_attn_backward(Args P, BackArgs B) {
