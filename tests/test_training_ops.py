@@ -312,6 +312,13 @@ def test_edge_attention_rows_at_the_borders_of_ranges(D, shift):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,N,E", [(torch.float32, 2_500, 50_003), (torch.float32, 900, 98_304), (torch.float16, 3_000, 65_537), (torch.bfloat16, 40, 70_001)])
+def test_edge_attention_ranges_of_several_batches(dtype, N, E):
+    """more batches of 16 edges than waves, the last range short"""
+    _check(_case(dtype, N, E, H=2, K=4, D=8, drop=0.1, seed=E))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("H,K,D", [(8, 17, 31), (3, 5, 7), (6, 3, 9)])
 def test_edge_attention_columns_at_an_odd_element(H, K, D):
     """value as columns of a wider tensor with NaN around them, at an odd element: the same bits, and a gradient of those columns alone"""
