@@ -230,11 +230,10 @@ template <class T, int MODE, int NV, int GA> struct Wave {
         for (int i = 0; i < NA; ++i) {
             int e, q, h;
             if (!a_place(i, e_first, e, q)) continue;
-            const f4 wq = *(const f4*)(w + 4 * q);
-            f4 x;
+            f4 wq = *(const f4*)(w + 4 * q), x;
             const int begin = begin_a(q, h), shared = MODE == kAligned ? 0 : quad_shared(begin - h * K);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = j < shared ? 0.0f : act((float)a[i][j]);          // (0 where the head has no such element)
+            for (int j = 0; j < 4; ++j) { x[j] = j < shared ? 0.0f : act((float)a[i][j]); wq[j] = j < shared ? 0.0f : wq[j]; }          // (0 where the head has no such element)
             part[e * qa + q] = fmaf(x[3], wq[3], fmaf(x[2], wq[2], fmaf(x[1], wq[1], x[0] * wq[0])));
         }
         wave_sync();

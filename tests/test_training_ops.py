@@ -319,6 +319,20 @@ def test_edge_attention_ranges_of_several_batches(dtype, N, E):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("K", [6, 7, 8])
+def test_edge_attention_a_weight_of_minus_infinity(K):
+    """positive features and one weight of -inf, also where two quads hold it: logits of -inf, so that head takes no part anywhere and the other is as without it"""
+    c = _case(torch.float32, 5, 70, H=2, K=K, D=12, seed=K)
+    c["alpha"] = c["alpha"].abs() + 0.1
+    want, _ = _gpu(c, train=False)
+    for k in range(K):
+        dot = c["dot"].clone()
+        dot[0, k] = -float("inf")
+        out, _ = _gpu(dict(c, dot=dot), train=False)
+        assert not out[:, 0].any() and torch.equal(out[:, 1], want[:, 1])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("H,K,D", [(8, 17, 31), (3, 5, 7), (6, 3, 9)])
 def test_edge_attention_columns_at_an_odd_element(H, K, D):
     """value as columns of a wider tensor with NaN around them, at an odd element: the same bits, and a gradient of those columns alone"""
