@@ -367,21 +367,23 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
             else if (base + kBatch < w.e1) w.load_a(a, base + kBatch, (int)min((int64_t)kBatch, w.e1 - base - kBatch), 0);
             // A "piece" is what one row has in this group.  Shares are relative to a logit that every lane of a head agrees on: the group's largest, if it is
             // at most 24 above the smallest (shares of 4e-11 and more keep full precision for any values above 1e-27), else the piece's own largest.
+            // (8 heads of 32 + 77 channels, 400 000 bfloat16 edges, forward: 0.275 ms, with the pieces' own 0.291.)
             const uint32_t starts = (w.starts >> g) | 1u;
             const int live = min(GA, w.n - g);
             bool near = false;
-            uint64_t some = ~(uint64_t)0;          // bit 4 e: edge e takes part somewhere
+            constexpr int NH = 64 / GA;            // lanes for each edge
+            uint64_t some = ~(uint64_t)0;          // bit NH e: edge e takes part somewhere
             bool select = true;                    // an edge may take part in one head and not in another
-            if (GA == 16 && H <= 4) {
+            if (H <= NH) {
                 // one edge and head a lane: the largest and smallest logits of the group, through the wave
-                const int e = lane >> 2, h = lane & 3;
+                const int e = lane / NH, h = lane % NH;
                 const bool there = h < H;
                 const double x = there ? w.logit(g, e, h) : -__builtin_inf();
                 const bool in = e < live && x != -__builtin_inf();
                 float most = in ? (float)x : -__builtin_inff(), least = in ? (float)x : __builtin_inff();
-                most = fmaxf(most, ror<0x124>(most)); least = fminf(least, ror<0x124>(least));
-                most = fmaxf(most, ror<0x128>(most)); least = fminf(least, ror<0x128>(least));
-                most = fmaxf(most, __shfl_xor(most, 16)); least = fminf(least, __shfl_xor(least, 16));
+                if (NH <= 4) { most = fmaxf(most, ror<0x124>(most)); least = fminf(least, ror<0x124>(least)); }
+                if (NH <= 8) { most = fmaxf(most, ror<0x128>(most)); least = fminf(least, ror<0x128>(least)); }
+                if (NH <= 16) { most = fmaxf(most, __shfl_xor(most, 16)); least = fminf(least, __shfl_xor(least, 16)); }
                 most = fmaxf(most, __shfl_xor(most, 32)); least = fminf(least, __shfl_xor(least, 32));
                 near = __ballot(most != -__builtin_inff() && !(most - least <= 24.0f && fabsf(most) <= 1e6f)) == 0;
                 if (near) {
@@ -390,9 +392,11 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
                         share[(g + e) * H + h] = float2{p, in ? p * w.dropped(base + g + e, h) : 0.0f};
                         top[(g + e) * H + h] = (double)most;
                     }
-                    const uint64_t b = __ballot(in), all = __ballot(in || !there), heads = 0x1111111111111111ull;
-                    some = b | b >> 1 | b >> 2 | b >> 3;
-                    select = ((some ^ (all & all >> 1 & all >> 2 & all >> 3)) & heads) != 0;
+                    uint64_t all = __ballot(in || !there);
+                    some = __ballot(in);
+#pragma unroll
+                    for (int i = 1; i < NH; i *= 2) { some |= some >> i; all &= all >> i; }
+                    select = ((some ^ all) & ~(uint64_t)0 / (((uint64_t)1 << NH) - 1)) != 0;
                 } else if (there) w.t[(g + e) * H + h] = x;
             } else {
                 for (int idx = lane; idx < GA * H; idx += 64) {
@@ -435,7 +439,7 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
                             for (int c = 0; c < 4; ++c) r.acc[j][c] *= w_old;
                         }
                     }
-                    if (GA != 16 || (some >> ((4 * e) & 63)) & 1)
+                    if ((some >> (NH * e)) & 1)
 #pragma unroll
                     for (int j = 0; j < NV; ++j) {
                         const float2 f = share[(g + e) * H + w.head_v[j]];

@@ -333,6 +333,31 @@ def test_edge_attention_a_weight_of_minus_infinity(K):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,K,D", [(1, 16, 20), (2, 3, 2), (3, 5, 7), (8, 16, 30), (8, 20, 9), (16, 9, 8), (15, 17, 3), (16, 2, 64)])
+def test_edge_attention_masks_and_far_logits_with_any_heads(H, K, D):
+    """heads that see one and two edges a lane and more: masked edges of NaN and infinities, a bucket that is out for one head alone, logits that lie far apart side
+    by side, a NaN that reaches its own row and head only"""
+    c = _case(torch.float32, 6, 200, H=H, K=K, D=D, buckets=4, seed=H, drop=0.2)
+    dead = (torch.rand(200, generator=torch.Generator().manual_seed(1)) < 0.3) | (c["dst"] == 2) | (c["dst"] == 5)
+    c["logits"][dead] = -INF
+    clean_out, clean = _check(c)
+    c["alpha"][dead], c["value"][dead] = float("nan"), INF
+    out, grads = _gpu(c)
+    assert torch.equal(out, clean_out) and not out[2].any() and all(torch.equal(grads[k], clean[k]) for k in grads)
+    c = _case(torch.float32, 6, 200, H=H, K=K, D=D, buckets=4, seed=4)
+    c["table"][1, H - 1] = -INF
+    _check(c)
+    for gap in (20.0, 30.0, 1e4):
+        c = _case(torch.float32, 40, 400, H=H, K=K, D=D, seed=int(gap))
+        c["logits"] = c["logits"] - gap * (c["dst"] % 3).float()
+        _check(c)
+    c = _case(torch.float32, 8, 300, H=H, K=K, D=D, seed=9)
+    c["alpha"][int((c["dst"] == 4).nonzero()[3]), H // 2, K - 1] = float("nan")
+    bad = _gpu(c)[0].isnan()
+    assert bad[4, H // 2].all() and int(bad.sum()) == D
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("H,K,D", [(8, 17, 31), (3, 5, 7), (6, 3, 9)])
 def test_edge_attention_columns_at_an_odd_element(H, K, D):
     """value as columns of a wider tensor with NaN around them, at an odd element: the same bits, and a gradient of those columns alone"""
