@@ -28,8 +28,8 @@ constexpr int kBatch = 16;                 // edges per step of a wave
 constexpr int kWaves = 4;                  // waves per workgroup
 enum { kElements = 0, kHeads = 1, kAligned = 2 };          // how a row is cut into quads: see load_quad
 // Waves a SIMD holds, by the registers of each instantiation; a launch has as many waves as are resident at once, each with one range of edges.  More
-// waves than that run in two rounds, of which the second is half empty: 1.97 M edges, float32, a training pass with 2 048 waves
-// in the backward kernel 1.65 ms, with 3 072 1.83 ms.
+// waves than that run in two rounds, of which the second is half empty: 1.97 M edges, float32, a training pass with two waves a SIMD
+// in the backward kernel 1.65 ms, with three 1.83 ms.
 constexpr int forward_waves(int nv, int bytes) { return nv == 4 ? 2 : nv == 1 && bytes == 2 ? 4 : 3; }
 constexpr int backward_waves(int nv, int bytes) { return bytes == 2 && nv <= 2 ? 3 : 2; }          // (499 979 edges, lmax 3, bfloat16: 0.46 ms with 3, 0.52 with 2)
 constexpr float kActNorm = 1.531320475574866f;
