@@ -385,7 +385,9 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
                 if (NH <= 8) { most = fmaxf(most, ror<0x128>(most)); least = fminf(least, ror<0x128>(least)); }
                 if (NH <= 16) { most = fmaxf(most, __shfl_xor(most, 16)); least = fminf(least, __shfl_xor(least, 16)); }
                 most = fmaxf(most, __shfl_xor(most, 32)); least = fminf(least, __shfl_xor(least, 32));
-                near = __ballot(most != -__builtin_inff() && !(most - least <= 24.0f && fabsf(most) <= 1e6f)) == 0;
+                // (no edge of the head takes part: -inf and +inf.  Logits beyond float's range, as two masks of its lowest value make together, leave a difference of NaN
+                // or infinity: not near)
+                near = __ballot(!(most == -__builtin_inff() && least == __builtin_inff()) && !(most - least <= 24.0f && fabsf(most) <= 1e6f)) == 0;
                 if (near) {
                     const float p = in ? exp_d(x - (double)most) : 0.0f;
                     if (there) {

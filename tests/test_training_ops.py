@@ -15,6 +15,7 @@ from oracle import training_oracle as O
 
 U = 2.0 ** -24
 INF = float("inf")
+FMAX = torch.finfo(torch.float32).max
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
 LMAX2 = "64x0e+32x1e+16x2e"
 
@@ -422,6 +423,40 @@ def test_edge_attention_lowest_finite_masks(lowest):
     c["logits"][torch.rand(150, generator=torch.Generator().manual_seed(2)) < 0.4] = lowest
     c["logits"][c["dst"] == 3] = lowest
     _check(c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,K,D", [(1, 16, 20), (4, 16, 60), (3, 5, 7), (8, 16, 30), (16, 16, 8), (16, 9, 8), (15, 17, 3)])
+def test_edge_attention_lowest_masks_in_logits_and_bias(dtype, H, K, D):
+    """edge logits and a bucket's bias at float32's lowest value at once: their sum is finite in 64 bits alone.  Such edges get nothing beside others and equal shares
+    among themselves: one group of 16 edges inside a row, a row that is masked as a whole, single edges, the last batch, one head alone.  The largest values in
+    both places: such edges share their row alone"""
+    n = torch.tensor([48, 37, 3, 20, 16, 29])          # 153 edges: a last batch of 9
+    dst = torch.repeat_interleave(torch.arange(6), n)
+    for low, heads in ((-FMAX, slice(None)), (-FMAX, slice(H - 1, H)), (FMAX, slice(None)), (FMAX, slice(0, 1))):
+        c = _case(dtype, 6, len(dst), H=H, K=K, D=D, buckets=4, dst=dst, seed=H + K)
+        dead = torch.zeros(len(dst), dtype=torch.bool)
+        dead[16:32] = dead[48:85] = dead[90:92] = dead[144:] = True
+        c["length"] = torch.where(dead, torch.full_like(c["length"], 3.0), torch.where(c["length"] < 5, c["length"] / 2.5, c["length"]))          # (bucket 1: 2.5 to 5)
+        c["table"][1, heads] = low
+        c["logits"][dead] = low
+        _check(c)
+
+
+@pytest.mark.gpu
+def test_edge_attention_lowest_masks_in_logits_and_bias_across_ranges():
+    """the same where a wave walks several groups, rows cross ranges, and workgroups leave one record"""
+    low, E = -FMAX, 70_003
+    g = torch.Generator().manual_seed(5)
+    for N in (3, 900):
+        c = _case(torch.float32, N, E, H=2, K=4, D=8, buckets=4, dst=torch.randint(0, N, (E,), generator=g).sort().values, seed=N)
+        dead = (torch.arange(E) // 32 % 3 == 1) | (c["dst"] == 1)
+        dead[-7:] = True
+        c["length"] = torch.where(dead, torch.full_like(c["length"], 3.0), torch.where(c["length"] < 5, c["length"] / 2.5, c["length"]))
+        c["table"][1] = low
+        c["logits"][dead] = low
+        _check(c)
 
 
 @pytest.mark.gpu
