@@ -372,6 +372,7 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
             const int live = min(GA, w.n - g);
             bool near = false;
             constexpr int NH = 64 / GA;            // lanes for each edge
+            constexpr uint64_t kEdgeBits = ~(uint64_t)0 / (((uint64_t)1 << NH) - 1);          // bit NH e for every edge e
             uint64_t some = ~(uint64_t)0;          // bit NH e: edge e takes part somewhere
             bool select = true;                    // an edge may take part in one head and not in another
             if (H <= NH) {
@@ -390,15 +391,23 @@ void k_attn_forward(Args P, T* out, float* out32, double* norm, void* records, i
                 near = __ballot(!(most == -__builtin_inff() && least == __builtin_inff()) && !(most - least <= 24.0f && fabsf(most) <= 1e6f)) == 0;
                 if (near) {
                     const float p = in ? exp_d(x - (double)most) : 0.0f;
+                    uint64_t all = __ballot(in || !there);
+                    some = __ballot(in);
                     if (there) {
                         share[(g + e) * H + h] = float2{p, in ? p * w.dropped(base + g + e, h) : 0.0f};
                         top[(g + e) * H + h] = (double)most;
                     }
-                    uint64_t all = __ballot(in || !there);
-                    some = __ballot(in);
+                    // The walk reads this where a piece begins.  A piece of which no edge takes part leaves its row's maximum alone: the largest logit here is another
+                    // row's and may lie so far above this row's that the sum would end as zero.  Bits 0, NH, 2 NH ... of kEdgeBits: the piece's edges from e on
+                    if (there && ~all) {
+                        const uint32_t after = starts & ~((2u << e) - 1u);
+                        const int to = min(after ? __builtin_ctz(after) : GA, GA);
+                        const uint64_t piece = (kEdgeBits & ~(uint64_t)0 >> (64 - NH * (to - e))) << lane;
+                        if (!(some & piece)) top[(g + e) * H + h] = -__builtin_inf();
+                    }
 #pragma unroll
                     for (int i = 1; i < NH; i *= 2) { some |= some >> i; all &= all >> i; }
-                    select = ((some ^ all) & ~(uint64_t)0 / (((uint64_t)1 << NH) - 1)) != 0;
+                    select = ((some ^ all) & kEdgeBits) != 0;
                 } else if (there) w.t[(g + e) * H + h] = x;
             } else {
                 for (int idx = lane; idx < GA * H; idx += 64) {

@@ -358,6 +358,54 @@ def test_edge_attention_masks_and_far_logits_with_any_heads(H, K, D):
     assert bad[4, H // 2].all() and int(bad.sum()) == D
 
 
+def _masked_rows_beside_far_ones(c, gap, seed):
+    """every second row's logits `gap` below its neighbours', runs of up to 20 edges at -inf at most rows' ends, so that a group of edges holds nothing of a row
+    but masked edges, beside a row that lies far from it"""
+    g = torch.Generator().manual_seed(seed)
+    E, dst = len(c["dst"]), c["dst"]
+    c["logits"] = c["logits"] - gap * (dst % 2).float()
+    first = torch.searchsorted(dst, torch.arange(c["N"] + 1))
+    for n in range(c["N"]):
+        a, b = int(first[n]), int(first[n + 1])
+        for front in (True, False):
+            run = min(int(torch.randint(0, 21, (1,), generator=g)), max(b - a - 1, 0))
+            if front:
+                c["logits"][a:a + run] = -INF
+            else:
+                c["logits"][max(b - run, a):b] = -INF
+        if n % 7 == 3:
+            c["logits"][a:b] = -INF
+    return c
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gap", [60.0, 95.0, 120.0, 1e4])
+@pytest.mark.parametrize("H,K,D", [(1, 16, 20), (4, 16, 60), (3, 5, 7), (8, 16, 30), (16, 16, 8), (16, 9, 8), (15, 17, 3)])
+def test_edge_attention_masked_edges_beside_far_rows(H, K, D, gap):
+    """a row keeps its weight and gradients where its only edges in a group of 16, 8 or 4 are masked ones, in all heads or in one, next to a row whose logits lie
+    far above or below"""
+    g = torch.Generator().manual_seed(int(gap) + H)
+    n = torch.randint(3, 60, (24,), generator=g)
+    n[5] = 0
+    c = _case(torch.float32, 24, int(n.sum()), H=H, K=K, D=D, buckets=4, dst=torch.repeat_interleave(torch.arange(24), n), drop=0.1, seed=int(gap))
+    _check(_masked_rows_beside_far_ones(c, gap, H))
+    c = _case(torch.float32, 24, int(n.sum()), H=H, K=K, D=D, buckets=4, dst=c["dst"], seed=int(gap) + 1)
+    c["table"][1, H // 2] = -INF          # out for one head
+    c["length"] = torch.where(_masked_rows_beside_far_ones(dict(c, logits=torch.zeros(len(c["dst"]))), 0.0, H)["logits"] == -INF, torch.full_like(c["length"], 3.0), c["length"])
+    c["logits"] = c["logits"] - gap * (c["dst"] % 2).float()
+    _check(c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gap", [95.0, 1e4])
+def test_edge_attention_masked_edges_beside_far_rows_across_ranges(gap):
+    """the same with several batches a wave, and with records of rows that cross ranges"""
+    g = torch.Generator().manual_seed(int(gap))
+    for N, E in ((40, 9_001), (900, 70_003)):
+        c = _case(torch.float32, N, E, H=2, K=4, D=8, buckets=3, dst=torch.randint(0, N, (E,), generator=g).sort().values, seed=N)
+        _check(_masked_rows_beside_far_ones(c, gap, N))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("H,K,D", [(8, 17, 31), (3, 5, 7), (6, 3, 9)])
 def test_edge_attention_columns_at_an_odd_element(H, K, D):
