@@ -549,20 +549,20 @@ void k_attn_merge(Args P, T* out, float* out32, double* norm, const void* record
 // 240 float32 36 us, 5.5 TB/s with what the caches still hold (a wave for each row, 64 lanes for a head of 60 channels: 57 us)
 template <class T> __global__ __launch_bounds__(256)
 void k_attn_delta(int64_t n_pairs, int D, const T* grad, const float* out32, float* delta) {
-    const int64_t pair = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (pair >= n_pairs) return;
     const int l = threadIdx.x & 15, quads = (D + 3) >> 2;
-    const T* g = grad + pair * D; const float* o = out32 + pair * D;
-    float s = 0.0f;
-    for (int q = l; q < quads; q += 16) {
-        const int c = quad_begin(q, D), shared = quad_shared(c);
-        const typename Quad<T>::type x = D < 4 ? load_quad<T, kElements>(g, D) : load_quad<T, kHeads>(g + c, 4);
-        const f4 y = D < 4 ? load_quad<float, kElements>(o, D) : load_quad<float, kHeads>(o + c, 4);
+    for (int64_t pair = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); pair < n_pairs; pair += (int64_t)gridDim.x * 16) {          // (one each up to 2^27 pairs)
+        const T* g = grad + pair * D; const float* o = out32 + pair * D;
+        float s = 0.0f;
+        for (int q = l; q < quads; q += 16) {
+            const int c = quad_begin(q, D), shared = quad_shared(c);
+            const typename Quad<T>::type x = D < 4 ? load_quad<T, kElements>(g, D) : load_quad<T, kHeads>(g + c, 4);
+            const f4 y = D < 4 ? load_quad<float, kElements>(o, D) : load_quad<float, kHeads>(o + c, 4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s = i < shared ? s : fmaf((float)x[i], y[i], s);
+            for (int i = 0; i < 4; ++i) s = i < shared ? s : fmaf((float)x[i], y[i], s);
+        }
+        s += ror<0xB1>(s); s += ror<0x4E>(s); s += ror<0x141>(s); s += ror<0x140>(s);
+        if (l == 0) delta[pair] = s;
     }
-    s += ror<0xB1>(s); s += ror<0x4E>(s); s += ror<0x141>(s); s += ror<0x140>(s);
-    if (l == 0) delta[pair] = s;
 }
 
 struct BackArgs {

@@ -16,7 +16,7 @@ struct Forward {
     const Plan& p; void* out; float* out32; double* norm; int64_t* rng_used; void* records; hipStream_t st;
     template <class T, int MODE, int NV, int GA> int run() {
         if (p.lds_forward > 65536 && hipFuncSetAttribute((const void*)k_attn_forward<T, MODE, NV, GA>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds_forward) != hipSuccess) return DEDF_ERR_RUNTIME;
-        const int empty_blocks = (p.a.n_dst + 64 * kWaves - 1) / (64 * kWaves);
+        const int empty_blocks = (int)(((int64_t)p.a.n_dst + 64 * kWaves - 1) / (64 * kWaves));
         hipLaunchKernelGGL((k_attn_forward<T, MODE, NV, GA>), dim3(p.blocks + empty_blocks), dim3(256), p.lds_forward, st, p.a, (T*)out, out32, norm, records, rng_used);
         if (p.a.n_waves > 1) hipLaunchKernelGGL((k_attn_merge<T, MODE, NV>), dim3((p.a.n_waves - 1 + merge_waves<NV>() - 1) / merge_waves<NV>()), dim3(1024 / NV), 0, st, p.a, (T*)out, out32, norm, (const void*)records);
         return hipGetLastError() == hipSuccess ? DEDF_OK : DEDF_ERR_RUNTIME;
@@ -27,8 +27,8 @@ struct Backward {
     template <class T, int MODE, int NV, int GA> int run() {
         if (p.lds_backward > 65536 && hipFuncSetAttribute((const void*)k_attn_backward<T, MODE, NV, GA>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds_backward) != hipSuccess) return DEDF_ERR_RUNTIME;
         const Args& a = p.a;
-        const int64_t pairs = (int64_t)a.n_dst * a.heads;
-        hipLaunchKernelGGL((k_attn_delta<T>), dim3((unsigned)((pairs + 15) / 16)), dim3(256), 0, st, pairs, a.d, (const T*)b.grad, out32, delta);
+        const int64_t pairs = (int64_t)a.n_dst * a.heads;          // (a launch has fewer than 2^32 threads: 16 a pair pass that at 2^28 pairs)
+        hipLaunchKernelGGL((k_attn_delta<T>), dim3((unsigned)std::min<int64_t>((pairs + 15) / 16, 1 << 23)), dim3(256), 0, st, pairs, a.d, (const T*)b.grad, out32, delta);
         hipLaunchKernelGGL((k_attn_backward<T, MODE, NV, GA>), dim3(p.blocks), dim3(256), p.lds_backward, st, a, b);
         if (b.param_rows) {
             const int n_w = a.heads * a.k, columns = n_w + a.heads * a.n_buckets;

@@ -567,6 +567,25 @@ def test_edge_attention_offsets_past_32_bits():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("N,H", [(67_200_000, 4), (2 ** 31 - 2, 1)])
+def test_edge_attention_rows_up_to_the_limit(N, H):
+    """more rows and heads than a launch has threads for at 16 each, and as many rows as there may be, nearly all of them empty"""
+    dst = torch.tensor([0, 0, N // 2, N - 257, N - 1, N - 1, N - 1], device="cuda")
+    value = torch.arange(1, 8, dtype=torch.float16, device="cuda")[:, None, None].expand(7, H, 1).contiguous().requires_grad_(True)
+    logits = torch.zeros(7, device="cuda", requires_grad=True)
+    out = edge_attention(torch.zeros(7, H, 1, dtype=torch.float16, device="cuda"), value, torch.ones(H, 1, device="cuda"), EdgeSegments(dst, N), edge_logits=logits)
+    want = {0: 1.5, N // 2: 3.0, N - 257: 4.0, N - 1: 6.0}
+    o = out.detach()
+    assert {r: float(o[r, H - 1, 0]) for r in want} == want and int(o.count_nonzero()) == 4 * H and float(o.sum(dtype=torch.float64)) == 14.5 * H
+    up = torch.ones_like(out)
+    dv, dl = torch.autograd.grad(out, [value, logits], up)
+    half = torch.tensor([0.5, 0.5, 1, 1, 1 / 3, 1 / 3, 1 / 3], dtype=torch.float64)
+    close(dv[:, H - 1, 0], half, 4 * U, "d_value")
+    # dt = p (v - out): 16 roundings of terms up to 7
+    close(dl, H * half * (torch.arange(1.0, 8.0, dtype=torch.float64) - torch.tensor([1.5, 1.5, 3, 4, 6, 6, 6], dtype=torch.float64)), 16 * 7 * H * U, "d_logits")
+
+
+@pytest.mark.gpu
 def test_edge_attention_repeats_bit_for_bit_and_draws_by_the_offset():
     c = _case(torch.float32, 300, 5_000, buckets=8, drop=0.25, seed=1)
     out, grads = _gpu(c)
