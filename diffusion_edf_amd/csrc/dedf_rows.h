@@ -318,14 +318,15 @@ template <class T, int NQ, bool FAST, int WPR> __global__ __launch_bounds__(256,
     f4 pw[NQ], pb[NQ], nw[NQ], nb[NQ], gate[NQ];
     if (P.post_w) { R.spread(pw, P.post_w, P.s.channels); R.spread(pb, P.post_b, P.s.scalars); }
     if (P.z) { R.spread(nw, P.next_w, P.s.channels); R.spread(nb, P.next_b, P.s.scalars); }
-    const int units = P.groups * P.slices, group_rows = P.n_rows / P.groups;
-    for (int u = blockIdx.x * TEAMS + team; u < units; u += gridDim.x * TEAMS) {
-        const int g = u / P.slices, first = (u - g * P.slices) * P.slice_rows, last = min(first + P.slice_rows, group_rows);
+    // (unsigned: the step behind the last unit and the end of a group's last slice pass 2^31)
+    const uint32_t slices = P.slices, slice_rows = P.slice_rows, units = P.groups * slices, group_rows = P.n_rows / P.groups;
+    for (uint32_t u = blockIdx.x * TEAMS + team; u < units; u += gridDim.x * TEAMS) {
+        const uint32_t g = u / slices, first = (u - g * slices) * slice_rows, last = min(first + slice_rows, group_rows);
 #pragma unroll
         for (int j = 0; j < NQ; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) gate[j][i] = P.scale * (P.gate ? gate_at<T>(P.gate, P.gate_f32, (int64_t)g * P.s.channels + R.channel[j][i]) : 1.0f);
-        for (int k = first; k < last; ++k) {
+        for (uint32_t k = first; k < last; ++k) {
             const int64_t row = (int64_t)g * group_rows + k;
             f4 h[NQ], y[NQ];
             R.load(h, P.x, row);
@@ -376,16 +377,17 @@ template <class T, int NQ, bool FAST, int WPR> __global__ __launch_bounds__(256,
     if (next) R.spread(nw, P.next_w, C);
 #pragma unroll
     for (int j = 0; j < NQ; ++j) d_pw[j] = d_pb[j] = d_nw[j] = d_nb[j] = d_gate[j] = f4{0, 0, 0, 0};
-    const int units = P.groups * P.slices, group_rows = P.n_rows / P.groups;
-    for (int u = blockIdx.x * TEAMS + team; u < units; u += gridDim.x * TEAMS) {
-        const int g = u / P.slices, slice = u - g * P.slices, first = slice * P.slice_rows, last = min(first + P.slice_rows, group_rows);
+    // (unsigned: as in the forward pass)
+    const uint32_t slices = P.slices, slice_rows = P.slice_rows, units = P.groups * slices, group_rows = P.n_rows / P.groups;
+    for (uint32_t u = blockIdx.x * TEAMS + team; u < units; u += gridDim.x * TEAMS) {
+        const uint32_t g = u / slices, first = (u - g * slices) * slice_rows, last = min(first + slice_rows, group_rows);
 #pragma unroll
         for (int j = 0; j < NQ; ++j) {
             if (P.n_params < 5) d_gate[j] = f4{0, 0, 0, 0};
 #pragma unroll
             for (int i = 0; i < 4; ++i) gate[j][i] = P.gate ? gate_at<T>(P.gate, P.gate_f32, (int64_t)g * C + R.channel[j][i]) : 1.0f;
         }
-        for (int k = first; k < last; ++k) {
+        for (uint32_t k = first; k < last; ++k) {
             const int64_t row = (int64_t)g * group_rows + k;
             f4 h[NQ], n[NQ], y[NQ], m[NQ], up[NQ];
             typename Rw::PerQuad ry;

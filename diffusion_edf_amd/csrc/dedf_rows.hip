@@ -48,10 +48,10 @@ int make_shape(int n_blocks, const int* mul, const int* degree, Shape& s, bool& 
 
 // groups of rows cut into slices until there is a unit for every wave
 void cut(Args& a, int waves) {
-    const int rows = a.n_rows / a.groups;
-    a.slices = std::max(1, std::min(rows, waves / a.groups));
-    a.slice_rows = (rows + a.slices - 1) / a.slices;
-    a.slices = (rows + a.slice_rows - 1) / a.slice_rows;
+    const int64_t rows = a.n_rows / a.groups;          // (sums of two counts pass 32 bits)
+    a.slices = (int)std::max<int64_t>(1, std::min<int64_t>(rows, waves / a.groups));
+    a.slice_rows = (int)((rows + a.slices - 1) / a.slices);
+    a.slices = (int)((rows + a.slice_rows - 1) / a.slice_rows);
 }
 int grid(const Args& a, int most) {
     const int teams = shared_rows(a.s.width) ? 1 : kWaves;
@@ -120,8 +120,9 @@ struct Dropout {
     template <class T, int NQ, bool FAST, int WPR> int run() {
         constexpr int teams = kWaves / WPR;
         Args b = a;
-        b.slice_rows = (a.n_rows + kDropoutBlocks * teams - 1) / (kDropoutBlocks * teams);
-        const int slices = (a.n_rows + b.slice_rows - 1) / b.slice_rows;
+        const int64_t rows = a.n_rows;
+        b.slice_rows = (int)((rows + kDropoutBlocks * teams - 1) / (kDropoutBlocks * teams));
+        const int slices = (int)((rows + b.slice_rows - 1) / b.slice_rows);
         hipLaunchKernelGGL((k_dropout<T, NQ, FAST, WPR>), dim3((slices + teams - 1) / teams), dim3(256), lds_bytes(a), st, b);
         return hipGetLastError() == hipSuccess ? DEDF_OK : DEDF_ERR_RUNTIME;
     }

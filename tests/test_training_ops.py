@@ -182,6 +182,16 @@ def test_c_entries_refuse_before_any_launch(built_lib):
     assert lib.dedf_channel_dropout(9, 6, 3, mul, degree, V(16), 0.5, V(16), V(16), None, None) == _lib.ERR_UNSUPPORTED
 
 
+def test_scratch_of_the_norms_at_the_largest_row_count(built_lib):
+    """what a workgroup leaves does not depend on the number of rows once there are enough of them, up to 2^31 - 1"""
+    def need(n, gates=0):
+        a = _lib.DedfNorm(type=1, n_rows=n, n_blocks=1, groups=gates or 1, mul=(C.c_int * 4)(1, 0, 0, 0), degree=(C.c_int * 4)(0, 0, 0, 0), x=16, y=16, gate=16 if gates else None, scale=1.0, eps=1e-5)
+        return built_lib.dedf_norm_scratch_bytes(C.byref(a))
+    some = need(2 ** 30)
+    assert 0 < some < 1 << 20
+    assert [need(2 ** 31 - k) for k in (1, 2, 4_095, 4_096, 8_193, 2 ** 20)] == [some] * 6 and need(2 ** 31 - 1, 2 ** 31 - 1) == some
+
+
 def test_modules_are_the_identity_in_eval_and_carry_the_reference_names():
     m = EquivariantDropout(LMAX2, 0.3).eval()
     x = torch.randn(3, 240)
@@ -835,6 +845,33 @@ def test_dropout_rate_and_independence():
     b = equivariant_dropout(x, "32x0e", 0.1, dropout_rng(7, 1)) == 0
     for share, want in ((a, 0.1), (b, 0.1), (a & b, 0.01), (a[1:] & a[:-1], 0.01), (a[:, 1:] & a[:, :-1], 0.01)):
         assert abs(float(share.double().mean()) - want) <= 6 * math.sqrt(want * (1 - want) / share.numel())
+
+
+@pytest.mark.gpu
+def test_row_operators_at_the_largest_row_count():
+    """2^31 - 1 rows of one channel: every row is written and read once, with a gate a row and with none; small whole numbers, so nothing rounds"""
+    R = 2 ** 31 - 1
+    rows = lambda n: torch.arange(n, dtype=torch.float16, device="cuda").repeat(R // n + 1)[:R, None]          # noqa: E731
+    x, y, up = rows(11), rows(7), rows(3)
+    gate = 1 + rows(5)
+    leaves = [t.requires_grad_(True) for t in (x, y, gate)]
+    h, _ = norm_gate_residual(x, y, "1x0e", scale=0.5, gate=gate)
+    dx, dy, dg = torch.autograd.grad(h, leaves, up)
+    with torch.no_grad():
+        assert torch.equal(h, x + 0.5 * gate * y)
+        del h
+        assert torch.equal(dx, up) and torch.equal(dy, 0.5 * gate * up) and torch.equal(dg, 0.5 * y * up)
+        del dx, dy, dg, gate, leaves
+    h, _ = norm_gate_residual(x, y, "1x0e", scale=0.5)
+    dx, dy = torch.autograd.grad(h, [x, y], up)
+    with torch.no_grad():
+        assert torch.equal(h, x + 0.5 * y) and torch.equal(dx, up) and torch.equal(dy, 0.5 * up)
+        del h, dx, dy
+        one = torch.ones(R, 1, dtype=torch.float16, device="cuda")
+        out = equivariant_dropout(one, "1x0e", 0.5, dropout_rng(5, 9))
+        assert bool(((out == 0) | (out == 2)).all()) and abs(float(out.sum(dtype=torch.float64)) / R - 1.0) < 6 * R ** -0.5          # (variance 1 a row)
+        for r in [*range(40), *range(R - 40, R)]:
+            assert float(out[r, 0]) == (2.0 if O.philox((r, 65536, 9, 0), (5, 0))[0] >= 2 ** 31 else 0.0), r
 
 
 @pytest.mark.gpu
