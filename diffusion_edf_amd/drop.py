@@ -3,11 +3,12 @@
 No mask is ever stored.  An operator keeps an element where its Philox4x32-10 word -- key: the seed, counter: the element's place and the offset -- is at
 least ``floor(p * 2**32)``, and its backward pass draws the same words again (``include/dedf.h`` lists the counters).  ``rng = [seed, offset]`` is an int64
 tensor on the device: the kernels read it there, so a captured graph draws a new mask in each replay if the program changes the offset in between.  Two
-calls with one ``rng`` draw the same words: give each call of a step an offset of its own (``EquivariantDropout``, ``EdgeAttention`` and ``NormGateResidual`` count theirs, from a seed that their state dicts do
-not hold; where a forward pass is run again for its activations, as in checkpointing, call the functions with an ``rng`` of your own, which such a run
-repeats)."""
+calls with one ``rng`` draw the same words: give each call of a step a seed or an offset of its own.  The modules (``EquivariantDropout``, ``EdgeAttention``, ``NormGateResidual``) have a seed
+each and count their calls (``DrawsMasks``); where a forward pass is run again for its activations, as in checkpointing, call the functions with an ``rng`` of your
+own, which such a run repeats."""
 from __future__ import annotations
 
+import copy
 import functools
 from typing import List, Optional, Tuple
 
@@ -56,18 +57,55 @@ def equivariant_dropout(x: torch.Tensor, irreps, p: float, rng: Optional[torch.T
     return _lib.ops().equivariant_dropout(x, row_shape(irreps).native, p, rng, current_stream(x))
 
 
-class EquivariantDropout(torch.nn.Module):
-    """reference ``equiformer/drop.py:76-96``: identity in eval.  ``rng`` (a buffer that is not saved) holds the seed and counts the training calls."""
+class DrawsMasks(torch.nn.Module):
+    """What the modules with dropout have in common: ``rng = [seed, offset]`` on the module's device, the offset counting its training calls.  Without a seed
+    every instance draws one from torch's generator, as its parameters' first values are drawn, so layers have masks of their own and ``torch.manual_seed`` repeats
+    them; ``deepcopy`` draws again.  A seed that was given stays, in copies too.  ``rng`` is in no state dict (the reference's have no such entry): a program that resumes where it stopped
+    saves and restores it beside them.  It is no buffer either: ``DistributedDataParallel`` would overwrite it on every rank with the first rank's; ranks that are to
+    drop different places seed torch differently, or each give a seed."""
 
-    def __init__(self, irreps, drop_prob: float, seed: int = 0):
+    def _start_masks(self, seed: Optional[int]) -> None:
+        self.seed_drawn = seed is None
+        self.rng = dropout_rng(_drawn_seed() if seed is None else seed, device="cpu")
+
+    def _rng_at(self, x: torch.Tensor) -> torch.Tensor:
+        if self.rng.device != x.device:
+            self.rng = self.rng.to(x.device)
+        return self.rng
+
+    def _apply(self, fn, recurse: bool = True):
+        super()._apply(fn, recurse)
+        moved = fn(self.rng)
+        if not (moved.is_meta or self.rng.is_meta):
+            moved.copy_(self.rng)          # (to_empty() makes memory without values)
+        self.rng = moved
+        return self
+
+    def __deepcopy__(self, memo):
+        twin = self.__class__.__new__(self.__class__)
+        memo[id(self)] = twin
+        twin.__setstate__(copy.deepcopy(self.__dict__, memo))
+        if twin.seed_drawn:
+            twin.rng[0] = _drawn_seed()
+        return twin
+
+
+def _drawn_seed() -> int:
+    return int(torch.empty((), dtype=torch.int64, device="cpu").random_())
+
+
+class EquivariantDropout(DrawsMasks):
+    """reference ``equiformer/drop.py:76-96``: identity in eval; masks as ``DrawsMasks`` has them"""
+
+    def __init__(self, irreps, drop_prob: float, seed: Optional[int] = None):
         super().__init__()
         self.irreps, self.drop_prob = irreps, float(drop_prob)
         row_shape(irreps)
-        self.register_buffer("rng", torch.tensor([seed, 0], dtype=torch.int64), persistent=False)
+        self._start_masks(seed)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if not self.training or self.drop_prob == 0.0:
             return x
-        out = equivariant_dropout(x, self.irreps, self.drop_prob, self.rng)
+        out = equivariant_dropout(x, self.irreps, self.drop_prob, self._rng_at(x))
         self.rng[1] += 1
         return out

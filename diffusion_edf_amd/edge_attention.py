@@ -10,7 +10,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from .drop import current_stream
+from .drop import DrawsMasks, current_stream
 
 
 class EdgeSegments:
@@ -61,25 +61,25 @@ def edge_attention(alpha: torch.Tensor, value: torch.Tensor, alpha_dot: torch.Te
                                      current_stream(value))
 
 
-class EdgeAttention(torch.nn.Module):
+class EdgeAttention(DrawsMasks):
     """``edge_attention`` with its parameters: ``alpha_dot`` ``(1, H, K)`` as in the reference's state dict (``graph_attention.py:139-214``) and, with
-    ``bias_boundaries``, ``bias_table`` (zero at the start); after ``half()`` they are used in float32 all the same.  Dropout in training only; ``rng`` holds the
-    seed and counts the training calls."""
+    ``bias_boundaries``, ``bias_table`` (zero at the start); after ``half()`` they are used in float32 all the same.  Dropout in training only, masks as
+    ``DrawsMasks`` has them."""
 
-    def __init__(self, num_heads: int, mul_alpha_head: int, alpha_drop: float = 0.0, bias_boundaries: Optional[Sequence[float]] = None, seed: int = 0):
+    def __init__(self, num_heads: int, mul_alpha_head: int, alpha_drop: float = 0.0, bias_boundaries: Optional[Sequence[float]] = None, seed: Optional[int] = None):
         super().__init__()
         self.alpha_drop = float(alpha_drop)
         bound = math.sqrt(6.0 / (num_heads + mul_alpha_head))
         self.alpha_dot = torch.nn.Parameter(torch.empty(1, num_heads, mul_alpha_head).uniform_(-bound, bound))
         self.register_buffer("bias_boundaries", None if bias_boundaries is None else torch.as_tensor(bias_boundaries, dtype=torch.float32))
         self.bias_table = None if bias_boundaries is None else torch.nn.Parameter(torch.zeros(len(self.bias_boundaries) + 1, num_heads))
-        self.register_buffer("rng", torch.tensor([seed, 0], dtype=torch.int64), persistent=False)
+        self._start_masks(seed)
 
     def forward(self, alpha: torch.Tensor, value: torch.Tensor, segments: EdgeSegments, edge_logits: Optional[torch.Tensor] = None,
                 edge_length: Optional[torch.Tensor] = None) -> torch.Tensor:
         p = self.alpha_drop if self.training else 0.0
         bias = {} if self.bias_table is None else {"edge_length": edge_length, "bias_boundaries": self.bias_boundaries.float(), "bias_table": self.bias_table.float()}
-        out = edge_attention(alpha, value, self.alpha_dot.float(), segments, edge_logits, dropout=p, rng=self.rng, **bias)
+        out = edge_attention(alpha, value, self.alpha_dot.float(), segments, edge_logits, dropout=p, rng=self._rng_at(value) if p > 0.0 else None, **bias)
         if p > 0.0:
             self.rng[1] += 1
         return out

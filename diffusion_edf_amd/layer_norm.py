@@ -8,7 +8,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .drop import current_stream, row_shape
+from .drop import DrawsMasks, current_stream, row_shape
 
 
 def norm_gate_residual(x: torch.Tensor, y: torch.Tensor, irreps, scale: float = 1.0, gate: Optional[torch.Tensor] = None,
@@ -45,21 +45,21 @@ class EquivariantLayerNormV2(torch.nn.Module):
         return equivariant_layer_norm(x, self.irreps, self.affine_weight.float(), self.affine_bias.float(), self.eps)          # (float32 after half() too)
 
 
-class NormGateResidual(torch.nn.Module):
+class NormGateResidual(DrawsMasks):
     """``norm_gate_residual`` with its parameters: ``post_norm`` and ``next_norm`` hold them under the names of ``EquivariantLayerNormV2``; either may be
-    left out.  Dropout in training only; ``rng`` holds the seed and counts the training calls."""
+    left out.  Dropout in training only, masks as ``DrawsMasks`` has them."""
 
-    def __init__(self, irreps, scale: float = 1.0, post_norm: bool = True, next_norm: bool = True, drop_prob: float = 0.0, eps: float = 1e-5, seed: int = 0):
+    def __init__(self, irreps, scale: float = 1.0, post_norm: bool = True, next_norm: bool = True, drop_prob: float = 0.0, eps: float = 1e-5, seed: Optional[int] = None):
         super().__init__()
         self.irreps, self.scale, self.drop_prob, self.eps = irreps, scale, float(drop_prob), eps
         self.post_norm = EquivariantLayerNormV2(irreps, eps) if post_norm else None
         self.next_norm = EquivariantLayerNormV2(irreps, eps) if next_norm else None
-        self.register_buffer("rng", torch.tensor([seed, 0], dtype=torch.int64), persistent=False)
+        self._start_masks(seed)
 
     def forward(self, x: torch.Tensor, y: torch.Tensor, gate: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
         p = self.drop_prob if self.training else 0.0
         affine = [None if n is None else t for n in (self.post_norm, self.next_norm) for t in ((None, None) if n is None else (n.affine_weight.float(), n.affine_bias.float()))]
-        out = norm_gate_residual(x, y, self.irreps, self.scale, gate, affine[0], affine[1], p, self.rng, affine[2], affine[3], self.eps)
+        out = norm_gate_residual(x, y, self.irreps, self.scale, gate, affine[0], affine[1], p, self._rng_at(x) if p > 0.0 else None, affine[2], affine[3], self.eps)
         if p > 0.0:
             self.rng[1] += 1
         return out

@@ -1,7 +1,10 @@
 """The training operators -- edge attention, the norms around a block, channel dropout -- against 64-bit restatements (oracle/training_oracle.py), and what
 they refuse.  Tolerances count roundings: u = 2^-24 is a float32 operation's, half a step of the type an output's own; each test says how many."""
+import copy
 import ctypes as C
 import math
+import os
+import socket
 
 import pytest
 import torch
@@ -200,6 +203,58 @@ def test_modules_are_the_identity_in_eval_and_carry_the_reference_names():
     assert EdgeAttention(4, 16, bias_boundaries=[1.0, 2.0]).bias_table.shape == (3, 4)
     assert {k: v.shape for k, v in EquivariantLayerNormV2(LMAX2).state_dict().items()} == {"affine_weight": (112,), "affine_bias": (64,)}
     assert set(NormGateResidual(LMAX2, post_norm=False).state_dict()) == {"next_norm.affine_weight", "next_norm.affine_bias"}
+
+
+MASKED = [lambda **kw: EquivariantDropout(LMAX2, 0.3, **kw), lambda **kw: EdgeAttention(4, 16, 0.1, **kw), lambda **kw: NormGateResidual(LMAX2, drop_prob=0.1, **kw)]
+
+
+@pytest.mark.parametrize("make", MASKED)
+def test_modules_have_masks_of_their_own(make):
+    """no seed: one drawn from torch's generator for every instance and every deepcopy; a given one: that, in copies too; casts and moves leave it"""
+    torch.manual_seed(3)
+    a, b = make(), make()
+    torch.manual_seed(3)
+    assert make().rng.tolist() == a.rng.tolist() and make().rng.tolist() == b.rng.tolist()
+    a.rng[1] = 7
+    c, d = copy.deepcopy(a), copy.deepcopy(torch.nn.Sequential(a, b))
+    assert len({int(m.rng[0]) for m in (a, b, c, d[0], d[1])}) == 5 and d[0].rng[1] == 7 and type(c) is type(a) and c.training
+    assert [(k, v.tolist()) for k, v in c.state_dict().items()] == [(k, v.tolist()) for k, v in a.state_dict().items()]
+    assert all(p.data_ptr() != q.data_ptr() for p, q in zip(a.parameters(), c.parameters()))
+    for seed in (0, -5, 2 ** 63 - 1):
+        e = make(seed=seed)
+        e.rng[1] = 4
+        assert copy.deepcopy(e).half().double().to_empty(device="cpu").rng.tolist() == [seed, 4]
+    with torch.device("meta"):
+        f = make(seed=9)
+    assert f.to_empty(device="cpu").rng.tolist() == [9, 0] and "rng" not in f.state_dict()
+
+
+def _ddp_worker(rank, port, q):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    torch.distributed.init_process_group("gloo", rank=rank, world_size=2)
+    drop = EquivariantDropout(LMAX2, 0.3, seed=11 + rank)
+    net = torch.nn.parallel.DistributedDataParallel(torch.nn.Sequential(torch.nn.Linear(240, 240), torch.nn.BatchNorm1d(240), drop).eval())
+    for _ in range(2):
+        net(torch.ones(3, 240)).sum().backward()
+    q.put((rank, drop.rng.tolist()))
+    torch.distributed.barrier()
+    torch.distributed.destroy_process_group()
+
+
+def test_data_parallel_ranks_keep_their_seeds():
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = torch.multiprocessing.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_ddp_worker, args=(r, port, q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    got = dict(q.get(timeout=120) for _ in procs)
+    for p in procs:
+        p.join(timeout=60)
+        assert p.exitcode == 0
+    assert got == {0: [11, 0], 1: [12, 0]}
 
 
 # ---- edge attention on the GPU ------------------------------------------------------------------------------------------------------------------
@@ -845,6 +900,24 @@ def test_dropout_rate_and_independence():
     b = equivariant_dropout(x, "32x0e", 0.1, dropout_rng(7, 1)) == 0
     for share, want in ((a, 0.1), (b, 0.1), (a & b, 0.01), (a[1:] & a[:-1], 0.01), (a[:, 1:] & a[:, :-1], 0.01)):
         assert abs(float(share.double().mean()) - want) <= 6 * math.sqrt(want * (1 - want) / share.numel())
+
+
+@pytest.mark.gpu
+def test_stacked_modules_drop_different_places():
+    """two layers of a network made with the defaults, and copies of one, drop independent channels and edges: both drop one of n places with probability p^2"""
+    x, p = torch.ones(4_000, 240, device="cuda"), 0.5
+    first = EquivariantDropout(LMAX2, p).cuda()
+    layers = [first, EquivariantDropout(LMAX2, p).cuda(), copy.deepcopy(first)]
+    dropped = [m(x)[:, :64] == 0 for m in layers]
+    residual = [NormGateResidual(LMAX2, post_norm=False, next_norm=False, drop_prob=p).cuda() for _ in range(2)]
+    dropped += [m(torch.zeros_like(x), x)[0][:, :64] == 0 for m in residual]
+    seg, alpha, value = EdgeSegments(torch.arange(64_000, device="cuda"), 64_000), torch.zeros(64_000, 4, 16, device="cuda"), torch.ones(64_000, 4, 4, device="cuda")
+    edges = [EdgeAttention(4, 16, p).cuda()(alpha, value, seg)[:, :, 0].reshape(4_000, 64) == 0 for _ in range(2)]
+    n = 4_000 * 64
+    for group in (dropped, edges):
+        for i, a in enumerate(group):
+            for b in group[:i]:
+                assert abs(float((a & b).sum()) / n - 0.25) < 6 * (0.25 * 0.75 / n) ** 0.5
 
 
 @pytest.mark.gpu
