@@ -3,6 +3,7 @@
 // go to the stream that the caller names (its current one); autograd runs a backward pass on the stream of its forward pass.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <c10/core/DeviceGuard.h>
 #include <cmath>
 #include <optional>
@@ -64,6 +65,12 @@ void check_dropout(double p, const Tensor& rng, const Tensor& x) {
     TORCH_CHECK_VALUE(rng.defined(), "dropout needs rng, an int64 tensor [seed, offset] (dropout_rng)");
     TORCH_CHECK_VALUE(rng.scalar_type() == at::kLong && has_shape(rng, {2}), "rng: int64 [seed, offset], got ", rng.scalar_type(), " ", rng.sizes());
     TORCH_CHECK_VALUE(rng.device() == x.device(), "rng on ", rng.device(), ", the features on ", x.device());
+}
+// What these calls would leave out without a word: the tangent of a forward-mode dual tensor, and themselves in a trace (they are no registered operators)
+void check_mode(const char* what, std::initializer_list<Tensor> all) {
+    for (const Tensor& t : all)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what, ": forward-mode derivatives are not supported");
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), what, " cannot be traced by torch.jit");
 }
 bool wants_grad(std::initializer_list<Tensor> all) {
     if (!at::GradMode::is_enabled()) return false;
@@ -180,6 +187,7 @@ Tensor edge_attention(const Tensor& alpha, const Tensor& value, const Tensor& do
     TORCH_CHECK_NOT_IMPLEMENTED(H <= 16 && H * K <= 256 && H * ((D + 3) / 4) <= 256 && (!table.defined() || (table.size(0) <= 1024 && table.numel() <= 2048)),
                                 "at most 16 heads, 256 attention features and 1024 value channels an edge (head widths rounded up to multiples of 4), 1024 buckets, 2048 bias entries");
     check_dropout(p, rng, value);
+    check_mode("edge_attention", {alpha, value, dot, logits, table});
     check_gpu("edge_attention", value, {alpha, dot, logits, length, bounds, table});
     TORCH_CHECK_VALUE(dst.device() == value.device(), "segments on ", dst.device(), ", the features on ", value.device());
     const Attn a{edge_rows(alpha), edge_rows(value), dot.contiguous(), whole(logits), whole(table), dst, rowptr, whole(length), whole(bounds), n_dst, p};
@@ -288,6 +296,7 @@ std::vector<Maybe> norm_gate_residual(const Tensor& x, const Maybe& y_, const Sh
     TORCH_CHECK_VALUE(y.defined() || next_w.defined(), "weight: float32 (", shape.channels, ",)");
     TORCH_CHECK_VALUE(eps >= 1e-30, "eps ", eps, ": at least 1e-30");
     check_dropout(p, rng, x);
+    check_mode("norm_gate_residual", {x, y, gate, post_w, post_b, next_w, next_b});
     check_gpu("norm_gate_residual", x, {y, gate, post_w, post_b, next_w, next_b});
     const Norm n{x.contiguous(), whole(y), whole(gate), post_w, post_b, next_w, next_b, scale, eps, p};
     rng = p > 0.0 ? rng.contiguous() : Tensor();
@@ -336,6 +345,7 @@ Tensor equivariant_dropout(const Tensor& x, const Shape& shape, double p, const 
     const Tensor rng = given(rng_);
     check_rows("x", x, shape);
     check_dropout(p, rng, x);
+    if (p > 0.0) check_mode("equivariant_dropout", {x});          // (else the result is x itself)
     check_gpu("equivariant_dropout", x, {});
     if (p == 0.0) return x;
     const Tensor in = x.contiguous(), words = rng.contiguous();

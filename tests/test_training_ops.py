@@ -185,6 +185,37 @@ def test_c_entries_refuse_before_any_launch(built_lib):
     assert lib.dedf_channel_dropout(9, 6, 3, mul, degree, V(16), 0.5, V(16), V(16), None, None) == _lib.ERR_UNSUPPORTED
 
 
+def _calls_without_gpu():
+    """each operator on its differentiable arguments, with what it takes beside them"""
+    seg, rng = _segments_without_gpu(6, 3), dropout_rng(1, device="cpu")
+    length, bounds = torch.rand(6), torch.linspace(0, 1, 4)
+    attention = lambda a, v, w, l, t: edge_attention(a, v, w, seg, l, length, bounds, t)          # noqa: E731
+    norm = lambda x, y, g, w, b, w2, b2: norm_gate_residual(x, y, LMAX2, gate=g, post_weight=w, post_bias=b, next_weight=w2, next_bias=b2)          # noqa: E731
+    w, b = torch.ones(112), torch.zeros(64)
+    yield attention, (torch.randn(6, 4, 16), torch.randn(6, 4, 60), torch.randn(4, 16), torch.zeros(6), torch.zeros(5, 4))
+    yield norm, (torch.randn(6, 240), torch.randn(6, 240), torch.ones(1, 112), w, b, w.clone(), b.clone())
+    yield lambda x: equivariant_dropout(x, LMAX2, 0.5, rng), (torch.randn(6, 240),)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_are_refused(grad):
+    """a dual tensor in any place, with and without gradients wanted: a refusal, not an output without its tangent"""
+    for call, args in _calls_without_gpu():
+        for i in range(len(args)):
+            with torch.autograd.forward_ad.dual_level():
+                with_dual = [torch.autograd.forward_ad.make_dual(t.clone(), torch.ones_like(t)) if i == k else t.clone().requires_grad_(grad) for k, t in enumerate(args)]
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(*with_dual)
+        with pytest.raises(RuntimeError, match="needs GPU tensors"):          # nothing is wrong but the device
+            call(*args)
+
+
+def test_tracing_is_refused():
+    for call, args in _calls_without_gpu():
+        with pytest.raises(NotImplementedError, match="traced"):
+            torch.jit.trace(lambda *a: call(*a), args)
+
+
 def test_scratch_of_the_norms_at_the_largest_row_count(built_lib):
     """what a workgroup leaves does not depend on the number of rows once there are enough of them, up to 2^31 - 1"""
     def need(n, gates=0):
