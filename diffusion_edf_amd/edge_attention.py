@@ -63,8 +63,8 @@ def edge_attention(alpha: torch.Tensor, value: torch.Tensor, alpha_dot: torch.Te
 
 class EdgeAttention(DrawsMasks):
     """``edge_attention`` with its parameters: ``alpha_dot`` ``(1, H, K)`` as in the reference's state dict (``graph_attention.py:139-214``) and, with
-    ``bias_boundaries``, ``bias_table`` (zero at the start); after ``half()`` they are used in float32 all the same.  Dropout in training only, masks as
-    ``DrawsMasks`` has them."""
+    ``bias_boundaries``, ``bias_table`` (zero at the start); after ``half()``, which rounds the parameters, they are used in float32 all the same, and the
+    boundaries stay as they were, in float32: an edge keeps its bucket.  Dropout in training only, masks as ``DrawsMasks`` has them."""
 
     def __init__(self, num_heads: int, mul_alpha_head: int, alpha_drop: float = 0.0, bias_boundaries: Optional[Sequence[float]] = None, seed: Optional[int] = None):
         super().__init__()
@@ -75,10 +75,17 @@ class EdgeAttention(DrawsMasks):
         self.bias_table = None if bias_boundaries is None else torch.nn.Parameter(torch.zeros(len(self.bias_boundaries) + 1, num_heads))
         self._start_masks(seed)
 
+    def _apply(self, fn, recurse: bool = True):
+        exact = self.bias_boundaries
+        super()._apply(fn, recurse)
+        if exact is not None and self.bias_boundaries.dtype != torch.float32:
+            self.bias_boundaries = exact.to(self.bias_boundaries.device)
+        return self
+
     def forward(self, alpha: torch.Tensor, value: torch.Tensor, segments: EdgeSegments, edge_logits: Optional[torch.Tensor] = None,
                 edge_length: Optional[torch.Tensor] = None) -> torch.Tensor:
         p = self.alpha_drop if self.training else 0.0
-        bias = {} if self.bias_table is None else {"edge_length": edge_length, "bias_boundaries": self.bias_boundaries.float(), "bias_table": self.bias_table.float()}
+        bias = {} if self.bias_table is None else {"edge_length": edge_length, "bias_boundaries": self.bias_boundaries, "bias_table": self.bias_table.float()}
         out = edge_attention(alpha, value, self.alpha_dot.float(), segments, edge_logits, dropout=p, rng=self._rng_at(value) if p > 0.0 else None, **bias)
         if p > 0.0:
             self.rng[1] += 1

@@ -260,6 +260,24 @@ def test_modules_have_masks_of_their_own(make):
     assert f.to_empty(device="cpu").rng.tolist() == [9, 0] and "rng" not in f.state_dict()
 
 
+@pytest.mark.parametrize("cast", ["half", "bfloat16", "double", "float"])
+def test_bucket_boundaries_survive_casts(cast):
+    """boundaries that no 16-bit type holds, two of which lie closer than its steps: the same float32 values after a cast, a move with one, a cast back, and in the
+    state dict"""
+    bounds = [0.1, 2.1, 19.99, 19.9901]
+    m = EdgeAttention(4, 16, bias_boundaries=bounds)
+    want = torch.tensor(bounds)
+    getattr(m, cast)()
+    assert m.alpha_dot.dtype == m.bias_table.dtype == getattr(torch, {"half": "float16", "double": "float64", "float": "float32"}.get(cast, cast))
+    assert m.bias_boundaries.dtype == torch.float32 and torch.equal(m.bias_boundaries, want) and torch.equal(m.state_dict()["bias_boundaries"], want)
+    net = torch.nn.Sequential(m).to("cpu", torch.float16).float()
+    assert torch.equal(net[0].bias_boundaries, want)
+    other = EdgeAttention(4, 16, bias_boundaries=[1.0, 2.0, 3.0, 4.0]).half()
+    other.load_state_dict(m.state_dict())
+    assert torch.equal(other.bias_boundaries, want) and other.bias_boundaries.dtype == torch.float32
+    assert EdgeAttention(4, 16).half().bias_boundaries is None
+
+
 def _ddp_worker(rank, port, q):
     os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
     torch.distributed.init_process_group("gloo", rank=rank, world_size=2)
@@ -1176,6 +1194,27 @@ def test_modules_in_half_precision():
     assert h.dtype == z.dtype == torch.float16
     (h.float().square().sum() + z.float().sum()).backward()
     assert all(p.grad is not None and p.grad.dtype == torch.float16 and bool(p.grad.isfinite().all()) for p in block.parameters())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cast", ["half", "bfloat16"])
+def test_edges_keep_their_buckets_in_half_precision(cast):
+    """lengths next to boundaries that a 16-bit type rounds past them: a table of one bias a bucket, which the cast holds exactly, tells which was taken"""
+    bounds = torch.tensor([0.1, 2.1, 19.99, 19.9901])
+    length = torch.cat([bounds, torch.nextafter(bounds, torch.zeros(4)), torch.nextafter(bounds, torch.full((4,), 99.0))])
+    m = EdgeAttention(1, 4, bias_boundaries=bounds)
+    with torch.no_grad():
+        m.bias_table.copy_(torch.arange(5.0)[:, None])
+    m = getattr(m.cuda(), cast)()
+    # one row of each edge beside one of the first bucket: its share is exp(bucket) / (exp(bucket) + 1)
+    n = len(length)
+    seg = EdgeSegments(torch.arange(n, device="cuda").repeat_interleave(2), n)
+    both = torch.stack([length, torch.zeros(n)], 1).flatten().cuda()
+    dtype = m.alpha_dot.dtype
+    value = torch.tensor([1.0, 0.0], dtype=dtype, device="cuda").repeat(n)[:, None, None]
+    share = m(torch.zeros(2 * n, 1, 4, dtype=dtype, device="cuda"), value, seg, edge_length=both)[:, 0, 0].detach().double().cpu()
+    bucket = (length[:, None] >= bounds[None, :]).sum(1).double()
+    close(share, torch.sigmoid(bucket), 16 * U, "share")          # (neighbouring buckets' shares lie 0.029 or more apart)
 
 
 @pytest.mark.gpu
