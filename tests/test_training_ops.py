@@ -1212,7 +1212,7 @@ def test_edges_keep_their_buckets_in_half_precision(cast):
     both = torch.stack([length, torch.zeros(n)], 1).flatten().cuda()
     dtype = m.alpha_dot.dtype
     value = torch.tensor([1.0, 0.0], dtype=dtype, device="cuda").repeat(n)[:, None, None]
-    share = m(torch.zeros(2 * n, 1, 4, dtype=dtype, device="cuda"), value, seg, edge_length=both)[:, 0, 0].detach().double().cpu()
+    share = m(torch.zeros(2 * n, 1, 4, dtype=dtype, device="cuda"), value, seg, edge_length=both)[:, 0, 0]
     bucket = (length[:, None] >= bounds[None, :]).sum(1).double()
     close(share, torch.sigmoid(bucket), 16 * U, "share")          # (neighbouring buckets' shares lie 0.029 or more apart)
 
