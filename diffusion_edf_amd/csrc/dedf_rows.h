@@ -530,13 +530,13 @@ template <class T> __global__ __launch_bounds__(1024) void k_row_sums(const floa
 
 // the same for many matrices of a few rows: a thread a sum
 template <class T> __global__ __launch_bounds__(256) void k_few_rows(const float* x, int rows, int columns, int64_t sums, T* narrow, float* wide) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= sums) return;
-    const int64_t m = i / columns;
-    const float* at = x + m * rows * columns + (i - m * columns);
-    double s = 0.0;
-    for (int r = 0; r < rows; ++r) s += (double)at[(int64_t)r * columns];
-    if (narrow) narrow[i] = (T)(float)s; else wide[i] = (float)s;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < sums; i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / columns;
+        const float* at = x + m * rows * columns + (i - m * columns);
+        double s = 0.0;
+        for (int r = 0; r < rows; ++r) s += (double)at[(int64_t)r * columns];
+        if (narrow) narrow[i] = (T)(float)s; else wide[i] = (float)s;
+    }
 }
 
 }  // namespace rows

@@ -184,8 +184,12 @@ int dedf_norm_gate_residual_backward(const dedf_norm* x, const void* grad_h, con
     if (rc != DEDF_OK) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const bool params = d_post_weight || d_post_bias || d_next_weight || d_next_bias;
-    if (a.n_rows == 0) {          // no row: the parameters' gradients are zero (a sum over no rows); the caller's gate gradient has no element
+    if (a.n_rows == 0) {          // no row: the parameters' gradients are zero (a sum over no rows), those of any number of gate rows too
         const int C = a.s.channels;
+        const int64_t sums = (int64_t)x->groups * C;
+        if (d_gate && sums > 0)          // (16-bit types share their zero)
+            hipLaunchKernelGGL(k_few_rows<_Float16>, dim3((unsigned)std::min<int64_t>((sums + 255) / 256, 1 << 20)), dim3(256), 0, st, (const float*)nullptr, 0, C, sums,
+                               a.gate_f32 ? nullptr : (_Float16*)d_gate, a.gate_f32 ? (float*)d_gate : nullptr);
         if (params) hipLaunchKernelGGL(k_row_sums<float>, dim3((4 * C + 15) / 16), dim3(1024), 0, st, (const float*)nullptr, 0, 4 * C, C,
                                        Outputs{{d_post_weight, d_post_bias, d_next_weight, d_next_bias, nullptr}, {C, a.s.scalars, C, a.s.scalars, 0}, {}});
         return hipGetLastError() == hipSuccess ? DEDF_OK : DEDF_ERR_RUNTIME;

@@ -287,8 +287,9 @@ std::vector<Maybe> norm_gate_residual(const Tensor& x, const Maybe& y_, const Sh
     check_rows("x", x, shape);
     TORCH_CHECK_VALUE(!y.defined() || (y.sizes() == x.sizes() && y.scalar_type() == x.scalar_type()), "y: ", x.scalar_type(), " ", x.sizes(), " like x");
     if (gate.defined()) {
-        TORCH_CHECK_VALUE(gate.dim() == 2 && gate.size(1) == shape.channels && gate.size(0) > 0 && x.size(0) > 0 && x.size(0) % gate.size(0) == 0, "gate: (G, ", shape.channels,
+        TORCH_CHECK_VALUE(gate.dim() == 2 && gate.size(1) == shape.channels && (x.size(0) == 0 || (gate.size(0) > 0 && x.size(0) % gate.size(0) == 0)), "gate: (G, ", shape.channels,
                           ") with G a divisor of ", x.size(0), " rows, got ", gate.sizes());
+        TORCH_CHECK_NOT_IMPLEMENTED(gate.size(0) < (int64_t{1} << 31), "gate: fewer than 2**31 rows");
         TORCH_CHECK_TYPE(gate.scalar_type() == x.scalar_type() || is_float(gate), "gate: ", x.scalar_type(), " or float32, got ", gate.scalar_type());
     }
     check_affine("post", post_w, post_b, shape);

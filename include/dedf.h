@@ -342,7 +342,7 @@ int dedf_edge_attention_backward(const dedf_edge_attn* a, const double* norm, co
 
 /* The norms around a block with what stands between them (gnn_block.py:164-218; EquivariantLayerNormV2, equiformer/layer_norm.py:91-156):
  *   u = post(y) (or y: no post_weight)     h = x + scale gate[group, channel] keep[row, channel] u     z = next(h) (if next_weight)
- * The n_rows rows fall into `groups` runs of n_rows / groups consecutive rows, one gate row each.  y == NULL: z = next(x) alone, h is not written.
+ * The n_rows rows fall into `groups` runs of n_rows / groups consecutive rows, one gate row each.  Without rows `groups` is any number.  y == NULL: z = next(x) alone, h is not written.
  * Irreps: up to 4 blocks mul[b] x degree[b], degrees ascending, at most 2048 components.  Weights: one float for each channel, biases: for each
  * channel of degree 0 (ignored without any). */
 typedef struct dedf_norm {

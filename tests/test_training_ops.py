@@ -1008,6 +1008,27 @@ def test_row_operators_without_rows():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("groups", [0, 1, 3, 5_000])
+def test_a_gate_on_no_rows(dtype, groups):
+    """an empty batch goes through with any gate, as it does without one; the gate's gradient is zero, in its own type"""
+    for gate_type in {dtype, torch.float32}:
+        c = {k: torch.zeros(0, 240, dtype=dtype, device="cuda", requires_grad=True) for k in "xy"}
+        gate = torch.ones(groups, 112, dtype=gate_type, device="cuda", requires_grad=True)
+        w, b = torch.ones(112, device="cuda", requires_grad=True), torch.zeros(64, device="cuda", requires_grad=True)
+        for _ in range(2):
+            junk = torch.full((groups * 112 + 1,), float("nan"), dtype=gate_type, device="cuda")          # (what the gradient's memory may hold before)
+            del junk
+            h, z = norm_gate_residual(c["x"], c["y"], LMAX2, gate=gate, post_weight=w, post_bias=b, next_weight=w, next_bias=b, dropout=0.3, rng=dropout_rng(1))
+            assert h.shape == z.shape == (0, 240) and h.dtype == dtype
+            grads = torch.autograd.grad(h.sum() + z.sum(), [c["x"], c["y"], gate, w, b])
+            assert [g.shape for g in grads] == [(0, 240), (0, 240), (groups, 112), (112,), (64,)] and grads[2].dtype == gate_type and not any(bool(g.any()) for g in grads)
+    block = NormGateResidual(LMAX2).cuda()
+    h, z = block(torch.zeros(0, 240, device="cuda"), torch.zeros(0, 240, device="cuda"), torch.nn.Parameter(torch.ones(1, 112, device="cuda")))
+    assert h.shape == z.shape == (0, 240)
+
+
+@pytest.mark.gpu
 def test_row_operators_views():
     """features as columns of a wider tensor, at an odd offset: read through a copy; misaligned contiguous storage: read in place"""
     c = _norm_case(torch.float16, LMAX2, 9, seed=6)
