@@ -92,8 +92,9 @@ __device__ inline int quad_shared(int begin) { return -begin & 3; }
 // LDS of one wave is written and read by its own lanes only: LDS operations of a wave complete in order, the compiler must keep that order
 __device__ inline void wave_sync() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
 
-// exp(x), x <= 0 (or -inf / NaN), to 1e-7 relative: the exponent is split into whole and fraction in 64 bits, so a long way below the maximum
-// loses nothing
+// exp(x) to 1e-7 relative, x = -inf and NaN too: the exponent is split into whole and fraction in 64 bits, so a long way below the maximum loses
+// nothing.  x is a logit less one that is at least the largest but for its rounding to float (0.03 at 1e6), or, in the backward pass, up to 24 above: no
+// result passes 1.04
 __device__ inline float exp_d(double x) {
     if (x < -150.0) return 0.0f;
     const double y = x * kLog2e, n = __builtin_rint(y);
@@ -573,7 +574,7 @@ struct BackArgs {
 
 // Reads the per-edge rows once and writes their gradients; the rows of dout come from the caches, read again for each edge rather than kept while a row
 // lasts, so nothing waits where rows are short.  1.97 M edges of 64 + 240 float32 channels: 1.01 ms, 4.8 TB/s, the rate of a large copy; 499 979 bfloat16 edges
-// of lmax 3 0.213 ms, 3.4 TB/s, bound by 135 vector instructions an edge (53 % of all cycles; with a fourth wave a SIMD, which spills, 0.25).  The dot of a value row with dout goes through LDS (a partial sum for each
+// of lmax 3 0.213 ms, 3.4 TB/s and 135 vector instructions an edge in 53 % of all cycles, neither unit full (with a fourth wave a SIMD, which spills, 0.25).  The dot of a value row with dout goes through LDS (a partial sum for each
 // quad part), since a head's quads are not a power of two of lanes.
 template <class T, int MODE, int NV, int GA> __global__ __launch_bounds__(256, backward_waves(NV, sizeof(T)))
 void k_attn_backward(Args P, BackArgs B) {

@@ -99,7 +99,7 @@ int make_plan(const dedf_edge_attn* x, bool backward, Plan& p, std::initializer_
     bool whole = a.k % 4 == 0 && a.d % 4 == 0 && whole_quads(a.a, a.a_stride, x->type) && whole_quads(a.v, a.v_stride, x->type);
     for (const void* t : tensors) whole = whole && whole_quads(t, 0, x->type);
     p.mode = whole ? kAligned : a.d >= 4 ? kHeads : kElements;
-    const int qa = row_quads(a.heads, a.k), qv = row_quads(a.heads, a.d);          // (qa <= 76: 16 heads, 256 channels)
+    const int qa = row_quads(a.heads, a.k), qv = row_quads(a.heads, a.d);          // (qa <= 75: 15 heads of 17)
     // as many edges a group as four feature quads a lane hold: with 8 heads of 3 + 33 channels (400 000 float32 edges, training) groups of 16 0.40 ms, of 8 0.43
     p.ga = qa > 64 ? 2 : qv > 128 || qa > 32 ? 4 : qa > 16 ? 8 : 16;
     p.nv = qv > 128 || p.ga == 2 ? 4 : qv > 64 || p.ga == 4 ? 2 : 1;

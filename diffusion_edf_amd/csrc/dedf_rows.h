@@ -87,8 +87,10 @@ __device__ inline float wave_sums4(const float (&v)[4], int lane) {
 __device__ inline void wave_sync() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
 
 // a lane's components of a row and where they belong.  FAST: blocks start on whole, aligned quads, so a quad has one degree and is one access.  WPR:
-// waves that share a row (1; 4, the whole workgroup, for rows over 512 components: one wave would have to spill its registers).  Lanes behind the row's end
-// repeat its last quad; they belong to no block and are not stored.
+// waves that share a row (1; 4, the whole workgroup, for rows over 512 components).  One wave with four quads a lane spills 329 registers in the backward kernel (bfloat16, two waves a
+// SIMD); with three, for up to 768 components, that kernel keeps its 246 and the forward one spills 121 at its four waves a SIMD: not timed.  Lanes behind the row's end repeat its last quad;
+// they belong to no block and are not stored.  Rows off whole quads are read element by element: 100 000 float32 rows of 33x0e+17x1e, post-norm to next norm, 65 us forward and
+// 142 backward, of 32x0e+16x1e 40 and 83 (bfloat16: 72 and 167, 36 and 82).
 template <class T, int NQ, bool FAST, int WPR> struct Row {
     typedef typename Quad<T>::type Raw;
     const Shape& s; int lane;             // of the row's WPR x 64
@@ -362,7 +364,8 @@ template <class T, int NQ, bool FAST, int WPR> __global__ __launch_bounds__(256,
 }
 
 // Reads x, y, dh, dz, writes dx, dy: 103 000 rows of 240 float32 in 149 us, 4.0 TB/s; 415 vector instructions a row at 4 waves a SIMD come next to the
-// memory.  Summing the four degrees with one value a lane (wave_sums4) instead of four chains, and choosing a degree's sum before its root: 218 us before.
+// memory.  16 384 rows of lmax 3 in float16 49 us, 1.2 TB/s: the two waves of a SIMD wait in half of their time, for a row's loads
+// and then for its sums, and vector instructions issue in 46 % of the cycles: latency.  Summing the four degrees with one value a lane (wave_sums4) instead of four chains, and choosing a degree's sum before its root: 218 us before.
 template <class T, int NQ, bool FAST, int WPR> __global__ __launch_bounds__(256, backward_waves(NQ)) void k_norm_backward(Args P) {
     extern __shared__ __align__(16) char lds[];
     typedef Row<T, NQ, FAST, WPR> Rw;
