@@ -681,6 +681,28 @@ def test_edge_attention_offsets_past_32_bits():
 
 
 @pytest.mark.gpu
+def test_edge_attention_edges_up_to_the_limit():
+    """2^31 - 1 edges, nearly all of them of one row: every one has its equal share, and the last ones, a row of their own, theirs"""
+    E = 2 ** 31 - 1
+    dst = torch.zeros(E, dtype=torch.int64, device="cuda")
+    dst[-5:] = 1
+    seg = EdgeSegments(dst, 2)
+    del dst
+    value = torch.ones(E, 1, 1, dtype=torch.bfloat16, device="cuda")
+    value[-5:, 0, 0] = torch.arange(1, 6, device="cuda").bfloat16()
+    value.requires_grad_(True)
+    alpha = torch.zeros(1, 1, 1, dtype=torch.bfloat16, device="cuda").expand(E, 1, 1)
+    out = edge_attention(alpha, value, torch.ones(1, 1, device="cuda"), seg)
+    # the sums of 2^31 ones: a range's 2^19 or so are whole numbers in float32, some thousand records are joined with one rounding each
+    close(out[:, 0, 0], torch.tensor([1.0, 3.0], dtype=torch.float64), 4_100 * U, "out")
+    g, = torch.autograd.grad(out, value, torch.ones_like(out))
+    close(g[-5:, 0, 0], torch.full((5,), 0.2, dtype=torch.float64), 8 * U, "d_value")
+    share = g[:-5, 0, 0]
+    assert bool((share == share[0]).all())
+    close(share[:1] * 2.0 ** 31, torch.full((1,), 2.0 ** 31 / (E - 5), dtype=torch.float64), 4_100 * U, "share")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("N,H", [(67_200_000, 4), (2 ** 31 - 2, 1)])
 def test_edge_attention_rows_up_to_the_limit(N, H):
     """more rows and heads than a launch has threads for at 16 each, and as many rows as there may be, nearly all of them empty"""
